@@ -386,9 +386,10 @@ def _act8_exact(s):
         for c in range(0, f, 32):
             b = x[:, c:c + 32]
             top = b.abs().amax(1, keepdim=True)
-            unit = torch.exp2(torch.ceil(torch.log2(top.clamp(min=1e-300) / 448)).clamp(min=-124))
+            m, e = torch.frexp(top.clamp(min=1e-300) / 448)  # a power of two itself has m = 1/2
+            unit = torch.exp2(torch.where(m > 0.5, e, e - 1).clamp(min=-124).double())
             v = b / unit
-            step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+            step = torch.exp2(torch.frexp(v.abs().clamp(min=2.0 ** -6))[1].double() - 4)
             out[:, c:c + 32] = torch.round(v / step) * step * unit
         return out
 
