@@ -810,6 +810,80 @@ int b200_attention_bwd(int bwd_dt, int num_seqs, int total_q, int total_k, const
 int b200_attention_status(int *status_out);
 
 /*
+ * ---- RMSNorm of every query and key head, with the rotation (a config's "QK Norm") --------------------------------
+ *
+ * y = R(pos) (w o x r) for every head's row x of head_dim values, r = rsqrt(mean(x^2) + eps), R the rotation of
+ * b200_rope (interleaved pairs, pos * theta^(-2i / head_dim)) with the angles formed in fp64, so that positions of
+ * millions keep their accuracy. X_q, out_q: [num_tokens][num_q_heads * head_dim]; X_k, out_k:
+ * [num_tokens][num_kv_heads * head_dim] (num_kv_heads may be 0, the key pointers are then ignored). q_weight, k_weight:
+ * [head_dim], shared by the query (key) heads; NULL means ones ("QK Norm Weight Type: none"). One rounding. out_q / out_k
+ * may be X_q / X_k themselves where no backward follows. head_dim a multiple of 8 up to 256, tensors 16-byte aligned,
+ * bf16 only. It stands where the reference submits rms_norm_noscale per head and rope (no fused counterpart there).
+ *
+ * Backward: dX_q, dX_k are overwritten (and may be d_out_q / d_out_k themselves). dq_weight, dk_weight [head_dim], either
+ * may be NULL: accumulate != 0 adds to them, 0 writes them. Their sums run in a fixed order (fp32 shares of the blocks in
+ * the workspace, then their sum): two runs give the same bits. The workspace is needed only for weight gradients;
+ * b200_qk_norm_rope_bwd_workspace_bytes(num_tokens, ...) covers every smaller number of tokens too.
+ */
+int b200_qk_norm_rope(int fwd_dt, int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, float eps, int theta,
+                      const int *seq_positions, const void *q_weight, const void *k_weight, const void *X_q, const void *X_k,
+                      void *out_q, void *out_k, void *stream);
+uint64_t b200_qk_norm_rope_bwd_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, int head_dim);
+int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, float eps, int theta,
+                          const int *seq_positions, const void *q_weight, const void *k_weight, const void *X_q, const void *X_k,
+                          const void *d_out_q, const void *d_out_k, void *dX_q, void *dX_k, void *dq_weight, void *dk_weight,
+                          int accumulate, uint64_t workspace_bytes, void *workspace, void *stream);
+
+/*
+ * ---- attention with a sliding window and sink tokens ------------------------------------------------------------------
+ *
+ * b200_attention_fwd / _bwd under another mask: the query at position p of its sequence (the last query stands at the
+ * last key) sees key j iff j <= p and (p - j < window or j < num_sinks). Tensors, head arguments and HOST sequence arrays
+ * as there; window >= 1, num_sinks >= 0; every query sees its own key, so no row is empty. Work and traffic follow the
+ * visible keys. The query ranges of the sequences must not overlap, nor, in the backward, their key ranges. Rows of
+ * x_attn_out, softmax_lse, dx_q, dx_k, dx_v outside every sequence are left as they were; a key that no query sees gets a
+ * zero gradient, and keys of a sequence that none of its queries sees, like rows outside the sequences, may hold anything.
+ * head_dim a multiple of 8 up to 256, tensors 16-byte aligned, bf16 only. The reference has no window: no counterpart.
+ *
+ * The forward needs no workspace. The backward's is sized by b200_attention_window_workspace_bytes(max_num_seqs, ...,
+ * max_total_q, num_sinks), which covers every smaller batch. dx_q / dx_k / dx_v are overwritten.
+ */
+uint64_t b200_attention_window_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int max_total_q,
+                                               int num_sinks);
+int b200_attention_window_fwd(int fwd_dt, int num_seqs, int total_q, int total_k, const int *q_seq_offsets, const int *q_seq_lens,
+                              const int *k_seq_offsets, const int *k_seq_lens, int num_q_heads, int num_kv_heads, int head_dim,
+                              const void *x_q, const void *x_k, const void *x_v, void *x_attn_out, float *softmax_lse, int window,
+                              int num_sinks, void *stream);
+int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, int total_k, const int *q_seq_offsets, const int *q_seq_lens,
+                              const int *k_seq_offsets, const int *k_seq_lens, int num_q_heads, int num_kv_heads, int head_dim,
+                              const void *x_q, const void *x_k, const void *x_v, const void *x_attn_out, const float *softmax_lse,
+                              const void *dx_out, void *dx_q, void *dx_k, void *dx_v, int window, int num_sinks,
+                              uint64_t workspaceBytes, void *workspace, void *stream);
+
+/*
+ * ---- SwiGLU activations held in 8 bits ------------------------------------------------------------------------------------
+ *
+ * x_w1 and x_w3 are held as e4m3 codes [n_rows][n_cols] and one byte per 32 columns of a row [n_rows][ceil(n_cols / 32)]
+ * (b200_act8_scales_bytes): value = code * 2^(byte - 127), the unit being the smallest power of two (2^-124 at least) that
+ * keeps the block within e4m3's 448. Values are rounded to nearest, ties to even; what a code stands for is exact in bf16.
+ * An infinity or NaN is held as NaN and does not touch the others of its block; numbers above 240 * 2^120 (3.19e38) are held
+ * as that, the largest multiple that bf16 has.
+ *
+ * b200_swiglu_act8: b200_swiglu (out = silu(x_w1) * x_w3; not formed when out is NULL) that also holds its inputs.
+ * b200_swiglu_recompute_act8: the held x_w1, x_w3 as bf16 and h = silu(x_w1) * x_w3 of them, each when not NULL.
+ * b200_swiglu_bwd_x_act8: b200_swiglu_bwd_x on the held values; out, when not NULL, receives h of them. dX_w1 or dX_w3 may be
+ * upstream_dX itself. n_cols a multiple of 8; bf16 tensors and codes 16-byte aligned. No counterpart in the reference, which
+ * keeps them in 16 bits or not at all.
+ */
+uint64_t b200_act8_scales_bytes(int n_rows, int n_cols);
+int b200_swiglu_act8(int fwd_dt, int n_rows, int n_cols, const void *x_w1, const void *x_w3, void *out, void *codes_w1, void *scales_w1,
+                     void *codes_w3, void *scales_w3, void *stream);
+int b200_swiglu_recompute_act8(int fwd_dt, int n_rows, int n_cols, const void *codes_w1, const void *scales_w1, const void *codes_w3,
+                               const void *scales_w3, void *x_w1, void *x_w3, void *out, void *stream);
+int b200_swiglu_bwd_x_act8(int bwd_dt, int n_rows, int n_cols, const void *codes_w1, const void *scales_w1, const void *codes_w3,
+                           const void *scales_w3, const void *upstream_dX, void *dX_w1, void *dX_w3, void *out, void *stream);
+
+/*
  * ---- a whole decoder block ---------------------------------------------------------------------------------------
  *
  * RMSNorm -> q / k / v projections -> RoPE -> causal attention -> output projection + residual -> RMSNorm -> MoE

@@ -90,6 +90,18 @@ SIGNATURES = {
     "b200_transformer_block_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_scatter_row_weights": (_i, [_i, _i, _vp, _vp, _vp, _vp]),
     "b200_gather_router_grad": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "b200_qk_norm_rope": (_i, [_i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200_qk_norm_rope_bwd_workspace_bytes": (_u64, [_i, _i, _i, _i]),
+    "b200_qk_norm_rope_bwd": (_i, [_i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i,
+                                   _u64, _vp, _vp]),
+    "b200_attention_window_workspace_bytes": (_u64, [_i, _i, _i, _i, _i, _i]),
+    "b200_attention_window_fwd": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "b200_attention_window_bwd": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                       _vp, _i, _i, _u64, _vp, _vp]),
+    "b200_act8_scales_bytes": (_u64, [_i, _i]),
+    "b200_swiglu_act8": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200_swiglu_recompute_act8": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200_swiglu_bwd_x_act8": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 
