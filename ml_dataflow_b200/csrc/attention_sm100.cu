@@ -19,6 +19,7 @@
 #include <math.h>
 #include <stddef.h>
 
+#include "attention_sm100.cuh"
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 #include "../../include/b200_moe.h"
@@ -67,25 +68,6 @@ template <int HD>
 constexpr size_t fwd_smem_bytes() {
   // Q tiles, P tiles, the K / V ring, bookkeeping, and the slack that aligns the tiles to 1024 bytes
   return 1024 + (size_t)QT * BM * HD * 2 + (size_t)QT * BM * BN * 2 + (size_t)KV_SLOTS * BN * HD * 2 + sizeof(FwdTail);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// shared-memory accesses by 32-bit shared address (kept in program order among themselves)
-__device__ __forceinline__ float4 lds128(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ void sts128(uint32_t addr, const uint4 &v) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-__device__ __forceinline__ void sts32(uint32_t addr, float v) {
-  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 template <int HD>
@@ -760,43 +742,7 @@ __global__ void __launch_bounds__(256) attn_round_kernel(int64_t n8, const float
 // ---------------------------------------------------------------------------------------
 using namespace b200;
 
-namespace {
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void *sym = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    fn = reinterpret_cast<EncodeTiledFn>(sym);
-  }
-  return fn;
-}
-
-// bf16 [rows][cols] with a row pitch of `cols` elements; boxes of 64 columns x 128 rows, 128-byte swizzle, rows past
-// the end read as zeros
-int rows_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t cols) {
-  EncodeTiledFn fn = encode_fn();
-  B200_REQUIRE(fn != nullptr, "attention: cuTensorMapEncodeTiled is not available from this driver");
-  B200_REQUIRE(b200_aligned16(base) && (cols * 2) % 16 == 0, "attention: tensors must be 16-byte aligned with a 16-byte row pitch");
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {cols * 2};
-  cuuint32_t box[2] = {64, 128};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  B200_REQUIRE(r == CUDA_SUCCESS, "attention: cuTensorMapEncodeTiled failed with code %d", (int)r);
-  return 0;
-}
-
-constexpr int MAX_DEVICES = 64;
+namespace b200 {
 
 int *attn_status_ptr() {
   static int *ptr[MAX_DEVICES];
@@ -805,6 +751,10 @@ int *attn_status_ptr() {
   if (!ptr[dev] && cudaGetSymbolAddress((void **)&ptr[dev], fa::g_attn_status) != cudaSuccess) ptr[dev] = nullptr;
   return ptr[dev];
 }
+
+}  // namespace b200
+
+namespace {
 
 template <int HD>
 int launch_fwd(const fa::FwdParams &p, int units, int num_q_heads, cudaStream_t s) {

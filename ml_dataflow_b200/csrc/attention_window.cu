@@ -12,6 +12,7 @@
 // every sum has a fixed order: two runs give the same bits.
 #include <math.h>
 
+#include "attention_window.cuh"
 #include "common.cuh"
 #include "../../include/b200_moe.h"
 
@@ -21,13 +22,6 @@ namespace window {
 constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int MAX_HEAD_DIM = 256;
 constexpr float LOG2E = 1.4426950408889634f;
-
-// sequences of one launch; first[s]: their query rows (or keys) numbered through
-constexpr int MAX_SEQS = 48;
-struct SeqTable {
-  int n;
-  int q_off[MAX_SEQS], Tq[MAX_SEQS], k_off[MAX_SEQS], Tk[MAX_SEQS], first[MAX_SEQS + 1];
-};
 
 struct Params {
   SeqTable seqs;
@@ -255,45 +249,84 @@ int window_check(const char *op, int dt, int num_seqs, int total_q, int total_k,
   return disjoint(op, "query", num_seqs, q_off, q_len);
 }
 
-// the next sequences that have work, at most MAX_SEQS; rows_of gives a sequence's number of rows
-template <typename F>
-int next_sequences(window::SeqTable &t, int *next, int num_seqs, const int *q_off, const int *q_len, const int *k_off, const int *k_len,
-                   F rows_of) {
-  t.n = 0;
-  t.first[0] = 0;
-  int64_t rows = 0;
-  while (*next < num_seqs && t.n < window::MAX_SEQS) {
-    const int s = (*next)++;
-    if (rows_of(s) == 0) continue;
-    t.q_off[t.n] = q_off[s];
-    t.Tq[t.n] = q_len[s];
-    t.k_off[t.n] = k_off[s];
-    t.Tk[t.n] = k_len[s];
-    rows += rows_of(s);
-    t.first[++t.n] = (int)rows;
-  }
-  return (int)rows;
-}
-
-window::Params window_params(int total_q, int num_q_heads, int num_kv_heads, int head_dim, const void *x_q, const void *x_k, const void *x_v,
-                             int window_, int num_sinks) {
+// the form without tensor cores: a unit of a launch is a row
+window::Params rows_params(const window::Call &c) {
   window::Params p{};
-  p.window = window_;
-  p.sinks = num_sinks;
-  p.q_heads = num_q_heads;
-  p.kv_heads = num_kv_heads;
-  p.head_dim = head_dim;
-  p.total_q = total_q;
-  p.scale = 1.0f / sqrtf((float)head_dim);
-  p.q = (const __nv_bfloat16 *)x_q;
-  p.k = (const __nv_bfloat16 *)x_k;
-  p.v = (const __nv_bfloat16 *)x_v;
+  p.window = c.window;
+  p.sinks = c.sinks;
+  p.q_heads = c.q_heads;
+  p.kv_heads = c.kv_heads;
+  p.head_dim = c.head_dim;
+  p.total_q = c.total_q;
+  p.scale = c.scale;
+  p.q = c.q;
+  p.k = c.k;
+  p.v = c.v;
+  p.o = c.o;
+  p.dout = c.dout;
+  p.lse_in = c.lse_in;
+  p.lse = c.lse;
+  p.delta = (float *)c.workspace;
+  p.out = c.out;
+  p.dq = c.dq;
+  p.dk = c.dk;
+  p.dv = c.dv;
   return p;
 }
 
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 unsigned blocks_for(int64_t warps) { return (unsigned)((warps + window::WARPS - 1) / window::WARPS); }
+
+int rows_fwd(const window::Call &c) {
+  window::Params p = rows_params(c);
+  for (int next = 0; next < c.num_seqs;) {
+    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.q_len[s]; });
+    if (rows == 0) continue;
+    window::rows_fwd_kernel<<<blocks_for(rows * c.q_heads), window::THREADS, 0, c.stream>>>(p);
+    B200_CHECK_LAUNCH("attention_window_fwd");
+  }
+  return 0;
+}
+
+int rows_bwd(const window::Call &c) {
+  window::Params p = rows_params(c);
+  for (int next = 0; next < c.num_seqs;) {
+    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.q_len[s]; });
+    if (rows == 0) continue;
+    window::rows_bwd_q_kernel<<<blocks_for(rows * c.q_heads), window::THREADS, 0, c.stream>>>(p);
+    B200_CHECK_LAUNCH("attention_window_bwd (dQ)");
+  }
+  for (int next = 0; next < c.num_seqs;) {
+    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.k_len[s]; });
+    if (rows == 0) continue;
+    window::rows_bwd_kv_kernel<<<blocks_for(rows * c.kv_heads), window::THREADS, 0, c.stream>>>(p);
+    B200_CHECK_LAUNCH("attention_window_bwd (dK, dV)");
+  }
+  return 0;
+}
+
+void fill_call(window::Call *c, int num_seqs, int total_q, int total_k, const int *q_off, const int *q_len, const int *k_off, const int *k_len,
+               int num_q_heads, int num_kv_heads, int head_dim, const void *x_q, const void *x_k, const void *x_v, int window_, int num_sinks,
+               void *stream) {
+  c->num_seqs = num_seqs;
+  c->total_q = total_q;
+  c->total_k = total_k;
+  c->q_off = q_off;
+  c->q_len = q_len;
+  c->k_off = k_off;
+  c->k_len = k_len;
+  c->q_heads = num_q_heads;
+  c->kv_heads = num_kv_heads;
+  c->head_dim = head_dim;
+  c->window = window_;
+  c->sinks = num_sinks;
+  c->scale = 1.0f / sqrtf((float)head_dim);
+  c->q = (const __nv_bfloat16 *)x_q;
+  c->k = (const __nv_bfloat16 *)x_k;
+  c->v = (const __nv_bfloat16 *)x_v;
+  c->stream = (cudaStream_t)stream;
+}
 
 }  // namespace
 
@@ -314,17 +347,12 @@ extern "C" int b200_attention_window_fwd(int fwd_dt, int num_seqs, int total_q, 
   B200_REQUIRE(x_q && x_k && x_v && x_attn_out && softmax_lse, "attention_window_fwd: null tensor");
   B200_REQUIRE(b200_aligned16(x_q) && b200_aligned16(x_k) && b200_aligned16(x_v) && b200_aligned16(x_attn_out),
                "attention_window_fwd: tensors must be 16-byte aligned");
-  window::Params p = window_params(total_q, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v, window, num_sinks);
-  p.out = (__nv_bfloat16 *)x_attn_out;
-  p.lse = softmax_lse;
-  for (int next = 0; next < num_seqs;) {
-    const int64_t rows = next_sequences(p.seqs, &next, num_seqs, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens,
-                                        [&](int s) { return q_seq_lens[s]; });
-    if (rows == 0) continue;
-    window::rows_fwd_kernel<<<blocks_for(rows * num_q_heads), window::THREADS, 0, (cudaStream_t)stream>>>(p);
-    B200_CHECK_LAUNCH("attention_window_fwd");
-  }
-  return 0;
+  window::Call c{};
+  fill_call(&c, num_seqs, total_q, total_k, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens, num_q_heads, num_kv_heads, head_dim, x_q,
+            x_k, x_v, window, num_sinks, stream);
+  c.out = (__nv_bfloat16 *)x_attn_out;
+  c.lse = softmax_lse;
+  return window::sm100_supported(head_dim) ? window::sm100_fwd(c) : rows_fwd(c);
 }
 
 extern "C" int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, int total_k, const int *q_seq_offsets, const int *q_seq_lens,
@@ -345,27 +373,15 @@ extern "C" int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, 
   B200_REQUIRE(total_q == 0 || (workspace && b200_aligned16(workspace) && workspaceBytes >= need),
                "attention_window_bwd: the workspace holds %llu bytes, %llu are needed (b200_attention_window_workspace_bytes)",
                (unsigned long long)workspaceBytes, (unsigned long long)need);
-  window::Params p = window_params(total_q, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v, window, num_sinks);
-  p.o = (const __nv_bfloat16 *)x_attn_out;
-  p.lse_in = softmax_lse;
-  p.dout = (const __nv_bfloat16 *)dx_out;
-  p.delta = (float *)workspace;
-  p.dq = (__nv_bfloat16 *)dx_q;
-  p.dk = (__nv_bfloat16 *)dx_k;
-  p.dv = (__nv_bfloat16 *)dx_v;
-  for (int next = 0; next < num_seqs;) {
-    const int64_t rows = next_sequences(p.seqs, &next, num_seqs, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens,
-                                        [&](int s) { return q_seq_lens[s]; });
-    if (rows == 0) continue;
-    window::rows_bwd_q_kernel<<<blocks_for(rows * num_q_heads), window::THREADS, 0, (cudaStream_t)stream>>>(p);
-    B200_CHECK_LAUNCH("attention_window_bwd (dQ)");
-  }
-  for (int next = 0; next < num_seqs;) {
-    const int64_t rows = next_sequences(p.seqs, &next, num_seqs, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens,
-                                        [&](int s) { return k_seq_lens[s]; });
-    if (rows == 0) continue;
-    window::rows_bwd_kv_kernel<<<blocks_for(rows * num_kv_heads), window::THREADS, 0, (cudaStream_t)stream>>>(p);
-    B200_CHECK_LAUNCH("attention_window_bwd (dK, dV)");
-  }
-  return 0;
+  window::Call c{};
+  fill_call(&c, num_seqs, total_q, total_k, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens, num_q_heads, num_kv_heads, head_dim, x_q,
+            x_k, x_v, window, num_sinks, stream);
+  c.o = (const __nv_bfloat16 *)x_attn_out;
+  c.lse_in = softmax_lse;
+  c.dout = (const __nv_bfloat16 *)dx_out;
+  c.dq = (__nv_bfloat16 *)dx_q;
+  c.dk = (__nv_bfloat16 *)dx_k;
+  c.dv = (__nv_bfloat16 *)dx_v;
+  c.workspace = (unsigned char *)workspace;
+  return rows_bwd(c);
 }

@@ -175,6 +175,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Registers per thread of the executing warpgroup from here on (all four warps execute it). The increase waits until the
+// block's other warpgroups have given up enough: the shares must add up to no more than the launch's total.
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // ---- CTA pairs (cta_group::2) -----------------------------------------------------------------
 // Two CTAs of a cluster drive one 256-row MMA: each holds 128 rows of A, half the columns of B and
 // its 128 rows of the accumulator. Only the even CTA issues; barriers are reached across the pair
