@@ -274,7 +274,10 @@ window::Params rows_params(const window::Call &c) {
   return p;
 }
 
-uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
+uint64_t bwd_workspace(int num_seqs, int q_heads, int kv_heads, int head_dim, int total_q, int sinks) {
+  if (window::sm100_supported(head_dim)) return window::sm100_bwd_workspace(num_seqs, q_heads, kv_heads, head_dim, total_q, sinks);
+  return ((uint64_t)total_q * q_heads * sizeof(float) + 255) / 256 * 256;  // delta
+}
 
 unsigned blocks_for(int64_t warps) { return (unsigned)((warps + window::WARPS - 1) / window::WARPS); }
 
@@ -333,7 +336,7 @@ void fill_call(window::Call *c, int num_seqs, int total_q, int total_k, const in
 extern "C" uint64_t b200_attention_window_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int max_total_q,
                                                           int num_sinks) {
   if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_total_q <= 0 || num_sinks < 0) return 0;
-  return up256((uint64_t)max_total_q * num_q_heads * sizeof(float));  // delta
+  return bwd_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, max_total_q, num_sinks);
 }
 
 extern "C" int b200_attention_window_fwd(int fwd_dt, int num_seqs, int total_q, int total_k, const int *q_seq_offsets, const int *q_seq_lens,
@@ -369,7 +372,7 @@ extern "C" int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, 
   B200_REQUIRE(b200_aligned16(x_q) && b200_aligned16(x_k) && b200_aligned16(x_v) && b200_aligned16(x_attn_out) && b200_aligned16(dx_out) &&
                    b200_aligned16(dx_q) && b200_aligned16(dx_k) && b200_aligned16(dx_v),
                "attention_window_bwd: tensors must be 16-byte aligned");
-  const uint64_t need = up256((uint64_t)total_q * num_q_heads * sizeof(float));
+  const uint64_t need = bwd_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, total_q, num_sinks);
   B200_REQUIRE(total_q == 0 || (workspace && b200_aligned16(workspace) && workspaceBytes >= need),
                "attention_window_bwd: the workspace holds %llu bytes, %llu are needed (b200_attention_window_workspace_bytes)",
                (unsigned long long)workspaceBytes, (unsigned long long)need);
@@ -383,5 +386,5 @@ extern "C" int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, 
   c.dk = (__nv_bfloat16 *)dx_k;
   c.dv = (__nv_bfloat16 *)dx_v;
   c.workspace = (unsigned char *)workspace;
-  return rows_bwd(c);
+  return window::sm100_supported(head_dim) ? window::sm100_bwd(c) : rows_bwd(c);
 }

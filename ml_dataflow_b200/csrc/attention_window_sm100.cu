@@ -442,6 +442,746 @@ teardown:
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------
+// Backward, two kernels, each with its sums in a fixed order in tensor memory (no atomics: two runs give the same bits). Both put
+// query rows on the tensor-memory lanes, so that a thread's log-sum-exp and delta are its own two numbers.
+//
+// dQ: one query tile of one head per unit, persistent CTAs. Per key block
+//     S = Q K^T,  dP = dO V^T,   dS = P o (dP - delta) as bf16 through shared memory,   dQ += dS K
+// S and dP of a block are issued while the threads still work on the block before, and a unit's first products before the last
+// unit's dQ is finished. delta = rowsum(dO o O) is formed here, in fp32, and written for the other kernel.
+//
+// dK, dV: one block of 128 keys of one key/value head per unit; it walks the query heads of the group and the query tiles that see
+// its keys, K and V stay in shared memory. Per tile
+//     S = Q K^T,  dP = dO V^T,   dV += P^T dO,   dK += dS^T Q      (P and dS are read by the tensor cores with the rows as reduction)
+// Blocks that hold sinks are seen by every later query: tiles behind the block's window are cut into further units that sum their
+// share of the sink rows into the workspace, and a last kernel adds the shares in order.
+//
+// Rounding: P and dS to bf16 once each (dS from the fp32 P), accumulators fp32, one rounding per output.
+// What bounds both: shared memory. A 128 x 128 x 128 product reads 64 KB of operands in the 512 cycles that it takes, all that
+// shared memory gives; writing P and dS and the tiles that arrive come on top.
+// ---------------------------------------------------------------------------------------------------------------------------
+constexpr int BWD_THREADS = 320;  // warp 0 loads, warp 1 issues the MMAs, 8 warps for the element-wise work
+constexpr int DS_TILE = TILE * TILE * 2;
+
+enum { ST_BQ_Q = 61, ST_BQ_KV_EMPTY, ST_BQ_Q_FULL, ST_BQ_KV_FULL, ST_BQ_S_FREE, ST_BQ_DP_FREE, ST_BQ_DS, ST_BQ_ACC, ST_BQ_STAT, ST_BQ_S, ST_BQ_DP,
+       ST_BQ_DQ, ST_BK_KV = 81, ST_BK_Q_EMPTY, ST_BK_DO_EMPTY, ST_BK_Q, ST_BK_DO, ST_BK_S_FREE, ST_BK_DP_FREE, ST_BK_P, ST_BK_DS, ST_BK_S,
+       ST_BK_DP, ST_BK_DV, ST_BK_DK, ST_BK_FIX };
+
+struct BwdParams {
+  CUtensorMap tmQ, tmK, tmV, tmdO;
+  SeqTable seqs;
+  const __nv_bfloat16 *o, *dout;
+  const float *lse;
+  float *delta;  // [q_heads][total_q]
+  __nv_bfloat16 *dq, *dk, *dv;
+  int window, sinks, group, q_heads, kv_heads, total_q, units;
+  // dK, dV: units from main_units on are shares of the sink rows; share[s]: the first slot of sequence s in the workspace
+  int main_units, slot_rows;
+  int far[MAX_SEQS + 1], slot[MAX_SEQS];
+  float *shares;  // [slots][kv_heads][slot_rows][2][head_dim]
+  float scale;
+  int *status;
+};
+
+// eight scores of a row, scaled, against its log-sum-exp: the probabilities; `seen` masks
+struct Seen {
+  int hi, lo, sinks;  // keys of the block (relative to its start) that a row sees: j <= hi and (j >= lo or j < sinks)
+  __device__ __forceinline__ bool operator()(int j) const { return j <= hi && (j >= lo || j < sinks); }
+};
+
+template <int HD>
+struct BwdQShape {
+  static constexpr int Q_TILE = TILE * HD * 2, KV_TILE = TILE * HD * 2;
+  static constexpr int SLOTS = HD == 128 ? 4 : 8;
+  struct Tail {
+    uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full, s_read, dp_full, dp_read, ds_ready, dq_done, acc_empty, stat, fixed;
+    uint32_t tmem_base;
+    int abort_flag;
+    float part[2][TILE];
+  };
+  static constexpr size_t smem = 1024 + 2 * (size_t)Q_TILE + DS_TILE + SLOTS * (size_t)KV_TILE + sizeof(Tail);
+  static_assert(smem <= 232448, "more shared memory than a CTA can be given");
+};
+
+// one tile of one head and its key blocks
+struct QUnit {
+  Span sp;
+  Tile x;
+  int n, n_sink;
+  __device__ __forceinline__ int block(int i) const { return i < n_sink ? i : x.lo + i - n_sink; }
+};
+__device__ __forceinline__ QUnit q_unit_of(const BwdParams &p, int unit) {
+  QUnit u;
+  int s = 0;
+  while (unit >= p.seqs.first[s + 1]) s++;
+  u.sp = span_of(p.seqs, s);
+  const int rel = unit - p.seqs.first[s], tiles = (u.sp.Tq + TILE - 1) / TILE;
+  u.x = tile_of(u.sp, p.window, rel % p.q_heads, (tiles - 1 - rel / p.q_heads) * TILE);
+  u.n_sink = min((p.sinks + TILE - 1) / TILE, u.x.lo);
+  u.n = u.n_sink + u.x.hi - u.x.lo + 1;
+  return u;
+}
+
+// every row of a tile of queries at positions pos0 .. last sees every key of the block
+__device__ __forceinline__ bool all_seen(int base, int pos0, int last, int window, int sinks) {
+  return base + TILE - 1 <= pos0 && (base >= last - window + 1 || base + TILE <= sinks);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __grid_constant__ BwdParams p) {
+  using Sh = BwdQShape<HD>;
+  constexpr int KSL = HD / 64, SLOTS = Sh::SLOTS;
+  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256;
+  extern __shared__ unsigned char window_smem[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(window_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char *sQ = smem, *sDO = sQ + Sh::Q_TILE, *sDS = sDO + Sh::Q_TILE, *sKV = sDS + DS_TILE;
+  auto *st = reinterpret_cast<typename Sh::Tail *>(sKV + SLOTS * Sh::KV_TILE);
+  volatile int *abort_flag = &st->abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto bar = [&](uint64_t *b) { return ptx::smem_u32(b); };
+  auto wait = [&](uint64_t *b, uint32_t par, int code) { return ptx::mbar_wait<false>(bar(b), par & 1u, abort_flag, p.status, code); };
+
+  if (tid == 0) {
+    ptx::mbar_init(bar(&st->q_full), 1);
+    ptx::mbar_init(bar(&st->q_empty), 1);
+    for (int s = 0; s < SLOTS; s++) {
+      ptx::mbar_init(bar(&st->kv_full[s]), 1);
+      ptx::mbar_init(bar(&st->kv_empty[s]), 1);
+    }
+    ptx::mbar_init(bar(&st->s_full), 1);
+    ptx::mbar_init(bar(&st->s_read), 256);
+    ptx::mbar_init(bar(&st->dp_full), 1);
+    ptx::mbar_init(bar(&st->dp_read), 256);
+    ptx::mbar_init(bar(&st->ds_ready), 256);
+    ptx::mbar_init(bar(&st->dq_done), 1);
+    ptx::mbar_init(bar(&st->acc_empty), 256);
+    ptx::mbar_init(bar(&st->stat), 256);
+    ptx::mbar_init(bar(&st->fixed), 1);
+    st->abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(&st->tmem_base), TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::tma_prefetch_desc(&p.tmQ);
+    ptx::tma_prefetch_desc(&p.tmK);
+    ptx::tma_prefetch_desc(&p.tmV);
+    ptx::tma_prefetch_desc(&p.tmdO);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = st->tmem_base;
+
+  if (warp == 0) {
+    // ================= loads: the whole warp walks, one lane issues =================
+    int n = 0;
+    uint32_t units = 0, fixes = 0;
+    bool ok = true;
+    auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
+    for (int unit = blockIdx.x; ok && unit < p.units; unit += gridDim.x) {
+      const QUnit u = q_unit_of(p, unit);
+      const int kvh = u.x.h / p.group;
+      ok = waitw(&st->q_empty, units + 1, ST_BQ_Q);
+      units++;
+      if (ok && lane == 0) {
+        ptx::mbar_arrive_expect_tx(bar(&st->q_full), (uint32_t)(2 * Sh::Q_TILE));
+        for (int s = 0; s < KSL; s++) {
+          ptx::tma_load_2d(ptx::smem_u32(sQ + s * SLAB), &p.tmQ, bar(&st->q_full), u.x.h * HD + s * 64, u.sp.q_off + u.x.row);
+          ptx::tma_load_2d(ptx::smem_u32(sDO + s * SLAB), &p.tmdO, bar(&st->q_full), u.x.h * HD + s * 64, u.sp.q_off + u.x.row);
+        }
+      }
+      for (int i = 0; ok && i < 2 * u.n; i++) {  // K_0, V_0, K_1, V_1, ...
+        const int slot = n % SLOTS, kb = u.block(i >> 1);
+        ok = waitw(&st->kv_empty[slot], (uint32_t)(n / SLOTS) + 1, ST_BQ_KV_EMPTY);
+        n++;
+        if (!ok) break;
+        // K multiplies dS: rows that no query sees have to be zero there. What they make of S and dP is dropped by a select.
+        const bool fix = (i & 1) == 0 && has_dead(u.sp, kb, p.window, p.sinks);
+        const uint32_t tile = ptx::smem_u32(sKV + slot * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(&st->kv_full[slot]);
+        if (lane == 0) {
+          ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::KV_TILE);
+          for (int s = 0; s < KSL; s++)
+            ptx::tma_load_2d(tile + s * SLAB, (i & 1) ? &p.tmV : &p.tmK, full, kvh * HD + s * 64, u.sp.k_off + kb * TILE);
+        }
+        if (!fix) continue;
+        ok = waitw(&st->fixed, fixes++, ST_FIX);
+        if (!ok) break;
+        zero_dead<HD>(tile, u.sp, kb, p.window, p.sinks, lane);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(&st->kv_full[slot]));
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ================= MMA issue =================
+    if (lane == 0) {
+      const uint32_t idesc_s = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
+      const uint32_t idesc_dq = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // K is read with its head dimension contiguous
+      const uint32_t q_base = ptx::smem_u32(sQ), do_base = ptx::smem_u32(sDO), ds_base = ptx::smem_u32(sDS), kv_base = ptx::smem_u32(sKV);
+      uint32_t t = 0, units = 0;  // steps and units so far
+      bool ok = true;
+      // dQ of the step before: issued after S and dP of the current one, across units too
+      bool pending = false, pending_first = false;
+      auto issue_dq = [&]() {
+        const uint32_t tp = t - 1;
+        ok = wait(&st->ds_ready, tp, ST_BQ_DS);
+        // the first of a unit overwrites the accumulator: the threads have read the unit before
+        if (ok && pending_first && units > 1) ok = wait(&st->acc_empty, units - 2, ST_BQ_ACC);
+        if (!ok) return;
+        ptx::tc_fence_after();
+        const int slot = (int)((2 * tp) % SLOTS);
+        const uint64_t ad = tile_desc(ds_base, 0), bd = tile_desc(kv_base + slot * Sh::KV_TILE, SLAB);
+#pragma unroll
+        for (int k16 = 0; k16 < TILE / 16; k16++)
+          ptx::umma_bf16(tmem_base + COL_DQ, desc_at(ad, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)), desc_at(bd, (uint32_t)(k16 * 2048)),
+                         idesc_dq, !pending_first || k16 > 0);
+        ptx::umma_commit(bar(&st->dq_done));
+        ptx::umma_commit(bar(&st->kv_empty[slot]));
+      };
+      for (int unit = blockIdx.x; ok && unit < p.units; unit += gridDim.x) {
+        const QUnit u = q_unit_of(p, unit);
+        ok = wait(&st->q_full, units, ST_BQ_Q_FULL);
+        for (int i = 0; ok && i < u.n; i++) {
+          const int ks = (int)((2 * t) % SLOTS), vs = (int)((2 * t + 1) % SLOTS);
+          if (!(ok = wait(&st->kv_full[ks], 2 * t / SLOTS, ST_BQ_KV_FULL))) break;
+          if (t > 0 && !(ok = wait(&st->s_read, t - 1, ST_BQ_S_FREE))) break;
+          ptx::tc_fence_after();
+          {
+            const uint64_t ad = tile_desc(q_base, 0), bd = tile_desc(kv_base + ks * Sh::KV_TILE, 0);
+#pragma unroll
+            for (int k16 = 0; k16 < HD / 16; k16++) {
+              const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
+              ptx::umma_bf16(tmem_base + COL_S, desc_at(ad, off), desc_at(bd, off), idesc_s, k16 > 0);
+            }
+            ptx::umma_commit(bar(&st->s_full));
+          }
+          if (!(ok = wait(&st->kv_full[vs], (2 * t + 1) / SLOTS, ST_BQ_KV_FULL))) break;
+          if (t > 0 && !(ok = wait(&st->dp_read, t - 1, ST_BQ_DP_FREE))) break;
+          ptx::tc_fence_after();
+          {
+            const uint64_t ad = tile_desc(do_base, 0), bd = tile_desc(kv_base + vs * Sh::KV_TILE, 0);
+#pragma unroll
+            for (int k16 = 0; k16 < HD / 16; k16++) {
+              const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
+              ptx::umma_bf16(tmem_base + COL_DP, desc_at(ad, off), desc_at(bd, off), idesc_s, k16 > 0);
+            }
+            ptx::umma_commit(bar(&st->dp_full));
+            ptx::umma_commit(bar(&st->kv_empty[vs]));
+            if (i == u.n - 1) ptx::umma_commit(bar(&st->q_empty));
+          }
+          if (pending) issue_dq();
+          if (!ok) break;
+          t++;
+          pending = true;
+          pending_first = i == 0;
+          if (i == 0) units++;
+        }
+      }
+      if (ok && pending) issue_dq();
+    }
+    __syncwarp();
+  } else {
+    // ================= element-wise work: a thread per (query row, half of the columns) =================
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int trow = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t ds_addr = ptx::smem_u32(sDS + half * SLAB + trow * 128);
+    const float c = p.scale * LOG2E;
+    uint32_t t = 0, units = 0;
+    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+      const QUnit u = q_unit_of(p, unit);
+      const int row = u.x.row + trow, pos = row + u.sp.shift;
+      const bool valid = row < u.sp.Tq;
+      const int64_t at = ((int64_t)(u.sp.q_off + row) * p.q_heads + u.x.h) * HD, stat = (int64_t)u.x.h * p.total_q + u.sp.q_off + row;
+      // delta: either thread of a row takes half of the dimensions
+      float lse2 = 0.0f, delta = 0.0f;
+      if (valid) {
+        lse2 = p.lse[stat] * LOG2E;
+        const uint4 *a = reinterpret_cast<const uint4 *>(p.dout + at + half * (HD / 2)), *b = reinterpret_cast<const uint4 *>(p.o + at + half * (HD / 2));
+#pragma unroll
+        for (int q = 0; q < HD / 16; q++) {
+          float x[8], y[8];
+          unpack8(a[q], x);
+          unpack8(b[q], y);
+#pragma unroll
+          for (int j = 0; j < 8; j++) delta = fmaf(x[j], y[j], delta);
+        }
+      }
+      st->part[half][trow] = delta;
+      ptx::mbar_arrive(bar(&st->stat));
+      if (!wait(&st->stat, units, ST_BQ_STAT)) goto teardown;
+      units++;
+      delta = st->part[0][trow] + st->part[1][trow];
+      if (valid && half == 0) p.delta[stat] = delta;
+      const int pos0 = u.x.row + u.sp.shift, last_pos = min(pos0 + TILE, u.sp.Tk) - 1;
+      for (int i = 0; i < u.n; i++) {
+        const int base = u.block(i) * TILE + half * 64;
+        const bool whole = all_seen(u.block(i) * TILE, pos0, last_pos, p.window, p.sinks);
+        const Seen seen{min(pos, u.sp.Tk - 1) - base, pos - p.window + 1 - base, p.sinks - base};
+        uint32_t s[64];
+        if (!wait(&st->s_full, t, ST_BQ_S)) goto teardown;
+        ptx::tc_fence_after();
+        ptx::tmem_ld32(lane_addr + COL_S + half * 64, s);
+        ptx::tmem_ld32(lane_addr + COL_S + half * 64 + 32, s + 32);
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(bar(&st->s_read));
+#pragma unroll
+        for (int j = 0; j < 64; j++) s[j] = __float_as_uint(ex2(fmaf(__uint_as_float(s[j]), c, -lse2)));
+        uint32_t d[64];
+        if (!wait(&st->dp_full, t, ST_BQ_DP)) goto teardown;
+        ptx::tc_fence_after();
+        ptx::tmem_ld32(lane_addr + COL_DP + half * 64, d);
+        ptx::tmem_ld32(lane_addr + COL_DP + half * 64 + 32, d + 32);
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(bar(&st->dp_read));
+#pragma unroll
+        for (int j = 0; j < 64; j++) d[j] = __float_as_uint(__uint_as_float(s[j]) * (__uint_as_float(d[j]) - delta));
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 64; j++) d[j] = seen(j) ? d[j] : 0u;
+        }
+        // the product of the step before has read dS
+        if (t > 0 && !wait(&st->dq_done, t - 1, ST_BQ_DQ)) goto teardown;
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+          uint4 v;
+          v.x = pack_bf16(__uint_as_float(d[q * 8 + 0]), __uint_as_float(d[q * 8 + 1]));
+          v.y = pack_bf16(__uint_as_float(d[q * 8 + 2]), __uint_as_float(d[q * 8 + 3]));
+          v.z = pack_bf16(__uint_as_float(d[q * 8 + 4]), __uint_as_float(d[q * 8 + 5]));
+          v.w = pack_bf16(__uint_as_float(d[q * 8 + 6]), __uint_as_float(d[q * 8 + 7]));
+          sts128(ds_addr + (uint32_t)((q ^ (trow & 7)) * 16), v);
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(bar(&st->ds_ready));
+        t++;
+      }
+      if (!wait(&st->dq_done, t - 1, ST_BQ_DQ)) goto teardown;
+      ptx::tc_fence_after();
+      uint32_t r[HD / 2];
+#pragma unroll
+      for (int q = 0; q < HD / 64; q++) ptx::tmem_ld32(lane_addr + COL_DQ + half * (HD / 2) + q * 32, r + q * 32);
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(bar(&st->acc_empty));
+      if (valid) {
+        uint4 *o = reinterpret_cast<uint4 *>(p.dq + at + half * (HD / 2));
+#pragma unroll
+        for (int q = 0; q < HD / 16; q++) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = __uint_as_float(r[q * 8 + j]) * p.scale;
+          o[q] = pack8(v);
+        }
+      }
+    }
+  }
+
+teardown:
+  if (*abort_flag) {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---- dK, dV ----------------------------------------------------------------------------------------------------------------
+// The query tiles of a sequence that a block of keys walks: t0 .. t1 - 1 see it through the window; for a block with sinks tiles
+// t1 .. tiles - 1 see the sinks only, and go to `chunks` further units of `chunk` tiles. (Host and device.)
+struct KeyWalk {
+  int t0, t1, tiles, chunk, chunks;
+};
+constexpr int MIN_CHUNK = 8;         // tiles of such a unit: at least this many, and as many as a block's window spans
+constexpr int MAX_SPLIT_SINKS = 1024;  // more sinks than this fill the GPU with blocks of their own: their units walk every tile
+__host__ __device__ inline KeyWalk key_walk(int Tq, int Tk, int kb, int window, int sinks) {
+  KeyWalk w;
+  const int shift = Tk - Tq;
+  w.tiles = (Tq + TILE - 1) / TILE;
+  const int64_t lo = (int64_t)kb * TILE - shift, hi = (int64_t)kb * TILE + TILE - 1 + window - 1 - shift;  // rows, hi inclusive
+  w.t0 = lo > 0 ? (int)(lo / TILE) : 0;
+  w.t1 = hi < 0 ? 0 : (hi >= Tq ? w.tiles : (int)(hi / TILE) + 1);
+  if (w.t1 < w.t0) w.t1 = w.t0;
+  w.chunk = window / TILE + 1 > MIN_CHUNK ? window / TILE + 1 : MIN_CHUNK;
+  w.chunks = 0;
+  if ((int64_t)kb * TILE < sinks) {
+    if (sinks > MAX_SPLIT_SINKS)
+      w.t1 = w.tiles;
+    else
+      w.chunks = (w.tiles - w.t1 + w.chunk - 1) / w.chunk;
+  }
+  return w;
+}
+// blocks with sinks whose far tiles are split off, and the most units one of them is split into (the first block's)
+__host__ __device__ inline int split_blocks(int Tk, int sinks) {
+  if (sinks > MAX_SPLIT_SINKS) return 0;
+  const int s = sinks < Tk ? sinks : Tk;
+  return (s + TILE - 1) / TILE;
+}
+
+template <int HD>
+struct BwdKShape {
+  static constexpr int T_TILE = TILE * HD * 2;
+  static constexpr int Q_SLOTS = HD == 128 ? 2 : 3, DO_SLOTS = HD == 128 ? 1 : 3;
+  struct Tail {
+    uint64_t kv_full, q_full[Q_SLOTS], q_empty[Q_SLOTS], do_full[DO_SLOTS], do_empty[DO_SLOTS], s_full, s_read, dp_full, dp_read, p_ready, ds_ready,
+        dv_done, dk_done, fixed;
+    uint32_t tmem_base;
+    int abort_flag;
+  };
+  static constexpr size_t smem = 1024 + (2 + Q_SLOTS + DO_SLOTS) * (size_t)T_TILE + 2 * DS_TILE + sizeof(Tail);
+  static_assert(smem <= 232448, "more shared memory than a CTA can be given");
+};
+
+template <int HD>
+__global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __grid_constant__ BwdParams p) {
+  using Sh = BwdKShape<HD>;
+  constexpr int KSL = HD / 64, QS = Sh::Q_SLOTS, DS = Sh::DO_SLOTS;
+  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DK = 256, COL_DV = 384;
+  extern __shared__ unsigned char window_smem[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(window_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char *sK = smem, *sV = sK + Sh::T_TILE, *sP = sV + Sh::T_TILE, *sDS = sP + DS_TILE, *sQ = sDS + DS_TILE, *sDO = sQ + QS * Sh::T_TILE;
+  auto *st = reinterpret_cast<typename Sh::Tail *>(sDO + DS * Sh::T_TILE);
+  volatile int *abort_flag = &st->abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto bar = [&](uint64_t *b) { return ptx::smem_u32(b); };
+  auto wait = [&](uint64_t *b, uint32_t par, int code) { return ptx::mbar_wait<false>(bar(b), par & 1u, abort_flag, p.status, code); };
+
+  if (tid == 0) {
+    ptx::mbar_init(bar(&st->kv_full), 1);
+    for (int s = 0; s < QS; s++) {
+      ptx::mbar_init(bar(&st->q_full[s]), 1);
+      ptx::mbar_init(bar(&st->q_empty[s]), 1);
+    }
+    for (int s = 0; s < DS; s++) {
+      ptx::mbar_init(bar(&st->do_full[s]), 1);
+      ptx::mbar_init(bar(&st->do_empty[s]), 1);
+    }
+    ptx::mbar_init(bar(&st->s_full), 1);
+    ptx::mbar_init(bar(&st->s_read), 256);
+    ptx::mbar_init(bar(&st->dp_full), 1);
+    ptx::mbar_init(bar(&st->dp_read), 256);
+    ptx::mbar_init(bar(&st->p_ready), 256);
+    ptx::mbar_init(bar(&st->ds_ready), 256);
+    ptx::mbar_init(bar(&st->dv_done), 1);
+    ptx::mbar_init(bar(&st->dk_done), 1);
+    ptx::mbar_init(bar(&st->fixed), 1);
+    st->abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(&st->tmem_base), TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::tma_prefetch_desc(&p.tmQ);
+    ptx::tma_prefetch_desc(&p.tmK);
+    ptx::tma_prefetch_desc(&p.tmV);
+    ptx::tma_prefetch_desc(&p.tmdO);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = st->tmem_base;
+
+  // the unit: a block of keys of one key/value head, and the query tiles it walks for every query head of the group
+  const int unit = blockIdx.x;
+  int s = 0, kb, kvh, t0, t1, share = -1;  // share: the slot of the workspace that takes the sink rows
+  if (unit < p.main_units) {
+    while (unit >= p.seqs.first[s + 1]) s++;
+    const int rel = unit - p.seqs.first[s];
+    kvh = rel % p.kv_heads;
+    kb = rel / p.kv_heads;
+  } else {
+    while (unit - p.main_units >= p.far[s + 1]) s++;
+    kvh = (unit - p.main_units - p.far[s]) % p.kv_heads;
+    kb = 0;
+  }
+  const Span sp = span_of(p.seqs, s);
+  const int most = key_walk(sp.Tq, sp.Tk, 0, p.window, p.sinks).chunks;
+  int part = 0;
+  if (unit >= p.main_units) {
+    const int rel = (unit - p.main_units - p.far[s]) / p.kv_heads;  // block, then chunk
+    kb = rel / most;
+    part = 1 + rel % most;
+  }
+  {
+    const KeyWalk w = key_walk(sp.Tq, sp.Tk, kb, p.window, p.sinks);
+    t0 = part == 0 ? w.t0 : w.t1 + (part - 1) * w.chunk;
+    t1 = part == 0 ? w.t1 : min(w.tiles, t0 + w.chunk);
+    if (w.chunks > 0) share = p.slot[s] + kb * (most + 1) + part;
+    if (part > w.chunks) share = -1;  // this block is split into fewer units than the first: nothing to do
+  }
+  const int tiles = max(0, t1 - t0), n = tiles * p.group;
+
+  if (n > 0 && warp == 0) {
+    // ================= loads: the whole warp walks, one lane issues =================
+    bool ok = true;
+    uint32_t fixes = 0;
+    auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
+    if (lane == 0) {
+      ptx::mbar_arrive_expect_tx(bar(&st->kv_full), (uint32_t)(2 * Sh::T_TILE));
+      for (int q = 0; q < KSL; q++) {
+        ptx::tma_load_2d(ptx::smem_u32(sK + q * SLAB), &p.tmK, bar(&st->kv_full), kvh * HD + q * 64, sp.k_off + kb * TILE);
+        ptx::tma_load_2d(ptx::smem_u32(sV + q * SLAB), &p.tmV, bar(&st->kv_full), kvh * HD + q * 64, sp.k_off + kb * TILE);
+      }
+    }
+    for (int i = 0; ok && i < n; i++) {
+      const int h = kvh * p.group + i / tiles, row = (t0 + i % tiles) * TILE;
+      const bool fix = row + TILE > sp.Tq;  // rows past the sequence's end are zeroed: dO and Q multiply P and dS
+#pragma unroll
+      for (int which = 0; which < 2; which++) {
+        const int slot = which == 0 ? i % QS : i % DS;
+        uint64_t *empty = which == 0 ? &st->q_empty[slot] : &st->do_empty[slot], *full_b = which == 0 ? &st->q_full[slot] : &st->do_full[slot];
+        if (!ok) continue;
+        ok = waitw(empty, (uint32_t)(i / (which == 0 ? QS : DS)) + 1, which == 0 ? ST_BK_Q_EMPTY : ST_BK_DO_EMPTY);
+        if (!ok) continue;
+        const uint32_t tile = ptx::smem_u32((which == 0 ? sQ : sDO) + slot * Sh::T_TILE), full = fix ? bar(&st->fixed) : bar(full_b);
+        if (lane == 0) {
+          ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::T_TILE);
+          for (int q = 0; q < KSL; q++)
+            ptx::tma_load_2d(tile + q * SLAB, which == 0 ? &p.tmQ : &p.tmdO, full, h * HD + q * 64, sp.q_off + row);
+        }
+        if (!fix) continue;
+        ok = waitw(&st->fixed, fixes++, ST_BK_FIX);
+        if (!ok) continue;
+        for (int r = sp.Tq - row + lane; r < TILE; r += 32)
+#pragma unroll
+          for (int q = 0; q < KSL; q++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) sts128(tile + q * SLAB + r * 128 + e * 16, make_uint4(0, 0, 0, 0));
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(full_b));
+      }
+    }
+    __syncwarp();
+  } else if (n > 0 && warp == 1) {
+    // ================= MMA issue =================
+    if (lane == 0) {
+      const uint32_t idesc_s = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
+      const uint32_t idesc_t = ptx::make_idesc_bf16(TILE, HD, 1, 1);  // both operands with their rows as the reduction
+      const uint32_t k_base = ptx::smem_u32(sK), v_base = ptx::smem_u32(sV), p_base = ptx::smem_u32(sP), ds_base = ptx::smem_u32(sDS),
+                     q_base = ptx::smem_u32(sQ), do_base = ptx::smem_u32(sDO);
+      auto rows_product = [&](uint32_t a, uint32_t b, uint32_t col) {  // [queries x head_dim] [keys x head_dim]^T
+        const uint64_t ad = tile_desc(a, 0), bd = tile_desc(b, 0);
+#pragma unroll
+        for (int k16 = 0; k16 < HD / 16; k16++) {
+          const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
+          ptx::umma_bf16(tmem_base + col, desc_at(ad, off), desc_at(bd, off), idesc_s, k16 > 0);
+        }
+      };
+      auto reduce_rows = [&](uint32_t a, uint32_t b, uint32_t col, bool add) {  // [queries x keys]^T [queries x head_dim]
+        const uint64_t ad = tile_desc(a, SLAB), bd = tile_desc(b, SLAB);
+#pragma unroll
+        for (int k16 = 0; k16 < TILE / 16; k16++)
+          ptx::umma_bf16(tmem_base + col, desc_at(ad, (uint32_t)(k16 * 2048)), desc_at(bd, (uint32_t)(k16 * 2048)), idesc_t, add || k16 > 0);
+      };
+      auto q_tile = [&](int i) { return q_base + (uint32_t)(i % QS) * Sh::T_TILE; };
+      auto do_tile = [&](int i) { return do_base + (uint32_t)(i % DS) * Sh::T_TILE; };
+      auto issue_s = [&](int i) {
+        if (!wait(&st->q_full[i % QS], (uint32_t)(i / QS), ST_BK_Q)) return false;
+        if (i > 0 && !wait(&st->s_read, (uint32_t)(i - 1), ST_BK_S_FREE)) return false;
+        ptx::tc_fence_after();
+        rows_product(q_tile(i), k_base, COL_S);
+        ptx::umma_commit(bar(&st->s_full));
+        return true;
+      };
+      auto issue_dp = [&](int i) {
+        if (!wait(&st->do_full[i % DS], (uint32_t)(i / DS), ST_BK_DO)) return false;
+        if (i > 0 && !wait(&st->dp_read, (uint32_t)(i - 1), ST_BK_DP_FREE)) return false;
+        ptx::tc_fence_after();
+        rows_product(do_tile(i), v_base, COL_DP);
+        ptx::umma_commit(bar(&st->dp_full));
+        return true;
+      };
+      bool ok = wait(&st->kv_full, 0, ST_BK_KV) && issue_s(0) && issue_dp(0);
+      for (int i = 0; ok && i < n; i++) {
+        if (i + 1 < n && !issue_s(i + 1)) break;
+        if (!wait(&st->p_ready, (uint32_t)i, ST_BK_P)) break;
+        ptx::tc_fence_after();
+        reduce_rows(p_base, do_tile(i), COL_DV, i > 0);
+        ptx::umma_commit(bar(&st->dv_done));
+        ptx::umma_commit(bar(&st->do_empty[i % DS]));
+        if (!wait(&st->ds_ready, (uint32_t)i, ST_BK_DS)) break;
+        ptx::tc_fence_after();
+        reduce_rows(ds_base, q_tile(i), COL_DK, i > 0);
+        ptx::umma_commit(bar(&st->dk_done));
+        ptx::umma_commit(bar(&st->q_empty[i % QS]));
+        if (i + 1 < n && !issue_dp(i + 1)) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 2) {
+    // ================= element-wise work: a thread per (query row, half of the keys); at the end per (key, half of the dims) ======
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int trow = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t p_addr = ptx::smem_u32(sP + half * SLAB + trow * 128), ds_addr = ptx::smem_u32(sDS + half * SLAB + trow * 128);
+    const float c = p.scale * LOG2E;
+    const int base = kb * TILE + half * 64;
+    auto stats_of = [&](int i, float &lse2, float &delta) {
+      const int row = (t0 + i % tiles) * TILE + trow;
+      lse2 = delta = 0.0f;
+      if (i < n && row < sp.Tq) {
+        const int64_t at = (int64_t)(kvh * p.group + i / tiles) * p.total_q + sp.q_off + row;
+        lse2 = p.lse[at] * LOG2E;
+        delta = p.delta[at];
+      }
+    };
+    float lse2 = 0.0f, delta = 0.0f, next_lse2 = 0.0f, next_delta = 0.0f;
+    if (n > 0) stats_of(0, next_lse2, next_delta);
+    for (int i = 0; i < n; i++) {
+      lse2 = next_lse2;
+      delta = next_delta;
+      if (i + 1 < n) stats_of(i + 1, next_lse2, next_delta);  // on their way while this step computes
+      const int row0 = (t0 + i % tiles) * TILE, row = row0 + trow, pos = row + sp.shift, pos0 = row0 + sp.shift;
+      const bool whole = row0 + TILE <= sp.Tq && all_seen(kb * TILE, pos0, pos0 + TILE - 1, p.window, p.sinks);
+      const Seen seen{row < sp.Tq ? pos - base : -1, pos - p.window + 1 - base, p.sinks - base};
+      uint32_t x[64];
+      if (!wait(&st->s_full, (uint32_t)i, ST_BK_S)) goto teardown;
+      ptx::tc_fence_after();
+      ptx::tmem_ld32(lane_addr + COL_S + half * 64, x);
+      ptx::tmem_ld32(lane_addr + COL_S + half * 64 + 32, x + 32);
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(bar(&st->s_read));
+#pragma unroll
+      for (int j = 0; j < 64; j++) x[j] = __float_as_uint(ex2(fmaf(__uint_as_float(x[j]), c, -lse2)));
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 64; j++) x[j] = seen(j) ? x[j] : 0u;
+      }
+      if (i > 0 && !wait(&st->dv_done, (uint32_t)(i - 1), ST_BK_DV)) goto teardown;  // has read P
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        uint4 v;
+        v.x = pack_bf16(__uint_as_float(x[q * 8 + 0]), __uint_as_float(x[q * 8 + 1]));
+        v.y = pack_bf16(__uint_as_float(x[q * 8 + 2]), __uint_as_float(x[q * 8 + 3]));
+        v.z = pack_bf16(__uint_as_float(x[q * 8 + 4]), __uint_as_float(x[q * 8 + 5]));
+        v.w = pack_bf16(__uint_as_float(x[q * 8 + 6]), __uint_as_float(x[q * 8 + 7]));
+        sts128(p_addr + (uint32_t)((q ^ (trow & 7)) * 16), v);
+      }
+      ptx::fence_proxy_async_smem();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(bar(&st->p_ready));
+      uint32_t d[64];
+      if (!wait(&st->dp_full, (uint32_t)i, ST_BK_DP)) goto teardown;
+      ptx::tc_fence_after();
+      ptx::tmem_ld32(lane_addr + COL_DP + half * 64, d);
+      ptx::tmem_ld32(lane_addr + COL_DP + half * 64 + 32, d + 32);
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(bar(&st->dp_read));
+#pragma unroll
+      for (int j = 0; j < 64; j++) d[j] = __float_as_uint(__uint_as_float(x[j]) * (__uint_as_float(d[j]) - delta));
+      if (!whole) {  // a masked product may be anything
+#pragma unroll
+        for (int j = 0; j < 64; j++) d[j] = seen(j) ? d[j] : 0u;
+      }
+      if (i > 0 && !wait(&st->dk_done, (uint32_t)(i - 1), ST_BK_DK)) goto teardown;  // has read dS
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        uint4 v;
+        v.x = pack_bf16(__uint_as_float(d[q * 8 + 0]), __uint_as_float(d[q * 8 + 1]));
+        v.y = pack_bf16(__uint_as_float(d[q * 8 + 2]), __uint_as_float(d[q * 8 + 3]));
+        v.z = pack_bf16(__uint_as_float(d[q * 8 + 4]), __uint_as_float(d[q * 8 + 5]));
+        v.w = pack_bf16(__uint_as_float(d[q * 8 + 6]), __uint_as_float(d[q * 8 + 7]));
+        sts128(ds_addr + (uint32_t)((q ^ (trow & 7)) * 16), v);
+      }
+      ptx::fence_proxy_async_smem();
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(bar(&st->ds_ready));
+    }
+    if (n > 0) {
+      if (!wait(&st->dk_done, (uint32_t)(n - 1), ST_BK_DK)) goto teardown;
+      ptx::tc_fence_after();
+    }
+    if (n > 0 || part == 0) {
+      // the accumulators' lanes are keys
+      const int key = kb * TILE + trow;
+      const bool to_share = share >= 0 && key < p.sinks;
+      float *sh = to_share ? p.shares + (((int64_t)share * p.kv_heads + kvh) * p.slot_rows + trow) * 2 * HD + half * (HD / 2) : nullptr;
+      const int64_t at = ((int64_t)(sp.k_off + key) * p.kv_heads + kvh) * HD + half * (HD / 2);
+#pragma unroll
+      for (int which = 0; which < 2; which++) {
+        uint32_t r[HD / 2];
+        if (n > 0) {
+#pragma unroll
+          for (int q = 0; q < HD / 64; q++)
+            ptx::tmem_ld32(lane_addr + (which == 0 ? COL_DK : COL_DV) + half * (HD / 2) + q * 32, r + q * 32);
+          ptx::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < HD / 2; j++) r[j] = 0u;
+        }
+        const float f = which == 0 ? p.scale : 1.0f;
+        if (key >= sp.Tk) continue;
+#pragma unroll
+        for (int q = 0; q < HD / 16; q++) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = __uint_as_float(r[q * 8 + j]) * f;
+          if (to_share) {
+            reinterpret_cast<float4 *>(sh + which * HD)[2 * q] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4 *>(sh + which * HD)[2 * q + 1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else if (part == 0) {
+            reinterpret_cast<uint4 *>((which == 0 ? p.dk : p.dv) + at)[q] = pack8(v);
+          }
+        }
+      }
+    }
+  }
+
+teardown:
+  if (*abort_flag) {
+    const uint64_t t_abort = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t_abort < 200000ull) __nanosleep(1000);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// dK and dV of the sink rows: the shares of a block's units, in order. Grid: (blocks with sinks * kv heads, sequences); a thread per
+// (row, dimension).
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ BwdParams p, int head_dim) {
+  const int s = blockIdx.y, kb = blockIdx.x / p.kv_heads, kvh = blockIdx.x % p.kv_heads;
+  const Span sp = span_of(p.seqs, s);
+  if (kb >= split_blocks(sp.Tk, p.sinks)) return;
+  const int chunks = key_walk(sp.Tq, sp.Tk, kb, p.window, p.sinks).chunks, most = key_walk(sp.Tq, sp.Tk, 0, p.window, p.sinks).chunks;
+  if (chunks == 0) return;
+  const int rows = min(min(p.sinks, sp.Tk) - kb * TILE, TILE);
+  const int64_t step = (int64_t)p.kv_heads * p.slot_rows * 2 * head_dim;
+  const float *first = p.shares + ((int64_t)(p.slot[s] + kb * (most + 1)) * p.kv_heads + kvh) * p.slot_rows * 2 * head_dim;
+  for (int i = threadIdx.x; i < rows * 2 * head_dim; i += 256) {
+    float sum = 0.0f;
+    for (int c = 0; c <= chunks; c++) sum += first[c * step + i];
+    const int row = i / (2 * head_dim), d = i - row * 2 * head_dim;
+    const int64_t at = ((int64_t)(sp.k_off + kb * TILE + row) * p.kv_heads + kvh) * head_dim;
+    if (d < head_dim)
+      p.dk[at + d] = __float2bfloat16_rn(sum);
+    else
+      p.dv[at + d - head_dim] = __float2bfloat16_rn(sum);
+  }
+}
+
 bool sm100_supported(int head_dim) { return head_dim == 64 || head_dim == 128; }
 
 }  // namespace window
@@ -479,10 +1219,107 @@ int launch_fwd(window::FwdParams &p, const Device &d, cudaStream_t s) {
   return 0;
 }
 
+template <int HD>
+int launch_bwd_q(const window::BwdParams &p, const Device &d, cudaStream_t s) {
+  static bool done[MAX_DEVICES];
+  constexpr size_t smem = window::BwdQShape<HD>::smem;
+  if (allow_smem(window::window_bwd_q_kernel<HD>, smem, &done[d.dev])) return -1;
+  window::window_bwd_q_kernel<HD><<<p.units < d.sms ? p.units : d.sms, window::BWD_THREADS, smem, s>>>(p);
+  B200_CHECK_LAUNCH("attention_window_bwd (dQ)");
+  return 0;
+}
+
+template <int HD>
+int launch_bwd_kv(const window::BwdParams &p, const Device &d, cudaStream_t s) {
+  static bool done[MAX_DEVICES];
+  constexpr size_t smem = window::BwdKShape<HD>::smem;
+  if (allow_smem(window::window_bwd_kv_kernel<HD>, smem, &done[d.dev])) return -1;
+  window::window_bwd_kv_kernel<HD><<<p.units, window::BWD_THREADS, smem, s>>>(p);
+  B200_CHECK_LAUNCH("attention_window_bwd (dK, dV)");
+  return 0;
+}
+
+uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+int slot_rows(int sinks) { return sinks < window::TILE ? sinks : window::TILE; }
+
 }  // namespace
 
 namespace b200 {
 namespace window {
+
+// delta, then the shares of the sink rows. A block's shares: its own and those of at most ceil(tiles / MIN_CHUNK) further units, that is
+// Tq / 1024 + 3 at most.
+uint64_t sm100_bwd_workspace(int num_seqs, int q_heads, int kv_heads, int head_dim, int total_q, int sinks) {
+  static_assert(TILE * MIN_CHUNK == 1024, "the bound on a sequence's shares");
+  uint64_t n = up256((uint64_t)total_q * q_heads * sizeof(float));
+  if (sinks > 0 && sinks <= MAX_SPLIT_SINKS) {
+    const uint64_t seqs = num_seqs < MAX_SEQS ? num_seqs : MAX_SEQS;  // of one launch
+    n += (uint64_t)((sinks + TILE - 1) / TILE) * ((uint64_t)total_q / 1024 + 3 * seqs) * kv_heads * slot_rows(sinks) * 2 * head_dim * sizeof(float);
+  }
+  return n;
+}
+
+int sm100_bwd(const Call &c) {
+  BwdParams p;
+  Device d;
+  if (current_device(&d)) return -1;
+  const uint64_t Dq = (uint64_t)c.q_heads * c.head_dim, Dk = (uint64_t)c.kv_heads * c.head_dim;
+  if (c.total_q == 0) {  // no query sees any key
+    for (int s = 0; s < c.num_seqs; s++) {
+      B200_CUDA(cudaMemsetAsync(c.dk + (int64_t)c.k_off[s] * Dk, 0, (size_t)c.k_len[s] * Dk * 2, c.stream));
+      B200_CUDA(cudaMemsetAsync(c.dv + (int64_t)c.k_off[s] * Dk, 0, (size_t)c.k_len[s] * Dk * 2, c.stream));
+    }
+    return 0;
+  }
+  if (rows_map(&p.tmQ, c.q, (uint64_t)c.total_q, Dq) || rows_map(&p.tmdO, c.dout, (uint64_t)c.total_q, Dq) ||
+      rows_map(&p.tmK, c.k, (uint64_t)c.total_k, Dk) || rows_map(&p.tmV, c.v, (uint64_t)c.total_k, Dk))
+    return -1;
+  p.o = c.o;
+  p.dout = c.dout;
+  p.lse = c.lse_in;
+  p.delta = (float *)c.workspace;
+  p.shares = (float *)(c.workspace + up256((uint64_t)c.total_q * c.q_heads * sizeof(float)));
+  p.dq = c.dq;
+  p.dk = c.dk;
+  p.dv = c.dv;
+  p.window = c.window;
+  p.sinks = c.sinks;
+  p.group = c.q_heads / c.kv_heads;
+  p.q_heads = c.q_heads;
+  p.kv_heads = c.kv_heads;
+  p.total_q = c.total_q;
+  p.scale = c.scale;
+  p.slot_rows = slot_rows(c.sinks);
+  p.main_units = 0;
+  p.status = attn_status_ptr();
+  B200_REQUIRE(p.status != nullptr, "attention_window: the status word of this device is not reachable");
+  for (int next = 0; next < c.num_seqs;) {
+    p.units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.q_len[s] + TILE - 1) / TILE * c.q_heads; });
+    if (p.units == 0) continue;
+    if (c.head_dim == 128 ? launch_bwd_q<128>(p, d, c.stream) : launch_bwd_q<64>(p, d, c.stream)) return -1;
+  }
+  for (int next = 0; next < c.num_seqs;) {
+    p.main_units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.k_len[s] + TILE - 1) / TILE * c.kv_heads; });
+    if (p.main_units == 0) continue;
+    int slots = 0, blocks = 0;
+    p.far[0] = 0;
+    for (int s = 0; s < p.seqs.n; s++) {
+      const int split = split_blocks(p.seqs.Tk[s], c.sinks), chunks = key_walk(p.seqs.Tq[s], p.seqs.Tk[s], 0, c.window, c.sinks).chunks;
+      const bool any = split > 0 && chunks > 0;
+      p.slot[s] = slots;
+      p.far[s + 1] = p.far[s] + (any ? split * chunks * c.kv_heads : 0);
+      if (any) slots += split * (chunks + 1);
+      if (any && split > blocks) blocks = split;
+    }
+    p.units = p.main_units + p.far[p.seqs.n];
+    if (c.head_dim == 128 ? launch_bwd_kv<128>(p, d, c.stream) : launch_bwd_kv<64>(p, d, c.stream)) return -1;
+    if (blocks == 0) continue;
+    window_join_kernel<<<dim3((unsigned)(blocks * c.kv_heads), (unsigned)p.seqs.n), 256, 0, c.stream>>>(p, c.head_dim);
+    B200_CHECK_LAUNCH("attention_window_bwd (sinks)");
+  }
+  return 0;
+}
 
 int sm100_fwd(const Call &c) {
   FwdParams p;

@@ -94,7 +94,8 @@ def window_attention(q_offs, q_lens, k_offs, k_lens, hq, hkv, hd, q, k, v, windo
             r["dk"][ko:ko + t, ck] += ds.T @ Q
             r["dk_slack"][ko:ko + t, ck] += 1.02 * (err.T @ Q.abs())
             r["dv"][ko:ko + t, ck] += p.T @ dO
-            r["dv_slack"][ko:ko + t, ck] += 1.02 * HALF * (p.T @ dO.abs())
+            # probabilities below 2^-126 are formed as 0 (the exponential's results are never subnormal)
+            r["dv_slack"][ko:ko + t, ck] += 1.02 * HALF * (p.T @ dO.abs()) + 2.0 ** -126 * dO.abs().sum(0)
     return r
 
 
