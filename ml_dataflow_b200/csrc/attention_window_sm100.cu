@@ -5,10 +5,14 @@
 // sees are never touched: the unit walks the blocks that hold sinks, then those of its window. A persistent CTA (one per SM)
 // takes units in turn: while one unit's last products and its output are under way, the next one's queries and keys load.
 //   warp 0     TMA loads: the query tiles, and K_0, K_1, V_0, K_2, V_1, ... through a ring, in the order they are used
-//   warp 1     one thread issues the tcgen05 MMAs  S_g = Q_g K^T  and  O_g += P_g V  (fp32 accumulators in tensor memory)
+//   warp 1     one thread issues the tcgen05 MMAs  S_g = Q_g K^T   (fp32 accumulators in tensor memory)
+//   warps 2, 3 one thread each issues  O_g += P_g V  of its tile. Three issuers, because a wait costs an issuing thread about 250
+//              cycles and the tensor pipe queues less than that: with a single one that waited for all of it in turn a step of a
+//              pair took 5600 cycles
 //   warps 4-11 four per tile, a thread per query row: scores to registers at once - which frees the accumulator for the next
 //              S, so that the tensor cores work while the exponentials are formed -, running maximum and sum,
-//              P = exp2((S - m) scale log2 e) as bf16 through shared memory
+//              P = exp2((S - m) scale log2 e) as bf16 through shared memory. The second tile starts when the first has formed its
+//              first P: one's waits and loads then lie under the other's exponentials
 // The maximum is raised, and O and the sum rescaled, only when a block's maximum exceeds it by more than 2^8.
 // Rounding: scores, statistics and accumulators fp32; P to bf16 (relative to m) before it multiplies V, the tensor cores take
 // no wider operand beside bf16 values; one rounding of the output.
@@ -34,11 +38,12 @@ using fa::sts128;
 
 constexpr int TILE = 128;     // query rows of a tile, keys of a block
 constexpr int SLAB = 16384;   // 128 rows x 64 bf16, one swizzled slab
-constexpr int FWD_THREADS = 384;
-// A thread of the softmax holds a row of 128 scores: the launch gives 168 registers to each of the three warpgroups' threads, the
-// loading and issuing one hands 96 of them on (72 + 216 + 216 = 3 * 168).
-constexpr int REGS_CONTROL = 72, REGS_SOFTMAX = 216;
-static_assert(REGS_CONTROL + 2 * REGS_SOFTMAX == 3 * 168, "a split of more registers than the launch has would wait for ever");
+// Forward: 4 warps that load and issue, 8 that compute. A thread of these holds a row of 128 scores: the launch gives 168 registers to each
+// of the three warpgroups' threads, the loading and issuing one hands 96 of them on (72 + 2 * 216 = 3 * 168).
+constexpr int FWD_THREADS = 384, REGS_CONTROL = 72, REGS_SOFTMAX = 216;
+static_assert(REGS_CONTROL + 2 * REGS_SOFTMAX <= 3 * 168, "a split of more registers than the launch has would wait for ever");
+// Backward: 4 warps that load and issue, 16 for the element-wise work.
+constexpr int BWD_THREADS = 640;
 constexpr float LOG2E = 1.4426950408889634f;
 
 enum { ST_Q_EMPTY = 51, ST_KV_EMPTY, ST_Q_FULL, ST_KV_FULL, ST_S_FREE, ST_P, ST_O_FREE, ST_S, ST_PV, ST_FIX };
@@ -65,6 +70,12 @@ struct FwdShape {
   static constexpr size_t smem = 1024 + 2 * (size_t)Q_TILE + 2 * (size_t)P_TILE + SLOTS * (size_t)KV_TILE + sizeof(Tail);
   static_assert(smem <= 232448, "more shared memory than a CTA can be given");
 };
+
+// The units of a persistent CTA: c, 2 G - 1 - c, 2 G + c, ... for G CTAs. Units are numbered from the longest of a sequence on, so
+// that a CTA that took a long one of a round takes a short one of the next.
+__device__ __forceinline__ int unit_at(int round) {
+  return (round & 1) ? (round + 1) * (int)gridDim.x - 1 - (int)blockIdx.x : round * (int)gridDim.x + (int)blockIdx.x;
+}
 
 // Which keys a sequence's rows see.
 struct Span {
@@ -125,6 +136,77 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lbo) {
 }
 __device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 
+// The keys that a row sees in 32 columns, as bits: j <= hi and (j >= lo or j < sinks), all relative to the first column.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
+__device__ __forceinline__ uint32_t seen_bits(int hi, int lo, int sinks) { return low_bits(hi + 1) & (~low_bits(lo) | low_bits(sinks)); }
+// every row of a tile of queries at positions pos0 .. last sees every key of the block
+__device__ __forceinline__ bool all_seen(int base, int pos0, int last, int window, int sinks) {
+  return base + TILE - 1 <= pos0 && (base >= last - window + 1 || base + TILE <= sinks);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// 16 fp32 values times f as bf16 to 32 bytes of global memory: one full sector per thread where the address allows it
+__device__ __forceinline__ void store16(__nv_bfloat16 *dst, const uint32_t *r, float f) {
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 16; j++) v[j] = __uint_as_float(r[j]) * f;
+  const uint4 lo = pack8(v), hi = pack8(v + 8);
+  if ((reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+    st_global_256(dst, lo, hi);
+  } else {
+    reinterpret_cast<uint4 *>(dst)[0] = lo;
+    reinterpret_cast<uint4 *>(dst)[1] = hi;
+  }
+}
+// N fp32 columns of this lane from tensor memory
+template <int N>
+__device__ __forceinline__ void load_columns(uint32_t addr, uint32_t *r) {
+  if (N == 16) {
+    ptx::tmem_ld16(addr, r);
+  } else {
+#pragma unroll
+    for (int q = 0; q < N / 32; q++) ptx::tmem_ld32(addr + q * 32, r + q * 32);
+  }
+  ptx::tmem_ld_wait();
+}
+// 8 N bf16 values of a row into a 128-byte-swizzled slab, from 16-byte chunk `chunk` of the row on
+template <int N>
+__device__ __forceinline__ void store_packed(uint32_t row_addr, int row, int chunk, const uint32_t *v) {
+#pragma unroll
+  for (int q = 0; q < N; q++) sts128(row_addr + (uint32_t)(((chunk + q) ^ (row & 7)) * 16), make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+}
+// the same from fp32
+template <int N>
+__device__ __forceinline__ void store_chunks(uint32_t row_addr, int row, int chunk, const uint32_t *x) {
+  uint32_t v[4 * N];
+#pragma unroll
+  for (int j = 0; j < 4 * N; j++) v[j] = pack_bf16(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+  store_packed<N>(row_addr, row, chunk, v);
+}
+
 // keys of a sequence that none of its queries sees: [sinks, dead_end), and those from Tk on
 __device__ __forceinline__ int dead_end(const Span &sp, int window) { return max(0, sp.shift - window + 1); }
 __device__ __forceinline__ bool has_dead(const Span &sp, int kb, int window, int sinks) {
@@ -147,7 +229,7 @@ __device__ __forceinline__ void zero_dead(uint32_t tile, const Span &sp, int kb,
 template <int HD>
 __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid_constant__ FwdParams p) {
   using Sh = FwdShape<HD>;
-  constexpr int KSL = HD / 64, SLOTS = Sh::SLOTS;
+  constexpr int SLOTS = Sh::SLOTS;
   constexpr uint32_t TMEM_COLS = 512, COL_O = 256;  // S_0, S_1 (128 columns each), then O_0, O_1 (HD each)
   extern __shared__ unsigned char window_smem[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(window_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -170,7 +252,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
     }
     for (int s = 0; s < SLOTS; s++) {
       ptx::mbar_init(bar(&st->kv_full[s]), 1);
-      ptx::mbar_init(bar(&st->kv_empty[s]), 1);
+      ptx::mbar_init(bar(&st->kv_empty[s]), 2);  // V: either tile's issuer; K: twice the one
     }
     ptx::mbar_init(bar(&st->fixed), 1);
     st->abort_flag = 0;
@@ -191,120 +273,140 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
   ptx::tc_fence_after();
   const uint32_t tmem_base = st->tmem_base;
 
+  // The ring: step t of the CTA (counted through its units) uses K at place max(0, 2 t - 1) and V at place 2 t + 2: a unit's first K
+  // goes before the last unit's last V.
+  auto k_at = [](uint32_t t) { return t == 0 ? 0u : 2 * t - 1; };
+  auto v_at = [](uint32_t t) { return 2 * t + 2; };
+
   if (warp < 4) {
     ptx::reg_dec<REGS_CONTROL>();
     if (warp == 0) {
       // ================= loads: the whole warp walks, one lane issues =================
-      int n = 0;
-      uint32_t uq[2] = {0, 0}, fixes = 0;
+      uint32_t t = 0, uq[2] = {0, 0}, fixes = 0;
       bool ok = true;
       auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
-      for (int unit = blockIdx.x; ok && unit < p.units; unit += gridDim.x) {
+      auto load = [&](const CUtensorMap *m, uint32_t n, const Span &sp, int kvh, int kb, bool fix) {
+        const uint32_t slot = n % SLOTS;
+        ok = waitw(&st->kv_empty[slot], n / SLOTS + 1, ST_KV_EMPTY);
+        if (!ok) return;
+        const uint32_t tile = ptx::smem_u32(sKV + slot * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(&st->kv_full[slot]);
+        if (lane == 0) {
+          ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::KV_TILE);
+          ptx::tma_load_3d(tile, m, full, 0, sp.k_off + kb * TILE, kvh * (HD / 64));
+        }
+        if (!fix) return;
+        ok = waitw(&st->fixed, fixes++, ST_FIX);
+        if (!ok) return;
+        zero_dead<HD>(tile, sp, kb, p.window, p.sinks, lane);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(&st->kv_full[slot]));
+      };
+      // the V of the step before
+      Span last_sp;
+      int last_kvh = 0, last_kb = 0;
+      auto load_last_v = [&]() {
+        load(&p.tmV, v_at(t - 1), last_sp, last_kvh, last_kb, has_dead(last_sp, last_kb, p.window, p.sinks));
+      };
+      for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
         const Unit u = unit_of(p, unit);
         const int kvh = u.a.h / p.group;
+        for (int i = 0; ok && i < u.n; i++) {
+          if (i == 0) {  // the last unit's S products still read its Q
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-          const Tile &x = g ? u.b : u.a;
-          if (!ok || !x.exists) continue;
-          ok = waitw(&st->q_empty[g], uq[g] + 1, ST_Q_EMPTY);
-          if (ok && lane == 0) {
-            ptx::mbar_arrive_expect_tx(bar(&st->q_full[g]), (uint32_t)Sh::Q_TILE);
-            for (int s = 0; s < KSL; s++)
-              ptx::tma_load_2d(ptx::smem_u32(sQ + g * Sh::Q_TILE + s * SLAB), &p.tmQ, bar(&st->q_full[g]), x.h * HD + s * 64,
-                               u.sp.q_off + x.row);
+            for (int g = 0; g < 2; g++) {
+              const Tile &x = g ? u.b : u.a;
+              if (!ok || !x.exists) continue;
+              ok = waitw(&st->q_empty[g], uq[g] + 1, ST_Q_EMPTY);
+              if (ok && lane == 0) {
+                ptx::mbar_arrive_expect_tx(bar(&st->q_full[g]), (uint32_t)Sh::Q_TILE);
+                ptx::tma_load_3d(ptx::smem_u32(sQ + g * Sh::Q_TILE), &p.tmQ, bar(&st->q_full[g]), 0, u.sp.q_off + x.row, x.h * (HD / 64));
+              }
+              uq[g]++;
+            }
           }
-          uq[g]++;
+          if (ok) load(&p.tmK, k_at(t), u.sp, kvh, u.block(i), false);
+          if (ok && t > 0) load_last_v();
+          last_sp = u.sp;
+          last_kvh = kvh;
+          last_kb = u.block(i);
+          t++;
         }
-        auto load = [&](const CUtensorMap *m, int kb, bool fix) {
-          const int slot = n % SLOTS;
-          ok = waitw(&st->kv_empty[slot], (uint32_t)(n / SLOTS) + 1, ST_KV_EMPTY);
-          n++;
-          if (!ok) return;
-          const uint32_t tile = ptx::smem_u32(sKV + slot * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(&st->kv_full[slot]);
-          if (lane == 0) {
-            ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::KV_TILE);
-            for (int s = 0; s < KSL; s++) ptx::tma_load_2d(tile + s * SLAB, m, full, kvh * HD + s * 64, u.sp.k_off + kb * TILE);
+      }
+      if (ok && t > 0) load_last_v();
+      __syncwarp();
+    } else if (warp == 1) {
+      // ================= S products =================
+      if (lane == 0) {
+        const uint32_t idesc = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
+        const uint32_t q_base = ptx::smem_u32(sQ), kv_base = ptx::smem_u32(sKV);
+        uint32_t t = 0, uq[2] = {0, 0}, ts[2] = {0, 0};  // steps; units and S products of either tile
+        bool ok = true;
+        for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
+          const Unit u = unit_of(p, unit);
+          if (u.a.exists) ok = wait(&st->q_full[0], uq[0]++, ST_Q_FULL);
+          if (ok && u.b.exists) ok = wait(&st->q_full[1], uq[1]++, ST_Q_FULL);
+          for (int i = 0; ok && i < u.n; i++, t++) {
+            const int kb = u.block(i);
+            const uint32_t n = k_at(t), slot = n % SLOTS;
+            if (!(ok = wait(&st->kv_full[slot], n / SLOTS, ST_KV_FULL))) break;
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+              const Tile &x = g ? u.b : u.a;
+              if (!ok || !x.active(kb, p.sinks)) continue;
+              if (ts[g] > 0 && !(ok = wait(&st->s_read[g], ts[g] - 1, ST_S_FREE))) continue;
+              ptx::tc_fence_after();
+              const uint64_t qd = tile_desc(q_base + g * Sh::Q_TILE, 0), kd = tile_desc(kv_base + slot * Sh::KV_TILE, 0);
+#pragma unroll
+              for (int k16 = 0; k16 < HD / 16; k16++) {
+                const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
+                ptx::umma_bf16(tmem_base + (uint32_t)(g * TILE), desc_at(qd, off), desc_at(kd, off), idesc, k16 > 0);
+              }
+              ptx::umma_commit(bar(&st->s_full[g]));
+              if (kb == x.hi) ptx::umma_commit(bar(&st->q_empty[g]));
+              ts[g]++;
+            }
+            if (!ok) break;
+            ptx::umma_commit(bar(&st->kv_empty[slot]));
+            ptx::mbar_arrive(bar(&st->kv_empty[slot]));
           }
-          if (!fix) return;
-          ok = waitw(&st->fixed, fixes++, ST_FIX);
-          if (!ok) return;
-          zero_dead<HD>(tile, u.sp, kb, p.window, p.sinks, lane);
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(&st->kv_full[slot]));
-        };
-        for (int i = 0; ok && i <= u.n; i++) {
-          if (i < u.n) load(&p.tmK, u.block(i), false);
-          if (ok && i > 0) load(&p.tmV, u.block(i - 1), has_dead(u.sp, u.block(i - 1), p.window, p.sinks));
         }
       }
       __syncwarp();
-    } else if (warp == 1) {
-      // ================= MMA issue =================
+    } else {
+      // ================= P V products of one tile =================
       if (lane == 0) {
-        const uint32_t idesc_s = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
-        const uint32_t idesc_pv = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // V is read with its head dimension contiguous
-        const uint32_t q_base = ptx::smem_u32(sQ), p_base = ptx::smem_u32(sP), kv_base = ptx::smem_u32(sKV);
-        int n = 0;
-        uint32_t uq[2] = {0, 0}, ts[2] = {0, 0}, tp[2] = {0, 0};  // units, S products and P V products of either tile so far
+        const int g = warp - 2;
+        const uint32_t idesc = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // V is read with its head dimension contiguous
+        const uint32_t p_base = ptx::smem_u32(sP + g * Sh::P_TILE), kv_base = ptx::smem_u32(sKV), o_col = tmem_base + COL_O + (uint32_t)(g * HD);
+        uint32_t t = 0, units = 0, tp = 0;  // steps; units and products of this tile
         bool ok = true;
-        for (int unit = blockIdx.x; ok && unit < p.units; unit += gridDim.x) {
+        for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
           const Unit u = unit_of(p, unit);
-          bool begun_s[2] = {false, false}, begun_o[2] = {false, false};
-          for (int i = 0; ok && i <= u.n; i++) {
-            if (i < u.n) {
-              const int slot = n % SLOTS, kb = u.block(i);
-              if (!(ok = wait(&st->kv_full[slot], (uint32_t)(n / SLOTS), ST_KV_FULL))) break;
-              n++;
-#pragma unroll
-              for (int g = 0; g < 2; g++) {
-                const Tile &x = g ? u.b : u.a;
-                if (!ok || !x.active(kb, p.sinks)) continue;
-                if (!begun_s[g]) {
-                  begun_s[g] = true;
-                  if (!(ok = wait(&st->q_full[g], uq[g], ST_Q_FULL))) continue;
-                }
-                if (ts[g] > 0 && !(ok = wait(&st->s_read[g], ts[g] - 1, ST_S_FREE))) continue;
-                ptx::tc_fence_after();
-                const uint64_t qd = tile_desc(q_base + g * Sh::Q_TILE, 0), kd = tile_desc(kv_base + slot * Sh::KV_TILE, 0);
-#pragma unroll
-                for (int k16 = 0; k16 < HD / 16; k16++) {
-                  const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
-                  ptx::umma_bf16(tmem_base + (uint32_t)(g * TILE), desc_at(qd, off), desc_at(kd, off), idesc_s, k16 > 0);
-                }
-                ptx::umma_commit(bar(&st->s_full[g]));
-                if (kb == x.hi) ptx::umma_commit(bar(&st->q_empty[g]));
-                ts[g]++;
-              }
-              if (!ok) break;
-              ptx::umma_commit(bar(&st->kv_empty[slot]));
+          const Tile x = g ? u.b : u.a;
+          bool begun = false;
+          for (int i = 0; ok && i < u.n; i++, t++) {
+            const uint32_t n = v_at(t), slot = n % SLOTS;
+            if (!(ok = wait(&st->kv_full[slot], n / SLOTS, ST_KV_FULL))) break;
+            if (!x.active(u.block(i), p.sinks)) {
+              ptx::mbar_arrive(bar(&st->kv_empty[slot]));
+              continue;
             }
-            if (i > 0) {
-              const int slot = n % SLOTS, kb = u.block(i - 1);
-              if (!(ok = wait(&st->kv_full[slot], (uint32_t)(n / SLOTS), ST_KV_FULL))) break;
-              n++;
+            // P of this step is in shared memory, the group has rescaled O if its maxima grew - and read the last unit's O
+            if (!(ok = wait(&st->p_ready[g], tp, ST_P))) break;
+            if (!begun && units > 0 && !(ok = wait(&st->o_empty[g], units - 1, ST_O_FREE))) break;
+            ptx::tc_fence_after();
+            const uint64_t pd = tile_desc(p_base, 0), vd = tile_desc(kv_base + slot * Sh::KV_TILE, SLAB);
 #pragma unroll
-              for (int g = 0; g < 2; g++) {
-                if (!ok || !(g ? u.b : u.a).active(kb, p.sinks)) continue;
-                // P of this step is in shared memory, the group has rescaled O if its maxima grew - and read the last unit's O
-                if (!(ok = wait(&st->p_ready[g], tp[g], ST_P))) continue;
-                if (!begun_o[g] && uq[g] > 0 && !(ok = wait(&st->o_empty[g], uq[g] - 1, ST_O_FREE))) continue;
-                ptx::tc_fence_after();
-                const uint64_t pd = tile_desc(p_base + g * Sh::P_TILE, 0), vd = tile_desc(kv_base + slot * Sh::KV_TILE, SLAB);
-#pragma unroll
-                for (int k16 = 0; k16 < TILE / 16; k16++)
-                  ptx::umma_bf16(tmem_base + COL_O + (uint32_t)(g * HD), desc_at(pd, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)),
-                                 desc_at(vd, (uint32_t)(k16 * 2048)), idesc_pv, begun_o[g] || k16 > 0);
-                begun_o[g] = true;
-                ptx::umma_commit(bar(&st->pv_done[g]));
-                tp[g]++;
-              }
-              if (!ok) break;
-              ptx::umma_commit(bar(&st->kv_empty[slot]));
-            }
+            for (int k16 = 0; k16 < TILE / 16; k16++)
+              ptx::umma_bf16(o_col, desc_at(pd, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)), desc_at(vd, (uint32_t)(k16 * 2048)), idesc,
+                             begun || k16 > 0);
+            begun = true;
+            ptx::umma_commit(bar(&st->pv_done[g]));
+            ptx::umma_commit(bar(&st->kv_empty[slot]));
+            tp++;
           }
-          uq[0] += u.a.exists;
-          uq[1] += u.b.exists;
+          units += x.exists;
         }
       }
       __syncwarp();
@@ -319,13 +421,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
     const uint32_t p_addr = ptx::smem_u32(sP + g * Sh::P_TILE + trow * 128);
     const float c = p.scale * LOG2E;
     uint32_t t = 0;  // steps of this tile so far
-    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+    if (g == 1 && !wait(&st->p_ready[0], 0, ST_P)) goto teardown;  // the first tile of a CTA's first unit always exists
+    for (int round = 0, unit = unit_at(0); unit < p.units; unit = unit_at(++round)) {
       const Unit u = unit_of(p, unit);
       const Tile x = g ? u.b : u.a;
       if (!x.exists) continue;
       const int row = x.row + trow, pos = row + u.sp.shift;
       const int tile_pos = x.row + u.sp.shift, last_pos = min(tile_pos + TILE, u.sp.Tk) - 1;
-      const int hi = min(pos, u.sp.Tk - 1), lo = pos - p.window + 1;  // the keys this row sees, besides the sinks
       float m = -INFINITY, l = 0.0f;
       bool first = true;
       for (int i = 0; i < u.n; i++) {
@@ -334,71 +436,63 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         if (!wait(&st->s_full[g], t, ST_S)) goto teardown;
         ptx::tc_fence_after();
         uint32_t s[TILE];
-#pragma unroll
-        for (int q = 0; q < 4; q++) ptx::tmem_ld32(s_addr + q * 32, s + q * 32);
-        ptx::tmem_ld_wait();
+        load_columns<TILE>(s_addr, s);
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->s_read[g]));
-        const int base = kb * TILE;
-        // every row of the tile sees every key of the block: the window reaches back from the last row to the block's start
-        const bool whole = base + TILE - 1 <= tile_pos && (base >= last_pos - p.window + 1 || base + TILE <= p.sinks);
-        if (!whole) {
+        if (!all_seen(kb * TILE, tile_pos, last_pos, p.window, p.sinks)) {
+          const int base = kb * TILE, hi = min(pos, u.sp.Tk - 1) - base, lo = pos - p.window + 1 - base, sk = p.sinks - base;
 #pragma unroll
-          for (int j = 0; j < TILE; j++) {
-            const int key = base + j;
-            if (!(key <= hi && (key >= lo || key < p.sinks))) s[j] = 0xff800000u;  // -infinity
+          for (int q = 0; q < 4; q++) {
+            const uint32_t see = seen_bits(hi - 32 * q, lo - 32 * q, sk - 32 * q);
+#pragma unroll
+            for (int j = 0; j < 32; j++) s[q * 32 + j] = (see >> j) & 1u ? s[q * 32 + j] : 0xff800000u;  // -infinity
           }
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < TILE; j++) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s[j]));
+        for (int j = 0; j < TILE; j += 2) mx4[(j >> 1) & 3] = max3(mx4[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        float alpha = 1.0f;
         if (first) {
           m = mx;
-        } else {
-          const bool grow = (mx - m) * c > 8.0f;
-          if (__any_sync(0xffffffffu, grow)) {  // tensor-memory accesses are warp-wide: every lane takes part
-            const float m_new = grow ? mx : m;
-            // 1 for the lanes that keep their offset; a row that had seen nothing has nothing to rescale
-            const float alpha = (m == -INFINITY || !grow) ? 1.0f : ex2((m - m_new) * c);
-            if (!wait(&st->pv_done[g], t - 1, ST_PV)) goto teardown;
-            ptx::tc_fence_after();
-#pragma unroll
-            for (int q = 0; q < HD / 32; q++) {
-              uint32_t r[32];
-              ptx::tmem_ld32(o_addr + q * 32, r);
-              ptx::tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; j++) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
-              ptx::tmem_st32(o_addr + q * 32, r);
-            }
-            ptx::tmem_st_wait();
-            l *= alpha;
-            m = m_new;
-          }
+        } else if ((mx - m) * c > 8.0f) {
+          // a row that had seen nothing has nothing to rescale
+          if (m != -INFINITY) alpha = ex2((m - mx) * c);
+          m = mx;
+          l *= alpha;
         }
         // a row that has seen no key yet keeps m = -inf: its probabilities are exp2(-inf) = 0 against a zero offset
         const float mc = (m == -INFINITY) ? 0.0f : m * c;
-        float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t cc = pack2(c, c), off = pack2(-mc, -mc);
+        uint64_t sum2[2] = {0, 0};
+        uint32_t pk[TILE / 2];
 #pragma unroll
-        for (int j = 0; j < TILE; j++) {
-          const float e = ex2(fmaf(__uint_as_float(s[j]), c, -mc));
-          sum4[j & 3] += e;
-          s[j] = __float_as_uint(e);
+        for (int j = 0; j < TILE; j += 2) {
+          float x0, x1;
+          unpack2(fma2(pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), cc, off), x0, x1);
+          const float e0 = ex2(x0), e1 = ex2(x1);
+          sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pack2(e0, e1));
+          pk[j >> 1] = pack_bf16(e0, e1);
         }
-        l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-        // the step before has read P
+        float sa, sb;
+        unpack2(add2(sum2[0], sum2[1]), sa, sb);
+        l += sa + sb;
+        // the step before has read P, and O is at rest
         if (t > 0 && !wait(&st->pv_done[g], t - 1, ST_PV)) goto teardown;
+        if (__any_sync(0xffffffffu, alpha != 1.0f)) {  // tensor-memory accesses are warp-wide: every lane takes part
+          ptx::tc_fence_after();
 #pragma unroll
-        for (int q = 0; q < 16; q++) {
-          // keys 8 q .. 8 q + 7 of this row: slab q / 8, 16-byte chunk q % 8, swizzled with the row
-          uint4 v;
-          v.x = pack_bf16(__uint_as_float(s[q * 8 + 0]), __uint_as_float(s[q * 8 + 1]));
-          v.y = pack_bf16(__uint_as_float(s[q * 8 + 2]), __uint_as_float(s[q * 8 + 3]));
-          v.z = pack_bf16(__uint_as_float(s[q * 8 + 4]), __uint_as_float(s[q * 8 + 5]));
-          v.w = pack_bf16(__uint_as_float(s[q * 8 + 6]), __uint_as_float(s[q * 8 + 7]));
-          sts128(p_addr + (uint32_t)((q >> 3) * SLAB + (((q & 7) ^ (trow & 7)) * 16)), v);
+          for (int q = 0; q < HD / 32; q++) {
+            uint32_t r[32];
+            load_columns<32>(o_addr + q * 32, r);
+#pragma unroll
+            for (int j = 0; j < 32; j++) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+            ptx::tmem_st32(o_addr + q * 32, r);
+          }
+          ptx::tmem_st_wait();
         }
+        store_packed<8>(p_addr, trow, 0, pk);
+        store_packed<8>(p_addr + SLAB, trow, 0, pk + 32);
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->p_ready[g]));
@@ -408,21 +502,14 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
       if (!wait(&st->pv_done[g], t - 1, ST_PV)) goto teardown;
       ptx::tc_fence_after();
       uint32_t r[HD];
-#pragma unroll
-      for (int q = 0; q < HD / 32; q++) ptx::tmem_ld32(o_addr + q * 32, r + q * 32);
-      ptx::tmem_ld_wait();
+      load_columns<HD>(o_addr, r);
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->o_empty[g]));
       if (row < u.sp.Tq) {
         const float inv = 1.0f / l;
-        uint4 *o = reinterpret_cast<uint4 *>(p.O + ((int64_t)(u.sp.q_off + row) * p.q_heads + x.h) * HD);
+        __nv_bfloat16 *o = p.O + ((int64_t)(u.sp.q_off + row) * p.q_heads + x.h) * HD;
 #pragma unroll
-        for (int q = 0; q < HD / 8; q++) {
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) v[j] = __uint_as_float(r[q * 8 + j]) * inv;
-          o[q] = pack8(v);
-        }
+        for (int q = 0; q < HD / 16; q++) store16(o + q * 16, r + q * 16, inv);
         p.lse[(int64_t)x.h * p.total_q + u.sp.q_off + row] = m * p.scale + logf(l);
       }
     }
@@ -461,7 +548,6 @@ teardown:
 // What bounds both: shared memory. A 128 x 128 x 128 product reads 64 KB of operands in the 512 cycles that it takes, all that
 // shared memory gives; writing P and dS and the tiles that arrive come on top.
 // ---------------------------------------------------------------------------------------------------------------------------
-constexpr int BWD_THREADS = 320;  // warp 0 loads, warp 1 issues the MMAs, 8 warps for the element-wise work
 constexpr int DS_TILE = TILE * TILE * 2;
 
 enum { ST_BQ_Q = 61, ST_BQ_KV_EMPTY, ST_BQ_Q_FULL, ST_BQ_KV_FULL, ST_BQ_S_FREE, ST_BQ_DP_FREE, ST_BQ_DS, ST_BQ_ACC, ST_BQ_STAT, ST_BQ_S, ST_BQ_DP,
@@ -484,12 +570,6 @@ struct BwdParams {
   int *status;
 };
 
-// eight scores of a row, scaled, against its log-sum-exp: the probabilities; `seen` masks
-struct Seen {
-  int hi, lo, sinks;  // keys of the block (relative to its start) that a row sees: j <= hi and (j >= lo or j < sinks)
-  __device__ __forceinline__ bool operator()(int j) const { return j <= hi && (j >= lo || j < sinks); }
-};
-
 template <int HD>
 struct BwdQShape {
   static constexpr int Q_TILE = TILE * HD * 2, KV_TILE = TILE * HD * 2;
@@ -498,7 +578,7 @@ struct BwdQShape {
     uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full, s_read, dp_full, dp_read, ds_ready, dq_done, acc_empty, stat, fixed;
     uint32_t tmem_base;
     int abort_flag;
-    float part[2][TILE];
+    float delta[TILE];
   };
   static constexpr size_t smem = 1024 + 2 * (size_t)Q_TILE + DS_TILE + SLOTS * (size_t)KV_TILE + sizeof(Tail);
   static_assert(smem <= 232448, "more shared memory than a CTA can be given");
@@ -523,15 +603,10 @@ __device__ __forceinline__ QUnit q_unit_of(const BwdParams &p, int unit) {
   return u;
 }
 
-// every row of a tile of queries at positions pos0 .. last sees every key of the block
-__device__ __forceinline__ bool all_seen(int base, int pos0, int last, int window, int sinks) {
-  return base + TILE - 1 <= pos0 && (base >= last - window + 1 || base + TILE <= sinks);
-}
-
 template <int HD>
 __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __grid_constant__ BwdParams p) {
   using Sh = BwdQShape<HD>;
-  constexpr int KSL = HD / 64, SLOTS = Sh::SLOTS;
+  constexpr int SLOTS = Sh::SLOTS;
   constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256;
   extern __shared__ unsigned char window_smem[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(window_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -544,19 +619,19 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
 
   if (tid == 0) {
     ptx::mbar_init(bar(&st->q_full), 1);
-    ptx::mbar_init(bar(&st->q_empty), 1);
+    ptx::mbar_init(bar(&st->q_empty), 2);  // the last S and the last dP of a unit
     for (int s = 0; s < SLOTS; s++) {
       ptx::mbar_init(bar(&st->kv_full[s]), 1);
       ptx::mbar_init(bar(&st->kv_empty[s]), 1);
     }
     ptx::mbar_init(bar(&st->s_full), 1);
-    ptx::mbar_init(bar(&st->s_read), 256);
+    ptx::mbar_init(bar(&st->s_read), 512);
     ptx::mbar_init(bar(&st->dp_full), 1);
-    ptx::mbar_init(bar(&st->dp_read), 256);
-    ptx::mbar_init(bar(&st->ds_ready), 256);
+    ptx::mbar_init(bar(&st->dp_read), 512);
+    ptx::mbar_init(bar(&st->ds_ready), 512);
     ptx::mbar_init(bar(&st->dq_done), 1);
-    ptx::mbar_init(bar(&st->acc_empty), 256);
-    ptx::mbar_init(bar(&st->stat), 256);
+    ptx::mbar_init(bar(&st->acc_empty), 512);
+    ptx::mbar_init(bar(&st->stat), 512);
     ptx::mbar_init(bar(&st->fixed), 1);
     st->abort_flag = 0;
     ptx::fence_barrier_init();
@@ -579,25 +654,23 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
 
   if (warp == 0) {
     // ================= loads: the whole warp walks, one lane issues =================
-    int n = 0;
-    uint32_t units = 0, fixes = 0;
+    uint32_t n = 0, units = 0, fixes = 0;
     bool ok = true;
     auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
-    for (int unit = blockIdx.x; ok && unit < p.units; unit += gridDim.x) {
+    for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
       const QUnit u = q_unit_of(p, unit);
       const int kvh = u.x.h / p.group;
       ok = waitw(&st->q_empty, units + 1, ST_BQ_Q);
       units++;
       if (ok && lane == 0) {
         ptx::mbar_arrive_expect_tx(bar(&st->q_full), (uint32_t)(2 * Sh::Q_TILE));
-        for (int s = 0; s < KSL; s++) {
-          ptx::tma_load_2d(ptx::smem_u32(sQ + s * SLAB), &p.tmQ, bar(&st->q_full), u.x.h * HD + s * 64, u.sp.q_off + u.x.row);
-          ptx::tma_load_2d(ptx::smem_u32(sDO + s * SLAB), &p.tmdO, bar(&st->q_full), u.x.h * HD + s * 64, u.sp.q_off + u.x.row);
-        }
+        ptx::tma_load_3d(ptx::smem_u32(sQ), &p.tmQ, bar(&st->q_full), 0, u.sp.q_off + u.x.row, u.x.h * (HD / 64));
+        ptx::tma_load_3d(ptx::smem_u32(sDO), &p.tmdO, bar(&st->q_full), 0, u.sp.q_off + u.x.row, u.x.h * (HD / 64));
       }
       for (int i = 0; ok && i < 2 * u.n; i++) {  // K_0, V_0, K_1, V_1, ...
-        const int slot = n % SLOTS, kb = u.block(i >> 1);
-        ok = waitw(&st->kv_empty[slot], (uint32_t)(n / SLOTS) + 1, ST_BQ_KV_EMPTY);
+        const uint32_t slot = n % SLOTS;
+        const int kb = u.block(i >> 1);
+        ok = waitw(&st->kv_empty[slot], n / SLOTS + 1, ST_BQ_KV_EMPTY);
         n++;
         if (!ok) break;
         // K multiplies dS: rows that no query sees have to be zero there. What they make of S and dP is dropped by a select.
@@ -605,8 +678,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
         const uint32_t tile = ptx::smem_u32(sKV + slot * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(&st->kv_full[slot]);
         if (lane == 0) {
           ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::KV_TILE);
-          for (int s = 0; s < KSL; s++)
-            ptx::tma_load_2d(tile + s * SLAB, (i & 1) ? &p.tmV : &p.tmK, full, kvh * HD + s * 64, u.sp.k_off + kb * TILE);
+          ptx::tma_load_3d(tile, (i & 1) ? &p.tmV : &p.tmK, full, 0, u.sp.k_off + kb * TILE, kvh * (HD / 64));
         }
         if (!fix) continue;
         ok = waitw(&st->fixed, fixes++, ST_FIX);
@@ -618,147 +690,135 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
-    // ================= MMA issue =================
+  } else if (warp < 3) {
+    // ================= S = Q K^T (warp 1) and dP = dO V^T (warp 2) =================
     if (lane == 0) {
-      const uint32_t idesc_s = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
-      const uint32_t idesc_dq = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // K is read with its head dimension contiguous
-      const uint32_t q_base = ptx::smem_u32(sQ), do_base = ptx::smem_u32(sDO), ds_base = ptx::smem_u32(sDS), kv_base = ptx::smem_u32(sKV);
-      uint32_t t = 0, units = 0;  // steps and units so far
+      const bool is_s = warp == 1;
+      const uint32_t idesc = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
+      const uint32_t a_base = ptx::smem_u32(is_s ? sQ : sDO), kv_base = ptx::smem_u32(sKV), col = tmem_base + (is_s ? COL_S : COL_DP);
+      uint64_t *full = is_s ? &st->s_full : &st->dp_full, *read = is_s ? &st->s_read : &st->dp_read;
+      uint32_t t = 0, units = 0;
       bool ok = true;
-      // dQ of the step before: issued after S and dP of the current one, across units too
-      bool pending = false, pending_first = false;
-      auto issue_dq = [&]() {
-        const uint32_t tp = t - 1;
-        ok = wait(&st->ds_ready, tp, ST_BQ_DS);
-        // the first of a unit overwrites the accumulator: the threads have read the unit before
-        if (ok && pending_first && units > 1) ok = wait(&st->acc_empty, units - 2, ST_BQ_ACC);
-        if (!ok) return;
-        ptx::tc_fence_after();
-        const int slot = (int)((2 * tp) % SLOTS);
-        const uint64_t ad = tile_desc(ds_base, 0), bd = tile_desc(kv_base + slot * Sh::KV_TILE, SLAB);
-#pragma unroll
-        for (int k16 = 0; k16 < TILE / 16; k16++)
-          ptx::umma_bf16(tmem_base + COL_DQ, desc_at(ad, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)), desc_at(bd, (uint32_t)(k16 * 2048)),
-                         idesc_dq, !pending_first || k16 > 0);
-        ptx::umma_commit(bar(&st->dq_done));
-        ptx::umma_commit(bar(&st->kv_empty[slot]));
-      };
-      for (int unit = blockIdx.x; ok && unit < p.units; unit += gridDim.x) {
-        const QUnit u = q_unit_of(p, unit);
-        ok = wait(&st->q_full, units, ST_BQ_Q_FULL);
-        for (int i = 0; ok && i < u.n; i++) {
-          const int ks = (int)((2 * t) % SLOTS), vs = (int)((2 * t + 1) % SLOTS);
-          if (!(ok = wait(&st->kv_full[ks], 2 * t / SLOTS, ST_BQ_KV_FULL))) break;
-          if (t > 0 && !(ok = wait(&st->s_read, t - 1, ST_BQ_S_FREE))) break;
+      for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
+        const int steps = q_unit_of(p, unit).n;
+        ok = wait(&st->q_full, units++, ST_BQ_Q_FULL);
+        for (int i = 0; ok && i < steps; i++, t++) {
+          const uint32_t n = 2 * t + (is_s ? 0 : 1), slot = n % SLOTS;
+          if (!(ok = wait(&st->kv_full[slot], n / SLOTS, ST_BQ_KV_FULL))) break;
+          if (t > 0 && !(ok = wait(read, t - 1, ST_BQ_S_FREE))) break;
           ptx::tc_fence_after();
-          {
-            const uint64_t ad = tile_desc(q_base, 0), bd = tile_desc(kv_base + ks * Sh::KV_TILE, 0);
+          const uint64_t ad = tile_desc(a_base, 0), bd = tile_desc(kv_base + slot * Sh::KV_TILE, 0);
 #pragma unroll
-            for (int k16 = 0; k16 < HD / 16; k16++) {
-              const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
-              ptx::umma_bf16(tmem_base + COL_S, desc_at(ad, off), desc_at(bd, off), idesc_s, k16 > 0);
-            }
-            ptx::umma_commit(bar(&st->s_full));
+          for (int k16 = 0; k16 < HD / 16; k16++) {
+            const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
+            ptx::umma_bf16(col, desc_at(ad, off), desc_at(bd, off), idesc, k16 > 0);
           }
-          if (!(ok = wait(&st->kv_full[vs], (2 * t + 1) / SLOTS, ST_BQ_KV_FULL))) break;
-          if (t > 0 && !(ok = wait(&st->dp_read, t - 1, ST_BQ_DP_FREE))) break;
-          ptx::tc_fence_after();
-          {
-            const uint64_t ad = tile_desc(do_base, 0), bd = tile_desc(kv_base + vs * Sh::KV_TILE, 0);
-#pragma unroll
-            for (int k16 = 0; k16 < HD / 16; k16++) {
-              const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
-              ptx::umma_bf16(tmem_base + COL_DP, desc_at(ad, off), desc_at(bd, off), idesc_s, k16 > 0);
-            }
-            ptx::umma_commit(bar(&st->dp_full));
-            ptx::umma_commit(bar(&st->kv_empty[vs]));
-            if (i == u.n - 1) ptx::umma_commit(bar(&st->q_empty));
-          }
-          if (pending) issue_dq();
-          if (!ok) break;
-          t++;
-          pending = true;
-          pending_first = i == 0;
-          if (i == 0) units++;
+          ptx::umma_commit(bar(full));
+          if (!is_s) ptx::umma_commit(bar(&st->kv_empty[slot]));  // K is read again by the dQ product
+          if (i == steps - 1) ptx::umma_commit(bar(&st->q_empty));
         }
       }
-      if (ok && pending) issue_dq();
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ================= dQ += dS K =================
+    if (lane == 0) {
+      const uint32_t idesc = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // K is read with its head dimension contiguous
+      const uint32_t ds_base = ptx::smem_u32(sDS), kv_base = ptx::smem_u32(sKV);
+      uint32_t t = 0, units = 0;
+      bool ok = true;
+      for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round), units++) {
+        const int steps = q_unit_of(p, unit).n;
+        for (int i = 0; ok && i < steps; i++, t++) {
+          const uint32_t slot = (2 * t) % SLOTS;
+          // dS is in shared memory, which the threads formed from S: K has landed
+          if (!(ok = wait(&st->ds_ready, t, ST_BQ_DS))) break;
+          // the first of a unit overwrites the accumulator: the threads have read the unit before
+          if (i == 0 && units > 0 && !(ok = wait(&st->acc_empty, units - 1, ST_BQ_ACC))) break;
+          if (!(ok = wait(&st->kv_full[slot], 2 * t / SLOTS, ST_BQ_KV_FULL))) break;
+          ptx::tc_fence_after();
+          const uint64_t ad = tile_desc(ds_base, 0), bd = tile_desc(kv_base + slot * Sh::KV_TILE, SLAB);
+#pragma unroll
+          for (int k16 = 0; k16 < TILE / 16; k16++)
+            ptx::umma_bf16(tmem_base + COL_DQ, desc_at(ad, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)), desc_at(bd, (uint32_t)(k16 * 2048)),
+                           idesc, i > 0 || k16 > 0);
+          ptx::umma_commit(bar(&st->dq_done));
+          ptx::umma_commit(bar(&st->kv_empty[slot]));
+        }
+      }
     }
     __syncwarp();
   } else {
-    // ================= element-wise work: a thread per (query row, half of the columns) =================
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    // ================= element-wise work: a thread per (query row, quarter of the columns) =================
+    const int quarter = warp & 3, cols = (warp - 4) >> 2;  // columns 32 * cols ...
     const int trow = quarter * 32 + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t ds_addr = ptx::smem_u32(sDS + half * SLAB + trow * 128);
+    const uint32_t ds_addr = ptx::smem_u32(sDS + (cols >> 1) * SLAB + trow * 128);
     const float c = p.scale * LOG2E;
     uint32_t t = 0, units = 0;
-    for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
+    for (int round = 0, unit = unit_at(0); unit < p.units; unit = unit_at(++round)) {
       const QUnit u = q_unit_of(p, unit);
       const int row = u.x.row + trow, pos = row + u.sp.shift;
       const bool valid = row < u.sp.Tq;
-      const int64_t at = ((int64_t)(u.sp.q_off + row) * p.q_heads + u.x.h) * HD, stat = (int64_t)u.x.h * p.total_q + u.sp.q_off + row;
-      // delta: either thread of a row takes half of the dimensions
-      float lse2 = 0.0f, delta = 0.0f;
-      if (valid) {
-        lse2 = p.lse[stat] * LOG2E;
-        const uint4 *a = reinterpret_cast<const uint4 *>(p.dout + at + half * (HD / 2)), *b = reinterpret_cast<const uint4 *>(p.o + at + half * (HD / 2));
+      const int64_t stat = (int64_t)u.x.h * p.total_q + u.sp.q_off + row;
+      const float lse2 = valid ? p.lse[stat] * LOG2E : 0.0f;
+      {
+        // delta = dO . O: this warp takes eight rows of the tile, HD / 8 lanes a row
+        constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES;
+        const int first = (warp - 4) * 8 + lane / LANES;
+        float d[8 / AT_ONCE];
 #pragma unroll
-        for (int q = 0; q < HD / 16; q++) {
-          float x[8], y[8];
-          unpack8(a[q], x);
-          unpack8(b[q], y);
+        for (int q = 0; q < 8 / AT_ONCE; q++) {
+          const int r = u.x.row + first + q * AT_ONCE;
+          d[q] = 0.0f;
+          if (r < u.sp.Tq) {
+            const int64_t at = ((int64_t)(u.sp.q_off + r) * p.q_heads + u.x.h) * LANES + lane % LANES;
+            float x[8], y[8];
+            unpack8(reinterpret_cast<const uint4 *>(p.dout)[at], x);
+            unpack8(reinterpret_cast<const uint4 *>(p.o)[at], y);
 #pragma unroll
-          for (int j = 0; j < 8; j++) delta = fmaf(x[j], y[j], delta);
+            for (int j = 0; j < 8; j++) d[q] = fmaf(x[j], y[j], d[q]);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 8 / AT_ONCE; q++) {
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) d[q] += __shfl_xor_sync(0xffffffffu, d[q], o);
+          if (lane % LANES == 0) st->delta[first + q * AT_ONCE] = d[q];
         }
       }
-      st->part[half][trow] = delta;
       ptx::mbar_arrive(bar(&st->stat));
       if (!wait(&st->stat, units, ST_BQ_STAT)) goto teardown;
       units++;
-      delta = st->part[0][trow] + st->part[1][trow];
-      if (valid && half == 0) p.delta[stat] = delta;
+      const float delta = st->delta[trow];
+      if (valid && cols == 0) p.delta[stat] = delta;
       const int pos0 = u.x.row + u.sp.shift, last_pos = min(pos0 + TILE, u.sp.Tk) - 1;
       for (int i = 0; i < u.n; i++) {
-        const int base = u.block(i) * TILE + half * 64;
-        const bool whole = all_seen(u.block(i) * TILE, pos0, last_pos, p.window, p.sinks);
-        const Seen seen{min(pos, u.sp.Tk - 1) - base, pos - p.window + 1 - base, p.sinks - base};
-        uint32_t s[64];
+        const int kb = u.block(i);
+        uint32_t s[32], d[32];
         if (!wait(&st->s_full, t, ST_BQ_S)) goto teardown;
         ptx::tc_fence_after();
-        ptx::tmem_ld32(lane_addr + COL_S + half * 64, s);
-        ptx::tmem_ld32(lane_addr + COL_S + half * 64 + 32, s + 32);
-        ptx::tmem_ld_wait();
+        load_columns<32>(lane_addr + COL_S + cols * 32, s);
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->s_read));
 #pragma unroll
-        for (int j = 0; j < 64; j++) s[j] = __float_as_uint(ex2(fmaf(__uint_as_float(s[j]), c, -lse2)));
-        uint32_t d[64];
+        for (int j = 0; j < 32; j++) s[j] = __float_as_uint(ex2(fmaf(__uint_as_float(s[j]), c, -lse2)));
         if (!wait(&st->dp_full, t, ST_BQ_DP)) goto teardown;
         ptx::tc_fence_after();
-        ptx::tmem_ld32(lane_addr + COL_DP + half * 64, d);
-        ptx::tmem_ld32(lane_addr + COL_DP + half * 64 + 32, d + 32);
-        ptx::tmem_ld_wait();
+        load_columns<32>(lane_addr + COL_DP + cols * 32, d);
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->dp_read));
 #pragma unroll
-        for (int j = 0; j < 64; j++) d[j] = __float_as_uint(__uint_as_float(s[j]) * (__uint_as_float(d[j]) - delta));
-        if (!whole) {
+        for (int j = 0; j < 32; j++) d[j] = __float_as_uint(__uint_as_float(s[j]) * (__uint_as_float(d[j]) - delta));
+        if (!all_seen(kb * TILE, pos0, last_pos, p.window, p.sinks)) {
+          const int base = kb * TILE + cols * 32;
+          const uint32_t see = seen_bits(min(pos, u.sp.Tk - 1) - base, pos - p.window + 1 - base, p.sinks - base);
 #pragma unroll
-          for (int j = 0; j < 64; j++) d[j] = seen(j) ? d[j] : 0u;
+          for (int j = 0; j < 32; j++) d[j] = (see >> j) & 1u ? d[j] : 0u;
         }
         // the product of the step before has read dS
         if (t > 0 && !wait(&st->dq_done, t - 1, ST_BQ_DQ)) goto teardown;
-#pragma unroll
-        for (int q = 0; q < 8; q++) {
-          uint4 v;
-          v.x = pack_bf16(__uint_as_float(d[q * 8 + 0]), __uint_as_float(d[q * 8 + 1]));
-          v.y = pack_bf16(__uint_as_float(d[q * 8 + 2]), __uint_as_float(d[q * 8 + 3]));
-          v.z = pack_bf16(__uint_as_float(d[q * 8 + 4]), __uint_as_float(d[q * 8 + 5]));
-          v.w = pack_bf16(__uint_as_float(d[q * 8 + 6]), __uint_as_float(d[q * 8 + 7]));
-          sts128(ds_addr + (uint32_t)((q ^ (trow & 7)) * 16), v);
-        }
+        store_chunks<4>(ds_addr, trow, (cols & 1) * 4, d);
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->ds_ready));
@@ -766,21 +826,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
       }
       if (!wait(&st->dq_done, t - 1, ST_BQ_DQ)) goto teardown;
       ptx::tc_fence_after();
-      uint32_t r[HD / 2];
-#pragma unroll
-      for (int q = 0; q < HD / 64; q++) ptx::tmem_ld32(lane_addr + COL_DQ + half * (HD / 2) + q * 32, r + q * 32);
-      ptx::tmem_ld_wait();
+      uint32_t r[HD / 4];
+      load_columns<HD / 4>(lane_addr + COL_DQ + cols * (HD / 4), r);
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->acc_empty));
       if (valid) {
-        uint4 *o = reinterpret_cast<uint4 *>(p.dq + at + half * (HD / 2));
+        __nv_bfloat16 *o = p.dq + ((int64_t)(u.sp.q_off + row) * p.q_heads + u.x.h) * HD + cols * (HD / 4);
 #pragma unroll
-        for (int q = 0; q < HD / 16; q++) {
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) v[j] = __uint_as_float(r[q * 8 + j]) * p.scale;
-          o[q] = pack8(v);
-        }
+        for (int q = 0; q < HD / 64; q++) store16(o + q * 16, r + q * 16, p.scale);
       }
     }
   }
@@ -867,14 +920,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
     }
     for (int s = 0; s < DS; s++) {
       ptx::mbar_init(bar(&st->do_full[s]), 1);
-      ptx::mbar_init(bar(&st->do_empty[s]), 1);
+      ptx::mbar_init(bar(&st->do_empty[s]), 2);  // dP and dV
     }
     ptx::mbar_init(bar(&st->s_full), 1);
-    ptx::mbar_init(bar(&st->s_read), 256);
+    ptx::mbar_init(bar(&st->s_read), 512);
     ptx::mbar_init(bar(&st->dp_full), 1);
-    ptx::mbar_init(bar(&st->dp_read), 256);
-    ptx::mbar_init(bar(&st->p_ready), 256);
-    ptx::mbar_init(bar(&st->ds_ready), 256);
+    ptx::mbar_init(bar(&st->dp_read), 512);
+    ptx::mbar_init(bar(&st->p_ready), 512);
+    ptx::mbar_init(bar(&st->ds_ready), 512);
     ptx::mbar_init(bar(&st->dv_done), 1);
     ptx::mbar_init(bar(&st->dk_done), 1);
     ptx::mbar_init(bar(&st->fixed), 1);
@@ -934,10 +987,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
     auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
     if (lane == 0) {
       ptx::mbar_arrive_expect_tx(bar(&st->kv_full), (uint32_t)(2 * Sh::T_TILE));
-      for (int q = 0; q < KSL; q++) {
-        ptx::tma_load_2d(ptx::smem_u32(sK + q * SLAB), &p.tmK, bar(&st->kv_full), kvh * HD + q * 64, sp.k_off + kb * TILE);
-        ptx::tma_load_2d(ptx::smem_u32(sV + q * SLAB), &p.tmV, bar(&st->kv_full), kvh * HD + q * 64, sp.k_off + kb * TILE);
-      }
+      ptx::tma_load_3d(ptx::smem_u32(sK), &p.tmK, bar(&st->kv_full), 0, sp.k_off + kb * TILE, kvh * KSL);
+      ptx::tma_load_3d(ptx::smem_u32(sV), &p.tmV, bar(&st->kv_full), 0, sp.k_off + kb * TILE, kvh * KSL);
     }
     for (int i = 0; ok && i < n; i++) {
       const int h = kvh * p.group + i / tiles, row = (t0 + i % tiles) * TILE;
@@ -952,8 +1003,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
         const uint32_t tile = ptx::smem_u32((which == 0 ? sQ : sDO) + slot * Sh::T_TILE), full = fix ? bar(&st->fixed) : bar(full_b);
         if (lane == 0) {
           ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::T_TILE);
-          for (int q = 0; q < KSL; q++)
-            ptx::tma_load_2d(tile + q * SLAB, which == 0 ? &p.tmQ : &p.tmdO, full, h * HD + q * 64, sp.q_off + row);
+          ptx::tma_load_3d(tile, which == 0 ? &p.tmQ : &p.tmdO, full, 0, sp.q_off + row, h * KSL);
         }
         if (!fix) continue;
         ok = waitw(&st->fixed, fixes++, ST_BK_FIX);
@@ -970,69 +1020,62 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
     }
     __syncwarp();
   } else if (n > 0 && warp == 1) {
-    // ================= MMA issue =================
+    // ================= S = Q K^T, dP = dO V^T =================
     if (lane == 0) {
-      const uint32_t idesc_s = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
-      const uint32_t idesc_t = ptx::make_idesc_bf16(TILE, HD, 1, 1);  // both operands with their rows as the reduction
-      const uint32_t k_base = ptx::smem_u32(sK), v_base = ptx::smem_u32(sV), p_base = ptx::smem_u32(sP), ds_base = ptx::smem_u32(sDS),
-                     q_base = ptx::smem_u32(sQ), do_base = ptx::smem_u32(sDO);
-      auto rows_product = [&](uint32_t a, uint32_t b, uint32_t col) {  // [queries x head_dim] [keys x head_dim]^T
+      const uint32_t idesc = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
+      auto product = [&](uint32_t a, uint32_t b, uint32_t col) {
         const uint64_t ad = tile_desc(a, 0), bd = tile_desc(b, 0);
 #pragma unroll
         for (int k16 = 0; k16 < HD / 16; k16++) {
           const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
-          ptx::umma_bf16(tmem_base + col, desc_at(ad, off), desc_at(bd, off), idesc_s, k16 > 0);
+          ptx::umma_bf16(tmem_base + col, desc_at(ad, off), desc_at(bd, off), idesc, k16 > 0);
         }
       };
-      auto reduce_rows = [&](uint32_t a, uint32_t b, uint32_t col, bool add) {  // [queries x keys]^T [queries x head_dim]
-        const uint64_t ad = tile_desc(a, SLAB), bd = tile_desc(b, SLAB);
-#pragma unroll
-        for (int k16 = 0; k16 < TILE / 16; k16++)
-          ptx::umma_bf16(tmem_base + col, desc_at(ad, (uint32_t)(k16 * 2048)), desc_at(bd, (uint32_t)(k16 * 2048)), idesc_t, add || k16 > 0);
-      };
-      auto q_tile = [&](int i) { return q_base + (uint32_t)(i % QS) * Sh::T_TILE; };
-      auto do_tile = [&](int i) { return do_base + (uint32_t)(i % DS) * Sh::T_TILE; };
-      auto issue_s = [&](int i) {
-        if (!wait(&st->q_full[i % QS], (uint32_t)(i / QS), ST_BK_Q)) return false;
-        if (i > 0 && !wait(&st->s_read, (uint32_t)(i - 1), ST_BK_S_FREE)) return false;
-        ptx::tc_fence_after();
-        rows_product(q_tile(i), k_base, COL_S);
-        ptx::umma_commit(bar(&st->s_full));
-        return true;
-      };
-      auto issue_dp = [&](int i) {
-        if (!wait(&st->do_full[i % DS], (uint32_t)(i / DS), ST_BK_DO)) return false;
-        if (i > 0 && !wait(&st->dp_read, (uint32_t)(i - 1), ST_BK_DP_FREE)) return false;
-        ptx::tc_fence_after();
-        rows_product(do_tile(i), v_base, COL_DP);
-        ptx::umma_commit(bar(&st->dp_full));
-        return true;
-      };
-      bool ok = wait(&st->kv_full, 0, ST_BK_KV) && issue_s(0) && issue_dp(0);
+      bool ok = wait(&st->kv_full, 0, ST_BK_KV);
       for (int i = 0; ok && i < n; i++) {
-        if (i + 1 < n && !issue_s(i + 1)) break;
-        if (!wait(&st->p_ready, (uint32_t)i, ST_BK_P)) break;
+        if (!wait(&st->q_full[i % QS], (uint32_t)(i / QS), ST_BK_Q)) break;
+        if (i > 0 && !wait(&st->s_read, (uint32_t)(i - 1), ST_BK_S_FREE)) break;
         ptx::tc_fence_after();
-        reduce_rows(p_base, do_tile(i), COL_DV, i > 0);
-        ptx::umma_commit(bar(&st->dv_done));
+        product(ptx::smem_u32(sQ + (i % QS) * Sh::T_TILE), ptx::smem_u32(sK), COL_S);
+        ptx::umma_commit(bar(&st->s_full));
+        if (!wait(&st->do_full[i % DS], (uint32_t)(i / DS), ST_BK_DO)) break;
+        if (i > 0 && !wait(&st->dp_read, (uint32_t)(i - 1), ST_BK_DP_FREE)) break;
+        ptx::tc_fence_after();
+        product(ptx::smem_u32(sDO + (i % DS) * Sh::T_TILE), ptx::smem_u32(sV), COL_DP);
+        ptx::umma_commit(bar(&st->dp_full));
         ptx::umma_commit(bar(&st->do_empty[i % DS]));
-        if (!wait(&st->ds_ready, (uint32_t)i, ST_BK_DS)) break;
-        ptx::tc_fence_after();
-        reduce_rows(ds_base, q_tile(i), COL_DK, i > 0);
-        ptx::umma_commit(bar(&st->dk_done));
-        ptx::umma_commit(bar(&st->q_empty[i % QS]));
-        if (i + 1 < n && !issue_dp(i + 1)) break;
       }
     }
     __syncwarp();
-  } else if (warp >= 2) {
-    // ================= element-wise work: a thread per (query row, half of the keys); at the end per (key, half of the dims) ======
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+  } else if (n > 0 && warp < 4) {
+    // ================= dV += P^T dO (warp 2), dK += dS^T Q (warp 3) =================
+    if (lane == 0) {
+      const bool is_v = warp == 2;
+      const uint32_t idesc = ptx::make_idesc_bf16(TILE, HD, 1, 1);  // both operands with their rows as the reduction
+      const uint32_t a_base = ptx::smem_u32(is_v ? sP : sDS), b_base = ptx::smem_u32(is_v ? sDO : sQ), col = tmem_base + (is_v ? COL_DV : COL_DK);
+      const uint32_t slots = is_v ? DS : QS;
+      for (int i = 0; i < n; i++) {
+        const uint32_t slot = (uint32_t)i % slots;
+        if (!wait(is_v ? &st->p_ready : &st->ds_ready, (uint32_t)i, is_v ? ST_BK_P : ST_BK_DS)) break;
+        if (!wait(is_v ? &st->do_full[slot] : &st->q_full[slot], (uint32_t)i / slots, ST_BK_DO)) break;
+        ptx::tc_fence_after();
+        const uint64_t ad = tile_desc(a_base, SLAB), bd = tile_desc(b_base + slot * Sh::T_TILE, SLAB);
+#pragma unroll
+        for (int k16 = 0; k16 < TILE / 16; k16++)
+          ptx::umma_bf16(col, desc_at(ad, (uint32_t)(k16 * 2048)), desc_at(bd, (uint32_t)(k16 * 2048)), idesc, i > 0 || k16 > 0);
+        ptx::umma_commit(bar(is_v ? &st->dv_done : &st->dk_done));
+        ptx::umma_commit(bar(is_v ? &st->do_empty[slot] : &st->q_empty[slot]));
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ================= element-wise work: a thread per (query row, quarter of the keys); at the end per (key, quarter of the dims) ====
+    const int quarter = warp & 3, cols = (warp - 4) >> 2;
     const int trow = quarter * 32 + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t p_addr = ptx::smem_u32(sP + half * SLAB + trow * 128), ds_addr = ptx::smem_u32(sDS + half * SLAB + trow * 128);
+    const uint32_t slab_row = (uint32_t)((cols >> 1) * SLAB + trow * 128);
+    const uint32_t p_addr = ptx::smem_u32(sP) + slab_row, ds_addr = ptx::smem_u32(sDS) + slab_row;
     const float c = p.scale * LOG2E;
-    const int base = kb * TILE + half * 64;
     auto stats_of = [&](int i, float &lse2, float &delta) {
       const int row = (t0 + i % tiles) * TILE + trow;
       lse2 = delta = 0.0f;
@@ -1049,98 +1092,76 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
       delta = next_delta;
       if (i + 1 < n) stats_of(i + 1, next_lse2, next_delta);  // on their way while this step computes
       const int row0 = (t0 + i % tiles) * TILE, row = row0 + trow, pos = row + sp.shift, pos0 = row0 + sp.shift;
-      const bool whole = row0 + TILE <= sp.Tq && all_seen(kb * TILE, pos0, pos0 + TILE - 1, p.window, p.sinks);
-      const Seen seen{row < sp.Tq ? pos - base : -1, pos - p.window + 1 - base, p.sinks - base};
-      uint32_t x[64];
+      uint32_t see = 0xffffffffu;
+      if (row0 + TILE > sp.Tq || !all_seen(kb * TILE, pos0, pos0 + TILE - 1, p.window, p.sinks)) {
+        const int base = kb * TILE + cols * 32;
+        see = row < sp.Tq ? seen_bits(pos - base, pos - p.window + 1 - base, p.sinks - base) : 0u;
+      }
+      const bool masked = __any_sync(0xffffffffu, see != 0xffffffffu);
+      uint32_t x[32], d[32];
       if (!wait(&st->s_full, (uint32_t)i, ST_BK_S)) goto teardown;
       ptx::tc_fence_after();
-      ptx::tmem_ld32(lane_addr + COL_S + half * 64, x);
-      ptx::tmem_ld32(lane_addr + COL_S + half * 64 + 32, x + 32);
-      ptx::tmem_ld_wait();
+      load_columns<32>(lane_addr + COL_S + cols * 32, x);
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->s_read));
 #pragma unroll
-      for (int j = 0; j < 64; j++) x[j] = __float_as_uint(ex2(fmaf(__uint_as_float(x[j]), c, -lse2)));
-      if (!whole) {
+      for (int j = 0; j < 32; j++) x[j] = __float_as_uint(ex2(fmaf(__uint_as_float(x[j]), c, -lse2)));
+      if (masked) {
 #pragma unroll
-        for (int j = 0; j < 64; j++) x[j] = seen(j) ? x[j] : 0u;
+        for (int j = 0; j < 32; j++) x[j] = (see >> j) & 1u ? x[j] : 0u;
       }
       if (i > 0 && !wait(&st->dv_done, (uint32_t)(i - 1), ST_BK_DV)) goto teardown;  // has read P
-#pragma unroll
-      for (int q = 0; q < 8; q++) {
-        uint4 v;
-        v.x = pack_bf16(__uint_as_float(x[q * 8 + 0]), __uint_as_float(x[q * 8 + 1]));
-        v.y = pack_bf16(__uint_as_float(x[q * 8 + 2]), __uint_as_float(x[q * 8 + 3]));
-        v.z = pack_bf16(__uint_as_float(x[q * 8 + 4]), __uint_as_float(x[q * 8 + 5]));
-        v.w = pack_bf16(__uint_as_float(x[q * 8 + 6]), __uint_as_float(x[q * 8 + 7]));
-        sts128(p_addr + (uint32_t)((q ^ (trow & 7)) * 16), v);
-      }
+      store_chunks<4>(p_addr, trow, (cols & 1) * 4, x);
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->p_ready));
-      uint32_t d[64];
       if (!wait(&st->dp_full, (uint32_t)i, ST_BK_DP)) goto teardown;
       ptx::tc_fence_after();
-      ptx::tmem_ld32(lane_addr + COL_DP + half * 64, d);
-      ptx::tmem_ld32(lane_addr + COL_DP + half * 64 + 32, d + 32);
-      ptx::tmem_ld_wait();
+      load_columns<32>(lane_addr + COL_DP + cols * 32, d);
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->dp_read));
 #pragma unroll
-      for (int j = 0; j < 64; j++) d[j] = __float_as_uint(__uint_as_float(x[j]) * (__uint_as_float(d[j]) - delta));
-      if (!whole) {  // a masked product may be anything
+      for (int j = 0; j < 32; j++) d[j] = __float_as_uint(__uint_as_float(x[j]) * (__uint_as_float(d[j]) - delta));
+      if (masked) {  // a masked product may be anything
 #pragma unroll
-        for (int j = 0; j < 64; j++) d[j] = seen(j) ? d[j] : 0u;
+        for (int j = 0; j < 32; j++) d[j] = (see >> j) & 1u ? d[j] : 0u;
       }
       if (i > 0 && !wait(&st->dk_done, (uint32_t)(i - 1), ST_BK_DK)) goto teardown;  // has read dS
-#pragma unroll
-      for (int q = 0; q < 8; q++) {
-        uint4 v;
-        v.x = pack_bf16(__uint_as_float(d[q * 8 + 0]), __uint_as_float(d[q * 8 + 1]));
-        v.y = pack_bf16(__uint_as_float(d[q * 8 + 2]), __uint_as_float(d[q * 8 + 3]));
-        v.z = pack_bf16(__uint_as_float(d[q * 8 + 4]), __uint_as_float(d[q * 8 + 5]));
-        v.w = pack_bf16(__uint_as_float(d[q * 8 + 6]), __uint_as_float(d[q * 8 + 7]));
-        sts128(ds_addr + (uint32_t)((q ^ (trow & 7)) * 16), v);
-      }
+      store_chunks<4>(ds_addr, trow, (cols & 1) * 4, d);
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->ds_ready));
     }
     if (n > 0) {
-      if (!wait(&st->dk_done, (uint32_t)(n - 1), ST_BK_DK)) goto teardown;
+      if (!wait(&st->dk_done, (uint32_t)(n - 1), ST_BK_DK) || !wait(&st->dv_done, (uint32_t)(n - 1), ST_BK_DV)) goto teardown;
       ptx::tc_fence_after();
     }
     if (n > 0 || part == 0) {
       // the accumulators' lanes are keys
+      constexpr int DIMS = HD / 4;
       const int key = kb * TILE + trow;
       const bool to_share = share >= 0 && key < p.sinks;
-      float *sh = to_share ? p.shares + (((int64_t)share * p.kv_heads + kvh) * p.slot_rows + trow) * 2 * HD + half * (HD / 2) : nullptr;
-      const int64_t at = ((int64_t)(sp.k_off + key) * p.kv_heads + kvh) * HD + half * (HD / 2);
+      float *sh = to_share ? p.shares + (((int64_t)share * p.kv_heads + kvh) * p.slot_rows + trow) * 2 * HD + cols * DIMS : nullptr;
+      const int64_t at = ((int64_t)(sp.k_off + key) * p.kv_heads + kvh) * HD + cols * DIMS;
 #pragma unroll
       for (int which = 0; which < 2; which++) {
-        uint32_t r[HD / 2];
+        uint32_t r[DIMS];
         if (n > 0) {
-#pragma unroll
-          for (int q = 0; q < HD / 64; q++)
-            ptx::tmem_ld32(lane_addr + (which == 0 ? COL_DK : COL_DV) + half * (HD / 2) + q * 32, r + q * 32);
-          ptx::tmem_ld_wait();
+          load_columns<DIMS>(lane_addr + (which == 0 ? COL_DK : COL_DV) + cols * DIMS, r);
         } else {
 #pragma unroll
-          for (int j = 0; j < HD / 2; j++) r[j] = 0u;
+          for (int j = 0; j < DIMS; j++) r[j] = 0u;
         }
         const float f = which == 0 ? p.scale : 1.0f;
         if (key >= sp.Tk) continue;
+        if (to_share) {
 #pragma unroll
-        for (int q = 0; q < HD / 16; q++) {
-          float v[8];
+          for (int q = 0; q < DIMS / 4; q++)
+            reinterpret_cast<float4 *>(sh + which * HD)[q] = make_float4(__uint_as_float(r[4 * q]) * f, __uint_as_float(r[4 * q + 1]) * f,
+                                                                         __uint_as_float(r[4 * q + 2]) * f, __uint_as_float(r[4 * q + 3]) * f);
+        } else if (part == 0) {
 #pragma unroll
-          for (int j = 0; j < 8; j++) v[j] = __uint_as_float(r[q * 8 + j]) * f;
-          if (to_share) {
-            reinterpret_cast<float4 *>(sh + which * HD)[2 * q] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(sh + which * HD)[2 * q + 1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else if (part == 0) {
-            reinterpret_cast<uint4 *>((which == 0 ? p.dk : p.dv) + at)[q] = pack8(v);
-          }
+          for (int q = 0; q < DIMS / 16; q++) store16((which == 0 ? p.dk : p.dv) + at + q * 16, r + q * 16, f);
         }
       }
     }
@@ -1209,6 +1230,21 @@ int allow_smem(K kernel, size_t bytes, bool *done) {
   return 0;
 }
 
+// bf16 [rows][cols] as [cols / 64][rows][64]: one copy brings a tile of 128 rows of one head, slab by slab (128-byte swizzle, rows past
+// the end read as zeros)
+int tile_map(CUtensorMap *m, const void *base, int rows, uint64_t cols, int head_dim) {
+  EncodeTiledFn fn = encode_fn();
+  B200_REQUIRE(fn != nullptr, "attention_window: cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[3] = {64, (cuuint64_t)rows, cols / 64};
+  cuuint64_t strides[2] = {cols * 2, 128};
+  cuuint32_t box[3] = {64, window::TILE, (cuuint32_t)head_dim / 64};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  B200_REQUIRE(r == CUDA_SUCCESS, "attention_window: cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return 0;
+}
+
 template <int HD>
 int launch_fwd(window::FwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
@@ -1272,8 +1308,8 @@ int sm100_bwd(const Call &c) {
     }
     return 0;
   }
-  if (rows_map(&p.tmQ, c.q, (uint64_t)c.total_q, Dq) || rows_map(&p.tmdO, c.dout, (uint64_t)c.total_q, Dq) ||
-      rows_map(&p.tmK, c.k, (uint64_t)c.total_k, Dk) || rows_map(&p.tmV, c.v, (uint64_t)c.total_k, Dk))
+  if (tile_map(&p.tmQ, c.q, c.total_q, Dq, c.head_dim) || tile_map(&p.tmdO, c.dout, c.total_q, Dq, c.head_dim) ||
+      tile_map(&p.tmK, c.k, c.total_k, Dk, c.head_dim) || tile_map(&p.tmV, c.v, c.total_k, Dk, c.head_dim))
     return -1;
   p.o = c.o;
   p.dout = c.dout;
@@ -1326,8 +1362,8 @@ int sm100_fwd(const Call &c) {
   Device d;
   if (current_device(&d)) return -1;
   const uint64_t Dq = (uint64_t)c.q_heads * c.head_dim, Dk = (uint64_t)c.kv_heads * c.head_dim;
-  if (rows_map(&p.tmQ, c.q, (uint64_t)c.total_q, Dq) || rows_map(&p.tmK, c.k, (uint64_t)c.total_k, Dk) ||
-      rows_map(&p.tmV, c.v, (uint64_t)c.total_k, Dk))
+  if (tile_map(&p.tmQ, c.q, c.total_q, Dq, c.head_dim) || tile_map(&p.tmK, c.k, c.total_k, Dk, c.head_dim) ||
+      tile_map(&p.tmV, c.v, c.total_k, Dk, c.head_dim))
     return -1;
   p.O = c.out;
   p.lse = c.lse;
