@@ -144,12 +144,6 @@ __device__ __forceinline__ bool all_seen(int base, int pos0, int last, int windo
   return base + TILE - 1 <= pos0 && (base >= last - window + 1 || base + TILE <= sinks);
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // two fp32 operations in one instruction
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t d;
@@ -165,6 +159,40 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// x[j] = 2^(x[j] c + off)
+template <int N>
+__device__ __forceinline__ void probabilities(uint32_t *x, float c, float off) {
+  const uint64_t cc = pack2(c, c), oo = pack2(off, off);
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    float a, b;
+    unpack2(fma2(pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), cc, oo), a, b);
+    x[j] = __float_as_uint(ex2(a));
+    x[j + 1] = __float_as_uint(ex2(b));
+  }
+}
+// d[j] = p[j] (d[j] - delta)
+template <int N>
+__device__ __forceinline__ void score_gradients(uint32_t *d, const uint32_t *p, float delta) {
+  const uint64_t minus = pack2(-delta, -delta);
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    float a, b;
+    unpack2(mul2(pack2(__uint_as_float(p[j]), __uint_as_float(p[j + 1])), add2(pack2(__uint_as_float(d[j]), __uint_as_float(d[j + 1])), minus)), a, b);
+    d[j] = __float_as_uint(a);
+    d[j + 1] = __float_as_uint(b);
+  }
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -801,15 +829,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
         load_columns<32>(lane_addr + COL_S + cols * 32, s);
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->s_read));
-#pragma unroll
-        for (int j = 0; j < 32; j++) s[j] = __float_as_uint(ex2(fmaf(__uint_as_float(s[j]), c, -lse2)));
+        probabilities<32>(s, c, -lse2);
         if (!wait(&st->dp_full, t, ST_BQ_DP)) goto teardown;
         ptx::tc_fence_after();
         load_columns<32>(lane_addr + COL_DP + cols * 32, d);
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->dp_read));
-#pragma unroll
-        for (int j = 0; j < 32; j++) d[j] = __float_as_uint(__uint_as_float(s[j]) * (__uint_as_float(d[j]) - delta));
+        score_gradients<32>(d, s, delta);
         if (!all_seen(kb * TILE, pos0, last_pos, p.window, p.sinks)) {
           const int base = kb * TILE + cols * 32;
           const uint32_t see = seen_bits(min(pos, u.sp.Tk - 1) - base, pos - p.window + 1 - base, p.sinks - base);
@@ -1104,8 +1130,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
       load_columns<32>(lane_addr + COL_S + cols * 32, x);
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->s_read));
-#pragma unroll
-      for (int j = 0; j < 32; j++) x[j] = __float_as_uint(ex2(fmaf(__uint_as_float(x[j]), c, -lse2)));
+      probabilities<32>(x, c, -lse2);
       if (masked) {
 #pragma unroll
         for (int j = 0; j < 32; j++) x[j] = (see >> j) & 1u ? x[j] : 0u;
@@ -1120,8 +1145,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
       load_columns<32>(lane_addr + COL_DP + cols * 32, d);
       ptx::tc_fence_before();
       ptx::mbar_arrive(bar(&st->dp_read));
-#pragma unroll
-      for (int j = 0; j < 32; j++) d[j] = __float_as_uint(__uint_as_float(x[j]) * (__uint_as_float(d[j]) - delta));
+      score_gradients<32>(d, x, delta);
       if (masked) {  // a masked product may be anything
 #pragma unroll
         for (int j = 0; j < 32; j++) d[j] = (see >> j) & 1u ? d[j] : 0u;
