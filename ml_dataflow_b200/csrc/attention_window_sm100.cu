@@ -42,8 +42,12 @@ constexpr int SLAB = 16384;   // 128 rows x 64 bf16, one swizzled slab
 // of the three warpgroups' threads, the loading and issuing one hands 96 of them on (72 + 2 * 216 = 3 * 168).
 constexpr int FWD_THREADS = 384, REGS_CONTROL = 72, REGS_SOFTMAX = 216;
 static_assert(REGS_CONTROL + 2 * REGS_SOFTMAX <= 3 * 168, "a split of more registers than the launch has would wait for ever");
-// Backward: 4 warps that load and issue, 16 for the element-wise work.
-constexpr int BWD_THREADS = 640;
+// Backward, dK and dV: 4 warps that load and issue, 16 for the element-wise work.
+constexpr int BWD_KV_THREADS = 640;
+// Backward, dQ: 4 more that prepare a unit's row statistics and write the last one's output meanwhile. The launch gives 80 registers to
+// each of the six warpgroups' threads, the first two hand 16 each on (2 * 64 + 4 * 88 = 6 * 80).
+constexpr int BWD_Q_THREADS = 768, REGS_BWD_Q = 88, REGS_BWD_Q_OTHER = 64;
+static_assert(2 * REGS_BWD_Q_OTHER + 4 * REGS_BWD_Q <= 6 * 80, "a split of more registers than the launch has would wait for ever");
 constexpr float LOG2E = 1.4426950408889634f;
 
 enum { ST_Q_EMPTY = 51, ST_KV_EMPTY, ST_Q_FULL, ST_KV_FULL, ST_S_FREE, ST_P, ST_O_FREE, ST_S, ST_PV, ST_FIX };
@@ -564,7 +568,10 @@ teardown:
 // dQ: one query tile of one head per unit, persistent CTAs. Per key block
 //     S = Q K^T,  dP = dO V^T,   dS = P o (dP - delta) as bf16 through shared memory,   dQ += dS K
 // S and dP of a block are issued while the threads still work on the block before, and a unit's first products before the last
-// unit's dQ is finished. delta = rowsum(dO o O) is formed here, in fp32, and written for the other kernel.
+// unit's dQ is finished. delta = rowsum(dO o O) is formed here, in fp32, and written for the other kernel. Four warps of their own
+// form it for the next unit and write the last one's dQ (two accumulators in tensor memory): with these in the computing
+// threads' way a unit of ten blocks spent 10 of its 43 thousand cycles between the blocks. K is needed from S to dQ, V for dP only:
+// three slots of shared memory for K, one for V.
 //
 // dK, dV: one block of 128 keys of one key/value head per unit; it walks the query heads of the group and the query tiles that see
 // its keys, K and V stay in shared memory. Per tile
@@ -601,14 +608,15 @@ struct BwdParams {
 template <int HD>
 struct BwdQShape {
   static constexpr int Q_TILE = TILE * HD * 2, KV_TILE = TILE * HD * 2;
-  static constexpr int SLOTS = HD == 128 ? 4 : 8;
+  static constexpr int KS = HD == 128 ? 3 : 5, VS = HD == 128 ? 1 : 3;
   struct Tail {
-    uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full, s_read, dp_full, dp_read, ds_ready, dq_done, acc_empty, stat, fixed;
+    uint64_t q_full, q_empty, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full, s_read, dp_full, dp_read, ds_ready, dq_done, acc_full[2],
+        acc_empty[2], stat_full[2], stat_empty[2], fixed;
     uint32_t tmem_base;
     int abort_flag;
-    float delta[TILE];
+    float delta[2][TILE];  // of even and odd units
   };
-  static constexpr size_t smem = 1024 + 2 * (size_t)Q_TILE + DS_TILE + SLOTS * (size_t)KV_TILE + sizeof(Tail);
+  static constexpr size_t smem = 1024 + 2 * (size_t)Q_TILE + DS_TILE + (KS + VS) * (size_t)KV_TILE + sizeof(Tail);
   static_assert(smem <= 232448, "more shared memory than a CTA can be given");
 };
 
@@ -632,14 +640,14 @@ __device__ __forceinline__ QUnit q_unit_of(const BwdParams &p, int unit) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __grid_constant__ BwdParams p) {
+__global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __grid_constant__ BwdParams p) {
   using Sh = BwdQShape<HD>;
-  constexpr int SLOTS = Sh::SLOTS;
-  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256;
+  constexpr int KS = Sh::KS, VS = Sh::VS;
+  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256;  // dQ of even and odd units: 128 columns each
   extern __shared__ unsigned char window_smem[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(window_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  unsigned char *sQ = smem, *sDO = sQ + Sh::Q_TILE, *sDS = sDO + Sh::Q_TILE, *sKV = sDS + DS_TILE;
-  auto *st = reinterpret_cast<typename Sh::Tail *>(sKV + SLOTS * Sh::KV_TILE);
+  unsigned char *sQ = smem, *sDO = sQ + Sh::Q_TILE, *sDS = sDO + Sh::Q_TILE, *sK = sDS + DS_TILE, *sV = sK + KS * Sh::KV_TILE;
+  auto *st = reinterpret_cast<typename Sh::Tail *>(sV + VS * Sh::KV_TILE);
   volatile int *abort_flag = &st->abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](uint64_t *b) { return ptx::smem_u32(b); };
@@ -648,9 +656,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
   if (tid == 0) {
     ptx::mbar_init(bar(&st->q_full), 1);
     ptx::mbar_init(bar(&st->q_empty), 2);  // the last S and the last dP of a unit
-    for (int s = 0; s < SLOTS; s++) {
-      ptx::mbar_init(bar(&st->kv_full[s]), 1);
-      ptx::mbar_init(bar(&st->kv_empty[s]), 1);
+    for (int s = 0; s < KS; s++) {
+      ptx::mbar_init(bar(&st->k_full[s]), 1);
+      ptx::mbar_init(bar(&st->k_empty[s]), 1);
+    }
+    for (int s = 0; s < VS; s++) {
+      ptx::mbar_init(bar(&st->v_full[s]), 1);
+      ptx::mbar_init(bar(&st->v_empty[s]), 1);
     }
     ptx::mbar_init(bar(&st->s_full), 1);
     ptx::mbar_init(bar(&st->s_read), 512);
@@ -658,8 +670,12 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
     ptx::mbar_init(bar(&st->dp_read), 512);
     ptx::mbar_init(bar(&st->ds_ready), 512);
     ptx::mbar_init(bar(&st->dq_done), 1);
-    ptx::mbar_init(bar(&st->acc_empty), 512);
-    ptx::mbar_init(bar(&st->stat), 512);
+    for (int s = 0; s < 2; s++) {
+      ptx::mbar_init(bar(&st->acc_full[s]), 1);
+      ptx::mbar_init(bar(&st->acc_empty[s]), TILE);
+      ptx::mbar_init(bar(&st->stat_full[s]), TILE);
+      ptx::mbar_init(bar(&st->stat_empty[s]), 512);
+    }
     ptx::mbar_init(bar(&st->fixed), 1);
     st->abort_flag = 0;
     ptx::fence_barrier_init();
@@ -680,159 +696,202 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
   ptx::tc_fence_after();
   const uint32_t tmem_base = st->tmem_base;
 
-  if (warp == 0) {
-    // ================= loads: the whole warp walks, one lane issues =================
-    uint32_t n = 0, units = 0, fixes = 0;
-    bool ok = true;
-    auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
-    for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
-      const QUnit u = q_unit_of(p, unit);
-      const int kvh = u.x.h / p.group;
-      ok = waitw(&st->q_empty, units + 1, ST_BQ_Q);
-      units++;
-      if (ok && lane == 0) {
-        ptx::mbar_arrive_expect_tx(bar(&st->q_full), (uint32_t)(2 * Sh::Q_TILE));
-        ptx::tma_load_3d(ptx::smem_u32(sQ), &p.tmQ, bar(&st->q_full), 0, u.sp.q_off + u.x.row, u.x.h * (HD / 64));
-        ptx::tma_load_3d(ptx::smem_u32(sDO), &p.tmdO, bar(&st->q_full), 0, u.sp.q_off + u.x.row, u.x.h * (HD / 64));
-      }
-      for (int i = 0; ok && i < 2 * u.n; i++) {  // K_0, V_0, K_1, V_1, ...
-        const uint32_t slot = n % SLOTS;
-        const int kb = u.block(i >> 1);
-        ok = waitw(&st->kv_empty[slot], n / SLOTS + 1, ST_BQ_KV_EMPTY);
-        n++;
-        if (!ok) break;
-        // K multiplies dS: rows that no query sees have to be zero there. What they make of S and dP is dropped by a select.
-        const bool fix = (i & 1) == 0 && has_dead(u.sp, kb, p.window, p.sinks);
-        const uint32_t tile = ptx::smem_u32(sKV + slot * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(&st->kv_full[slot]);
-        if (lane == 0) {
-          ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::KV_TILE);
-          ptx::tma_load_3d(tile, (i & 1) ? &p.tmV : &p.tmK, full, 0, u.sp.k_off + kb * TILE, kvh * (HD / 64));
-        }
-        if (!fix) continue;
-        ok = waitw(&st->fixed, fixes++, ST_FIX);
-        if (!ok) break;
-        zero_dead<HD>(tile, u.sp, kb, p.window, p.sinks, lane);
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(&st->kv_full[slot]));
-      }
-    }
-    __syncwarp();
-  } else if (warp < 3) {
-    // ================= S = Q K^T (warp 1) and dP = dO V^T (warp 2) =================
-    if (lane == 0) {
-      const bool is_s = warp == 1;
-      const uint32_t idesc = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
-      const uint32_t a_base = ptx::smem_u32(is_s ? sQ : sDO), kv_base = ptx::smem_u32(sKV), col = tmem_base + (is_s ? COL_S : COL_DP);
-      uint64_t *full = is_s ? &st->s_full : &st->dp_full, *read = is_s ? &st->s_read : &st->dp_read;
-      uint32_t t = 0, units = 0;
+  if (warp < 4) {
+    ptx::reg_dec<REGS_BWD_Q_OTHER>();
+    if (warp == 0) {
+      // ================= loads: the whole warp walks, one lane issues =================
+      uint32_t t = 0, units = 0, fixes = 0;
       bool ok = true;
+      auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
       for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
-        const int steps = q_unit_of(p, unit).n;
-        ok = wait(&st->q_full, units++, ST_BQ_Q_FULL);
-        for (int i = 0; ok && i < steps; i++, t++) {
-          const uint32_t n = 2 * t + (is_s ? 0 : 1), slot = n % SLOTS;
-          if (!(ok = wait(&st->kv_full[slot], n / SLOTS, ST_BQ_KV_FULL))) break;
-          if (t > 0 && !(ok = wait(read, t - 1, ST_BQ_S_FREE))) break;
-          ptx::tc_fence_after();
-          const uint64_t ad = tile_desc(a_base, 0), bd = tile_desc(kv_base + slot * Sh::KV_TILE, 0);
-#pragma unroll
-          for (int k16 = 0; k16 < HD / 16; k16++) {
-            const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
-            ptx::umma_bf16(col, desc_at(ad, off), desc_at(bd, off), idesc, k16 > 0);
+        const QUnit u = q_unit_of(p, unit);
+        const int kvh = u.x.h / p.group;
+        ok = waitw(&st->q_empty, units + 1, ST_BQ_Q);
+        units++;
+        if (ok && lane == 0) {
+          ptx::mbar_arrive_expect_tx(bar(&st->q_full), (uint32_t)(2 * Sh::Q_TILE));
+          ptx::tma_load_3d(ptx::smem_u32(sQ), &p.tmQ, bar(&st->q_full), 0, u.sp.q_off + u.x.row, u.x.h * (HD / 64));
+          ptx::tma_load_3d(ptx::smem_u32(sDO), &p.tmdO, bar(&st->q_full), 0, u.sp.q_off + u.x.row, u.x.h * (HD / 64));
+        }
+        for (int i = 0; ok && i < u.n; i++, t++) {
+          const int kb = u.block(i);
+          const uint32_t ks = t % KS, vs = t % VS;
+          ok = waitw(&st->k_empty[ks], t / KS + 1, ST_BQ_KV_EMPTY);
+          if (!ok) break;
+          // K multiplies dS: rows that no query sees have to be zero there. What they make of S and dP is dropped by a select.
+          const bool fix = has_dead(u.sp, kb, p.window, p.sinks);
+          const uint32_t tile = ptx::smem_u32(sK + ks * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(&st->k_full[ks]);
+          if (lane == 0) {
+            ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::KV_TILE);
+            ptx::tma_load_3d(tile, &p.tmK, full, 0, u.sp.k_off + kb * TILE, kvh * (HD / 64));
           }
-          ptx::umma_commit(bar(full));
-          if (!is_s) ptx::umma_commit(bar(&st->kv_empty[slot]));  // K is read again by the dQ product
-          if (i == steps - 1) ptx::umma_commit(bar(&st->q_empty));
+          if (fix) {
+            ok = waitw(&st->fixed, fixes++, ST_FIX);
+            if (!ok) break;
+            zero_dead<HD>(tile, u.sp, kb, p.window, p.sinks, lane);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(&st->k_full[ks]));
+          }
+          ok = waitw(&st->v_empty[vs], t / VS + 1, ST_BQ_KV_EMPTY);
+          if (ok && lane == 0) {
+            ptx::mbar_arrive_expect_tx(bar(&st->v_full[vs]), (uint32_t)Sh::KV_TILE);
+            ptx::tma_load_3d(ptx::smem_u32(sV + vs * Sh::KV_TILE), &p.tmV, bar(&st->v_full[vs]), 0, u.sp.k_off + kb * TILE, kvh * (HD / 64));
+          }
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == 3) {
-    // ================= dQ += dS K =================
-    if (lane == 0) {
-      const uint32_t idesc = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // K is read with its head dimension contiguous
-      const uint32_t ds_base = ptx::smem_u32(sDS), kv_base = ptx::smem_u32(sKV);
-      uint32_t t = 0, units = 0;
-      bool ok = true;
-      for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round), units++) {
-        const int steps = q_unit_of(p, unit).n;
-        for (int i = 0; ok && i < steps; i++, t++) {
-          const uint32_t slot = (2 * t) % SLOTS;
-          // dS is in shared memory, which the threads formed from S: K has landed
-          if (!(ok = wait(&st->ds_ready, t, ST_BQ_DS))) break;
-          // the first of a unit overwrites the accumulator: the threads have read the unit before
-          if (i == 0 && units > 0 && !(ok = wait(&st->acc_empty, units - 1, ST_BQ_ACC))) break;
-          if (!(ok = wait(&st->kv_full[slot], 2 * t / SLOTS, ST_BQ_KV_FULL))) break;
-          ptx::tc_fence_after();
-          const uint64_t ad = tile_desc(ds_base, 0), bd = tile_desc(kv_base + slot * Sh::KV_TILE, SLAB);
+      __syncwarp();
+    } else if (warp < 3) {
+      // ================= S = Q K^T (warp 1) and dP = dO V^T (warp 2) =================
+      if (lane == 0) {
+        const bool is_s = warp == 1;
+        const uint32_t idesc = ptx::make_idesc_bf16(TILE, TILE, 0, 0);
+        const uint32_t a_base = ptx::smem_u32(is_s ? sQ : sDO), b_base = ptx::smem_u32(is_s ? sK : sV), col = tmem_base + (is_s ? COL_S : COL_DP);
+        uint64_t *full = is_s ? &st->s_full : &st->dp_full, *read = is_s ? &st->s_read : &st->dp_read;
+        const uint32_t slots = is_s ? KS : VS;
+        uint32_t t = 0, units = 0;
+        bool ok = true;
+        for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
+          const int steps = q_unit_of(p, unit).n;
+          ok = wait(&st->q_full, units++, ST_BQ_Q_FULL);
+          for (int i = 0; ok && i < steps; i++, t++) {
+            const uint32_t slot = t % slots;
+            if (!(ok = wait(is_s ? &st->k_full[slot] : &st->v_full[slot], t / slots, ST_BQ_KV_FULL))) break;
+            if (t > 0 && !(ok = wait(read, t - 1, ST_BQ_S_FREE))) break;
+            ptx::tc_fence_after();
+            const uint64_t ad = tile_desc(a_base, 0), bd = tile_desc(b_base + slot * Sh::KV_TILE, 0);
 #pragma unroll
-          for (int k16 = 0; k16 < TILE / 16; k16++)
-            ptx::umma_bf16(tmem_base + COL_DQ, desc_at(ad, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)), desc_at(bd, (uint32_t)(k16 * 2048)),
-                           idesc, i > 0 || k16 > 0);
-          ptx::umma_commit(bar(&st->dq_done));
-          ptx::umma_commit(bar(&st->kv_empty[slot]));
+            for (int k16 = 0; k16 < HD / 16; k16++) {
+              const uint32_t off = (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32);
+              ptx::umma_bf16(col, desc_at(ad, off), desc_at(bd, off), idesc, k16 > 0);
+            }
+            ptx::umma_commit(bar(full));
+            if (!is_s) ptx::umma_commit(bar(&st->v_empty[slot]));  // K is read again by the dQ product
+            if (i == steps - 1) ptx::umma_commit(bar(&st->q_empty));
+          }
         }
       }
+      __syncwarp();
+    } else {
+      // ================= dQ += dS K =================
+      if (lane == 0) {
+        const uint32_t idesc = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // K is read with its head dimension contiguous
+        const uint32_t ds_base = ptx::smem_u32(sDS), k_base = ptx::smem_u32(sK);
+        uint32_t t = 0, units = 0;
+        bool ok = true;
+        for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round), units++) {
+          const int steps = q_unit_of(p, unit).n;
+          const uint32_t acc = units & 1;
+          // the unit before the last one has been read out of this accumulator
+          if (units > 1) ok = wait(&st->acc_empty[acc], units / 2 - 1, ST_BQ_ACC);
+          for (int i = 0; ok && i < steps; i++, t++) {
+            const uint32_t slot = t % KS;
+            if (!(ok = wait(&st->ds_ready, t, ST_BQ_DS))) break;
+            if (!(ok = wait(&st->k_full[slot], t / KS, ST_BQ_KV_FULL))) break;
+            ptx::tc_fence_after();
+            const uint64_t ad = tile_desc(ds_base, 0), bd = tile_desc(k_base + slot * Sh::KV_TILE, SLAB);
+#pragma unroll
+            for (int k16 = 0; k16 < TILE / 16; k16++)
+              ptx::umma_bf16(tmem_base + COL_DQ + acc * TILE, desc_at(ad, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)),
+                             desc_at(bd, (uint32_t)(k16 * 2048)), idesc, i > 0 || k16 > 0);
+            ptx::umma_commit(bar(&st->dq_done));
+            ptx::umma_commit(bar(&st->k_empty[slot]));
+            if (i == steps - 1) ptx::umma_commit(bar(&st->acc_full[acc]));
+          }
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  } else {
-    // ================= element-wise work: a thread per (query row, quarter of the columns) =================
-    const int quarter = warp & 3, cols = (warp - 4) >> 2;  // columns 32 * cols ...
-    const int trow = quarter * 32 + lane;
+  } else if (warp < 8) {
+    ptx::reg_dec<REGS_BWD_Q_OTHER>();
+    // ================= row statistics of the next unit, output of the last one =================
+    const int quarter = warp & 3, trow = quarter * 32 + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    auto statistics = [&](int unit, uint32_t units) {
+      const QUnit u = q_unit_of(p, unit);
+      const uint32_t set = units & 1;
+      if (units > 1 && !wait(&st->stat_empty[set], units / 2 - 1, ST_BQ_STAT)) return false;
+      const int64_t row0 = u.sp.q_off + u.x.row;
+      const int rows = u.sp.Tq - u.x.row;
+      // delta = dO . O: HD / 8 lanes a row, this warp's 32 rows
+      constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES;
+#pragma unroll 4
+      for (int q = 0; q < 32; q += AT_ONCE) {
+        const int r = quarter * 32 + q + lane / LANES;
+        float d = 0.0f;
+        if (r < rows) {
+          const int64_t at = ((row0 + r) * p.q_heads + u.x.h) * LANES + lane % LANES;
+          float x[8], y[8];
+          unpack8(reinterpret_cast<const uint4 *>(p.dout)[at], x);
+          unpack8(reinterpret_cast<const uint4 *>(p.o)[at], y);
+#pragma unroll
+          for (int j = 0; j < 8; j++) d = fmaf(x[j], y[j], d);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (lane % LANES == 0) {
+          st->delta[set][r] = d;
+          if (r < rows) p.delta[(int64_t)u.x.h * p.total_q + row0 + r] = d;
+        }
+      }
+      ptx::mbar_arrive(bar(&st->stat_full[set]));
+      return true;
+    };
+    uint32_t units = 0;
+    int unit = unit_at(0);
+    if (unit < p.units && !statistics(unit, 0)) goto teardown;
+    for (int round = 0; unit < p.units; units++) {
+      const int next = unit_at(++round);
+      if (next < p.units && !statistics(next, units + 1)) goto teardown;
+      const QUnit u = q_unit_of(p, unit);
+      const int row = u.x.row + trow;
+      __nv_bfloat16 *o = p.dq + ((int64_t)(u.sp.q_off + row) * p.q_heads + u.x.h) * HD;
+      if (!wait(&st->acc_full[units & 1], units / 2, ST_BQ_DQ)) goto teardown;
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < HD / 32; q++) {
+        uint32_t r[32];
+        load_columns<32>(lane_addr + COL_DQ + (units & 1) * TILE + q * 32, r);
+        if (q == HD / 32 - 1) {
+          ptx::tc_fence_before();
+          ptx::mbar_arrive(bar(&st->acc_empty[units & 1]));
+        }
+        if (row < u.sp.Tq) {
+          store16(o + q * 32, r, p.scale);
+          store16(o + q * 32 + 16, r + 16, p.scale);
+        }
+      }
+      unit = next;
+    }
+  } else {
+    ptx::reg_inc<REGS_BWD_Q>();
+    // ================= element-wise work: a thread per (query row, quarter of the columns) =================
+    const int quarter = warp & 3, cols = (warp - 8) >> 2;  // columns 32 * cols ...
+    const int trow = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + cols * 32;
     const uint32_t ds_addr = ptx::smem_u32(sDS + (cols >> 1) * SLAB + trow * 128);
     const float c = p.scale * LOG2E;
     uint32_t t = 0, units = 0;
-    for (int round = 0, unit = unit_at(0); unit < p.units; unit = unit_at(++round)) {
+    for (int round = 0, unit = unit_at(0); unit < p.units; unit = unit_at(++round), units++) {
       const QUnit u = q_unit_of(p, unit);
       const int row = u.x.row + trow, pos = row + u.sp.shift;
-      const bool valid = row < u.sp.Tq;
-      const int64_t stat = (int64_t)u.x.h * p.total_q + u.sp.q_off + row;
-      const float lse2 = valid ? p.lse[stat] * LOG2E : 0.0f;
-      {
-        // delta = dO . O: this warp takes eight rows of the tile, HD / 8 lanes a row
-        constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES;
-        const int first = (warp - 4) * 8 + lane / LANES;
-        float d[8 / AT_ONCE];
-#pragma unroll
-        for (int q = 0; q < 8 / AT_ONCE; q++) {
-          const int r = u.x.row + first + q * AT_ONCE;
-          d[q] = 0.0f;
-          if (r < u.sp.Tq) {
-            const int64_t at = ((int64_t)(u.sp.q_off + r) * p.q_heads + u.x.h) * LANES + lane % LANES;
-            float x[8], y[8];
-            unpack8(reinterpret_cast<const uint4 *>(p.dout)[at], x);
-            unpack8(reinterpret_cast<const uint4 *>(p.o)[at], y);
-#pragma unroll
-            for (int j = 0; j < 8; j++) d[q] = fmaf(x[j], y[j], d[q]);
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 8 / AT_ONCE; q++) {
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) d[q] += __shfl_xor_sync(0xffffffffu, d[q], o);
-          if (lane % LANES == 0) st->delta[first + q * AT_ONCE] = d[q];
-        }
-      }
-      ptx::mbar_arrive(bar(&st->stat));
-      if (!wait(&st->stat, units, ST_BQ_STAT)) goto teardown;
-      units++;
-      const float delta = st->delta[trow];
-      if (valid && cols == 0) p.delta[stat] = delta;
       const int pos0 = u.x.row + u.sp.shift, last_pos = min(pos0 + TILE, u.sp.Tk) - 1;
-      for (int i = 0; i < u.n; i++) {
+      const float lse2 = row < u.sp.Tq ? p.lse[(int64_t)u.x.h * p.total_q + u.sp.q_off + row] * LOG2E : 0.0f;
+      if (!wait(&st->stat_full[units & 1], units / 2, ST_BQ_STAT)) goto teardown;
+      const float delta = st->delta[units & 1][trow];
+      ptx::mbar_arrive(bar(&st->stat_empty[units & 1]));
+      for (int i = 0; i < u.n; i++, t++) {
         const int kb = u.block(i);
         uint32_t s[32], d[32];
         if (!wait(&st->s_full, t, ST_BQ_S)) goto teardown;
         ptx::tc_fence_after();
-        load_columns<32>(lane_addr + COL_S + cols * 32, s);
+        load_columns<32>(lane_addr + COL_S, s);
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->s_read));
         probabilities<32>(s, c, -lse2);
         if (!wait(&st->dp_full, t, ST_BQ_DP)) goto teardown;
         ptx::tc_fence_after();
-        load_columns<32>(lane_addr + COL_DP + cols * 32, d);
+        load_columns<32>(lane_addr + COL_DP, d);
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->dp_read));
         score_gradients<32>(d, s, delta);
@@ -848,18 +907,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_q_kernel(const __gr
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         ptx::mbar_arrive(bar(&st->ds_ready));
-        t++;
-      }
-      if (!wait(&st->dq_done, t - 1, ST_BQ_DQ)) goto teardown;
-      ptx::tc_fence_after();
-      uint32_t r[HD / 4];
-      load_columns<HD / 4>(lane_addr + COL_DQ + cols * (HD / 4), r);
-      ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(&st->acc_empty));
-      if (valid) {
-        __nv_bfloat16 *o = p.dq + ((int64_t)(u.sp.q_off + row) * p.q_heads + u.x.h) * HD + cols * (HD / 4);
-#pragma unroll
-        for (int q = 0; q < HD / 64; q++) store16(o + q * 16, r + q * 16, p.scale);
       }
     }
   }
@@ -925,7 +972,7 @@ struct BwdKShape {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __grid_constant__ BwdParams p) {
+__global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const __grid_constant__ BwdParams p) {
   using Sh = BwdKShape<HD>;
   constexpr int KSL = HD / 64, QS = Sh::Q_SLOTS, DS = Sh::DO_SLOTS;
   constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DK = 256, COL_DV = 384;
@@ -1016,8 +1063,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
       ptx::tma_load_3d(ptx::smem_u32(sK), &p.tmK, bar(&st->kv_full), 0, sp.k_off + kb * TILE, kvh * KSL);
       ptx::tma_load_3d(ptx::smem_u32(sV), &p.tmV, bar(&st->kv_full), 0, sp.k_off + kb * TILE, kvh * KSL);
     }
-    for (int i = 0; ok && i < n; i++) {
-      const int h = kvh * p.group + i / tiles, row = (t0 + i % tiles) * TILE;
+    for (int i = 0, tile_at = t0, h = kvh * p.group; ok && i < n; i++) {
+      const int row = tile_at * TILE;
       const bool fix = row + TILE > sp.Tq;  // rows past the sequence's end are zeroed: dO and Q multiply P and dS
 #pragma unroll
       for (int which = 0; which < 2; which++) {
@@ -1042,6 +1089,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(full_b));
+      }
+      if (++tile_at == t1) {
+        tile_at = t0;
+        h++;
       }
     }
     __syncwarp();
@@ -1102,22 +1153,28 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) window_bwd_kv_kernel(const __g
     const uint32_t slab_row = (uint32_t)((cols >> 1) * SLAB + trow * 128);
     const uint32_t p_addr = ptx::smem_u32(sP) + slab_row, ds_addr = ptx::smem_u32(sDS) + slab_row;
     const float c = p.scale * LOG2E;
-    auto stats_of = [&](int i, float &lse2, float &delta) {
-      const int row = (t0 + i % tiles) * TILE + trow;
-      lse2 = delta = 0.0f;
-      if (i < n && row < sp.Tq) {
-        const int64_t at = (int64_t)(kvh * p.group + i / tiles) * p.total_q + sp.q_off + row;
-        lse2 = p.lse[at] * LOG2E;
-        delta = p.delta[at];
+    // a step's statistics are fetched while the step before computes: `ahead` is its tile, stat_at its row in the arrays
+    int ahead = t0;
+    int64_t stat_at = (int64_t)(kvh * p.group) * p.total_q + sp.q_off + t0 * TILE + trow;
+    float lse2 = 0.0f, delta = 0.0f, next_lse = 0.0f, next_delta = 0.0f;
+    auto fetch = [&]() {
+      if (ahead * TILE + trow < sp.Tq) {
+        next_lse = p.lse[stat_at];
+        next_delta = p.delta[stat_at];
+      }
+      stat_at += TILE;
+      if (++ahead == t1) {
+        ahead = t0;
+        stat_at += p.total_q - tiles * TILE;
       }
     };
-    float lse2 = 0.0f, delta = 0.0f, next_lse2 = 0.0f, next_delta = 0.0f;
-    if (n > 0) stats_of(0, next_lse2, next_delta);
-    for (int i = 0; i < n; i++) {
-      lse2 = next_lse2;
+    if (n > 0) fetch();
+    for (int i = 0, tile_at = t0; i < n; i++) {
+      lse2 = next_lse * LOG2E;
       delta = next_delta;
-      if (i + 1 < n) stats_of(i + 1, next_lse2, next_delta);  // on their way while this step computes
-      const int row0 = (t0 + i % tiles) * TILE, row = row0 + trow, pos = row + sp.shift, pos0 = row0 + sp.shift;
+      if (i + 1 < n) fetch();
+      const int row0 = tile_at * TILE, row = row0 + trow, pos = row + sp.shift, pos0 = row0 + sp.shift;
+      if (++tile_at == t1) tile_at = t0;
       uint32_t see = 0xffffffffu;
       if (row0 + TILE > sp.Tq || !all_seen(kb * TILE, pos0, pos0 + TILE - 1, p.window, p.sinks)) {
         const int base = kb * TILE + cols * 32;
@@ -1284,7 +1341,7 @@ int launch_bwd_q(const window::BwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
   constexpr size_t smem = window::BwdQShape<HD>::smem;
   if (allow_smem(window::window_bwd_q_kernel<HD>, smem, &done[d.dev])) return -1;
-  window::window_bwd_q_kernel<HD><<<p.units < d.sms ? p.units : d.sms, window::BWD_THREADS, smem, s>>>(p);
+  window::window_bwd_q_kernel<HD><<<p.units < d.sms ? p.units : d.sms, window::BWD_Q_THREADS, smem, s>>>(p);
   B200_CHECK_LAUNCH("attention_window_bwd (dQ)");
   return 0;
 }
@@ -1294,7 +1351,7 @@ int launch_bwd_kv(const window::BwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
   constexpr size_t smem = window::BwdKShape<HD>::smem;
   if (allow_smem(window::window_bwd_kv_kernel<HD>, smem, &done[d.dev])) return -1;
-  window::window_bwd_kv_kernel<HD><<<p.units, window::BWD_THREADS, smem, s>>>(p);
+  window::window_bwd_kv_kernel<HD><<<p.units, window::BWD_KV_THREADS, smem, s>>>(p);
   B200_CHECK_LAUNCH("attention_window_bwd (dK, dV)");
   return 0;
 }
