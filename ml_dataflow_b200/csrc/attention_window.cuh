@@ -53,6 +53,9 @@ int next_sequences(SeqTable &t, int *next, const Call &c, F units_of) {
 // attention_window_sm100.cu: tensor-core kernels for head sizes 64 and 128
 bool sm100_supported(int head_dim);
 int sm100_fwd(const Call &c);
+// attention_window_few.cu: its forward for sequences with few queries
+bool is_few(const Call &c, int s);
+int few_fwd(const Call &c);
 uint64_t sm100_bwd_workspace(int num_seqs, int q_heads, int kv_heads, int head_dim, int total_q, int sinks);
 int sm100_bwd(const Call &c);
 

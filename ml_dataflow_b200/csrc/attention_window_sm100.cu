@@ -1448,6 +1448,10 @@ int sm100_bwd(const Call &c) {
 }
 
 int sm100_fwd(const Call &c) {
+  if (few_fwd(c)) return -1;
+  bool tiles = false;
+  for (int s = 0; s < c.num_seqs && !tiles; s++) tiles = c.q_len[s] > 0 && !is_few(c, s);
+  if (!tiles) return 0;
   FwdParams p;
   Device d;
   if (current_device(&d)) return -1;
@@ -1468,7 +1472,7 @@ int sm100_fwd(const Call &c) {
   B200_REQUIRE(p.status != nullptr, "attention_window: the status word of this device is not reachable");
   for (int next = 0; next < c.num_seqs;) {
     p.units = next_sequences(p.seqs, &next, c, [&](int s) {
-      const int tiles = (c.q_len[s] + TILE - 1) / TILE;
+      const int tiles = is_few(c, s) ? 0 : (c.q_len[s] + TILE - 1) / TILE;
       return p.pair_heads ? tiles * (c.q_heads / 2) : (tiles + 1) / 2 * c.q_heads;
     });
     if (p.units == 0) continue;
