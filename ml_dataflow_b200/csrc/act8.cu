@@ -11,9 +11,11 @@
 // e is at least -124, so that the smallest step, 2^(e - 9), is still a bf16 number. An infinity or a NaN is held as NaN
 // and takes no part in the maximum: the other values of its block keep their precision.
 //
-// All three kernels touch every byte once and are bound by memory: a thread takes eight columns (16 bytes of bf16, 8 of
-// codes), four neighbouring lanes share a scale block, and the maximum costs two shuffles. Two groups of eight per thread
-// are in flight.
+// All three kernels touch every byte once. A thread takes eight columns (16 bytes of bf16, 8 of codes), four neighbouring lanes
+// share a scale block, and the maximum costs two shuffles; two groups of eight per thread are in flight. What bounds them besides
+// memory is the number of instructions: hence arithmetic on pairs, the special-function units' reciprocal in the sigmoid (2^-22
+// relative, far below the outputs' 2^-9), special values looked for once per group, and no index divisions where the columns are whole
+// scale blocks.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -36,16 +38,32 @@ struct Shape {
   int64_t padded;  // rows * padded groups per row
   int vecs, padded_vecs, blocks;
 };
-__device__ __forceinline__ Place place(const Shape &s, int64_t base_row, int base_col, int at, int64_t unit) {
-  // at: groups past (base_row, base_col); 32-bit division
-  const int c = base_col + at;
-  const int rows = c / s.padded_vecs, col = c - rows * s.padded_vecs;
-  Place p;
-  p.vec = (base_row + rows) * s.vecs + col;
-  p.block = (base_row + rows) * s.blocks + (col >> 2);
-  p.on = unit < s.padded && col < s.vecs;
-  return p;
-}
+// The groups of one thread, `at` past the block's first group `base`. WHOLE: the columns are whole scale blocks, nothing is padded.
+template <bool WHOLE>
+struct Places {
+  int64_t base, row;
+  int col;
+  __device__ __forceinline__ Places(const Shape &s, int64_t first) : base(first) {
+    if (!WHOLE) {
+      row = first / s.padded_vecs;
+      col = (int)(first - row * s.padded_vecs);
+    }
+  }
+  __device__ __forceinline__ Place operator()(const Shape &s, int at) const {
+    Place p;
+    if (WHOLE) {
+      p.vec = base + at;
+      p.block = p.vec >> 2;
+      p.on = p.vec < s.padded;
+    } else {
+      const int c = col + at, rows = c / s.padded_vecs, cc = c - rows * s.padded_vecs;
+      p.vec = (row + rows) * s.vecs + cc;
+      p.block = (row + rows) * s.blocks + (cc >> 2);
+      p.on = base + at < s.padded && cc < s.vecs;
+    }
+    return p;
+  }
+};
 
 // exponent of the block's unit, biased by 127, from the bf16 bits of its largest finite magnitude
 __device__ __forceinline__ int unit_of(uint32_t top) {
@@ -53,12 +71,13 @@ __device__ __forceinline__ int unit_of(uint32_t top) {
   return max(e, -124) + 127;
 }
 
-// largest finite magnitude of eight bf16 numbers, as bf16 bits
-__device__ __forceinline__ uint32_t top_of(const uint4 &v) {
-  uint32_t a[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
-  uint32_t m = __vmaxu2(__vmaxu2(a[0], a[1]), __vmaxu2(a[2], a[3]));
+// largest finite magnitude of eight bf16 numbers, as bf16 bits; `odd`: an infinity or NaN is among them
+__device__ __forceinline__ uint32_t top_of(const uint4 &v, bool &odd) {
+  const uint32_t a[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
+  const uint32_t m = __vmaxu2(__vmaxu2(a[0], a[1]), __vmaxu2(a[2], a[3]));
   uint32_t t = max(m & 0xffffu, m >> 16);
-  if (t >= 0x7f80u) {  // an infinity or NaN: take the others
+  odd = t >= 0x7f80u;
+  if (odd) {  // take the others
     t = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -69,169 +88,196 @@ __device__ __forceinline__ uint32_t top_of(const uint4 &v) {
   return t;
 }
 
-__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+__device__ __forceinline__ uint32_t codes2(uint64_t v) {
+  float lo, hi;
+  unpack2(v, lo, hi);
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float no_infinity(float x) { return fabsf(x) == INFINITY ? __int_as_float(0x7fffffff) : x; }
 
-// the codes of one group; every lane of the warp takes part
-__device__ __forceinline__ uint2 encode(const uint4 &v, const float *x, int &biased) {
-  uint32_t top = top_of(v);
+// the codes of one group from its pairs x; every lane of the warp takes part
+__device__ __forceinline__ uint2 encode(const uint4 &v, const uint64_t *x, int &biased) {
+  bool odd;
+  uint32_t top = top_of(v, odd);
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   biased = unit_of(top);
   const float inv = __int_as_float((254 - biased) << 23);  // 2^-e
-  float y[8];
+  const uint64_t ii = pack2(inv, inv);
+  uint64_t y[4];
 #pragma unroll
-  for (int i = 0; i < 8; i++) y[i] = no_infinity(x[i] * inv);
-  if (biased == 120 + 127) {
+  for (int i = 0; i < 4; i++) y[i] = mul2(x[i], ii);
+  if (odd || biased == 120 + 127) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = fabsf(y[i]) > 240.0f ? copysignf(240.0f, y[i]) : y[i];  // NaN stays
+    for (int i = 0; i < 4; i++) {
+      float z[2];
+      unpack2(y[i], z[0], z[1]);
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        if (fabsf(z[e]) == INFINITY) z[e] = __int_as_float(0x7fffffff);
+        else if (biased == 120 + 127 && fabsf(z[e]) > 240.0f) z[e] = copysignf(240.0f, z[e]);  // NaN stays
+      }
+      y[i] = pack2(z[0], z[1]);
+    }
   }
-  uint32_t c[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) c[i] = codes2(y[2 * i], y[2 * i + 1]);
-  return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+  return make_uint2(codes2(y[0]) | (codes2(y[1]) << 16), codes2(y[2]) | (codes2(y[3]) << 16));
 }
 
-__device__ __forceinline__ void decode(const uint2 &codes, int biased, float *x) {
+__device__ __forceinline__ void decode(const uint2 &codes, int biased, uint64_t *x) {
   const float unit = __int_as_float(biased << 23);
+  const uint64_t uu = pack2(unit, unit);
   const uint32_t w[2] = {codes.x, codes.y};
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w[i >> 1] >> ((i & 1) * 16))));
     const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&h));
-    x[2 * i] = f.x * unit;
-    x[2 * i + 1] = f.y * unit;
+    x[i] = mul2(pack2(f.x, f.y), uu);
   }
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+// of a pair: 1 / (1 + exp(-x))
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t x) {
+  const float minus_log2e = -1.4426950408889634f;
+  float a, b;
+  unpack2(mul2(x, pack2(minus_log2e, minus_log2e)), a, b);
+  asm("ex2.approx.f32 %0, %0;" : "+f"(a));
+  asm("ex2.approx.f32 %0, %0;" : "+f"(b));
+  unpack2(add2(pack2(a, b), pack2(1.0f, 1.0f)), a, b);
+  asm("rcp.approx.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.f32 %0, %0;" : "+f"(b));
+  return pack2(a, b);
+}
+__device__ __forceinline__ void widen(const uint4 &v, uint64_t *x) {
+  x[0] = widen2(v.x);
+  x[1] = widen2(v.y);
+  x[2] = widen2(v.z);
+  x[3] = widen2(v.w);
+}
+__device__ __forceinline__ uint4 round_all(const uint64_t *x) { return make_uint4(round2(x[0]), round2(x[1]), round2(x[2]), round2(x[3])); }
+__device__ __forceinline__ void swiglu(const uint64_t *x, const uint64_t *y, uint64_t *h) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) h[i] = mul2(mul2(x[i], sigmoid2(x[i])), y[i]);
+}
 
 // h = silu(x1) * x3 (when asked for) and the codes of x1 and x3
+template <bool WHOLE>
 __global__ void __launch_bounds__(THREADS) keep_kernel(Shape s, const uint4 *x1, const uint4 *x3, uint4 *out, uint2 *c1, uint8_t *e1,
                                                        uint2 *c3, uint8_t *e3) {
   const int64_t step = (int64_t)gridDim.x * THREADS * UNROLL;
   for (int64_t base = (int64_t)blockIdx.x * THREADS * UNROLL; base < s.padded; base += step) {
-    const int64_t row = base / s.padded_vecs;
-    const int col = (int)(base - row * s.padded_vecs);
-    Place p[UNROLL];
+    const Places<WHOLE> places(s, base);
     uint4 a[UNROLL], b[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      const int at = u * THREADS + threadIdx.x;
-      p[u] = place(s, row, col, at, base + at);
+      const Place p = places(s, u * THREADS + threadIdx.x);
       a[u] = b[u] = make_uint4(0, 0, 0, 0);
-      if (p[u].on) {
-        a[u] = ld_stream(x1 + p[u].vec);
-        b[u] = ld_stream(x3 + p[u].vec);
+      if (p.on) {
+        a[u] = ld_stream(x1 + p.vec);
+        b[u] = ld_stream(x3 + p.vec);
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      float x[8], y[8];
+      const Place p = places(s, u * THREADS + threadIdx.x);
+      uint64_t x[4], y[4];
       int ex, ey;
-      unpack8(a[u], x);
-      unpack8(b[u], y);
+      widen(a[u], x);
+      widen(b[u], y);
       const uint2 cx = encode(a[u], x, ex), cy = encode(b[u], y, ey);
-      if (!p[u].on) continue;
-      c1[p[u].vec] = cx;
-      c3[p[u].vec] = cy;
+      if (!p.on) continue;
+      c1[p.vec] = cx;
+      c3[p.vec] = cy;
       if ((threadIdx.x & 3) == 0) {
-        e1[p[u].block] = (uint8_t)ex;
-        e3[p[u].block] = (uint8_t)ey;
+        e1[p.block] = (uint8_t)ex;
+        e3[p.block] = (uint8_t)ey;
       }
       if (out != nullptr) {
-#pragma unroll
-        for (int q = 0; q < 8; q++) x[q] = x[q] * sigmoid(x[q]) * y[q];
-        st_stream(out + p[u].vec, pack8(x));
+        swiglu(x, y, x);
+        st_stream(out + p.vec, round_all(x));
       }
     }
   }
 }
 
 // the held x1 and x3 as bf16, and h again from them: each output when its pointer is not null
+template <bool WHOLE>
 __global__ void __launch_bounds__(THREADS) restore_kernel(Shape s, const uint2 *c1, const uint8_t *e1, const uint2 *c3, const uint8_t *e3,
                                                           uint4 *x1, uint4 *x3, uint4 *out) {
   const int64_t step = (int64_t)gridDim.x * THREADS * UNROLL;
   for (int64_t base = (int64_t)blockIdx.x * THREADS * UNROLL; base < s.padded; base += step) {
-    const int64_t row = base / s.padded_vecs;
-    const int col = (int)(base - row * s.padded_vecs);
-    Place p[UNROLL];
+    const Places<WHOLE> places(s, base);
     uint2 a[UNROLL], b[UNROLL];
     int ea[UNROLL], eb[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      const int at = u * THREADS + threadIdx.x;
-      p[u] = place(s, row, col, at, base + at);
-      if (p[u].on) {
-        a[u] = c1[p[u].vec];
-        b[u] = c3[p[u].vec];
-        ea[u] = e1[p[u].block];
-        eb[u] = e3[p[u].block];
+      const Place p = places(s, u * THREADS + threadIdx.x);
+      if (p.on) {
+        a[u] = c1[p.vec];
+        b[u] = c3[p.vec];
+        ea[u] = e1[p.block];
+        eb[u] = e3[p.block];
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      if (!p[u].on) continue;
-      float x[8], y[8];
+      const Place p = places(s, u * THREADS + threadIdx.x);
+      if (!p.on) continue;
+      uint64_t x[4], y[4];
       decode(a[u], ea[u], x);
       decode(b[u], eb[u], y);
-      if (x1 != nullptr) st_stream(x1 + p[u].vec, pack8(x));
-      if (x3 != nullptr) st_stream(x3 + p[u].vec, pack8(y));
+      if (x1 != nullptr) st_stream(x1 + p.vec, round_all(x));
+      if (x3 != nullptr) st_stream(x3 + p.vec, round_all(y));
       if (out != nullptr) {
-#pragma unroll
-        for (int q = 0; q < 8; q++) x[q] = x[q] * sigmoid(x[q]) * y[q];
-        st_stream(out + p[u].vec, pack8(x));
+        swiglu(x, y, x);
+        st_stream(out + p.vec, round_all(x));
       }
     }
   }
 }
 
 // the SwiGLU's backward on the held values: with g = sigmoid(x1)
-//   dx1 = dh x3 g (1 + x1 (1 - g)),   dx3 = dh x1 g,   h = x1 g x3 (when asked for; the W2 weight gradient reads it)
+//   dx1 = dh x3 (g + x1 g (1 - g)),   dx3 = dh x1 g,   h = x1 g x3 (when asked for; the W2 weight gradient reads it)
+template <bool WHOLE>
 __global__ void __launch_bounds__(THREADS) backward_kernel(Shape s, const uint2 *c1, const uint8_t *e1, const uint2 *c3, const uint8_t *e3,
                                                            const uint4 *dh, uint4 *dx1, uint4 *dx3, uint4 *out) {
   const int64_t step = (int64_t)gridDim.x * THREADS * UNROLL;
   for (int64_t base = (int64_t)blockIdx.x * THREADS * UNROLL; base < s.padded; base += step) {
-    const int64_t row = base / s.padded_vecs;
-    const int col = (int)(base - row * s.padded_vecs);
-    Place p[UNROLL];
+    const Places<WHOLE> places(s, base);
     uint2 a[UNROLL], b[UNROLL];
     uint4 d[UNROLL];
     int ea[UNROLL], eb[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      const int at = u * THREADS + threadIdx.x;
-      p[u] = place(s, row, col, at, base + at);
-      if (p[u].on) {
-        a[u] = c1[p[u].vec];
-        b[u] = c3[p[u].vec];
-        d[u] = dh[p[u].vec];
-        ea[u] = e1[p[u].block];
-        eb[u] = e3[p[u].block];
+      const Place p = places(s, u * THREADS + threadIdx.x);
+      if (p.on) {
+        a[u] = c1[p.vec];
+        b[u] = c3[p.vec];
+        d[u] = dh[p.vec];  // a plain load: a gradient may be written over it
+        ea[u] = e1[p.block];
+        eb[u] = e3[p.block];
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      if (!p[u].on) continue;
-      float x[8], y[8], g[8], o1[8], o3[8];
+      const Place p = places(s, u * THREADS + threadIdx.x);
+      if (!p.on) continue;
+      uint64_t x[4], y[4], g[4], o1[4], o3[4];
       decode(a[u], ea[u], x);
       decode(b[u], eb[u], y);
-      unpack8(d[u], g);
+      widen(d[u], g);
+      const uint64_t one = pack2(1.0f, 1.0f), minus = pack2(-1.0f, -1.0f);
 #pragma unroll
-      for (int q = 0; q < 8; q++) {
-        const float sg = sigmoid(x[q]), silu = x[q] * sg;
-        o3[q] = g[q] * silu;
-        o1[q] = g[q] * y[q] * (sg * (1.0f + x[q] * (1.0f - sg)));
-        x[q] = silu * y[q];
+      for (int i = 0; i < 4; i++) {
+        const uint64_t sg = sigmoid2(x[i]), silu = mul2(x[i], sg);
+        o3[i] = mul2(g[i], silu);
+        o1[i] = mul2(mul2(g[i], y[i]), fma2(silu, fma2(sg, minus, one), sg));
+        x[i] = mul2(silu, y[i]);
       }
-      st_stream(dx1 + p[u].vec, pack8(o1));
-      st_stream(dx3 + p[u].vec, pack8(o3));
-      if (out != nullptr) st_stream(out + p[u].vec, pack8(x));
+      st_stream(dx1 + p.vec, round_all(o1));
+      st_stream(dx3 + p.vec, round_all(o3));
+      if (out != nullptr) st_stream(out + p.vec, round_all(x));
     }
   }
 }
@@ -240,6 +286,15 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(Shape s, const uint2 
 }  // namespace b200
 
 using namespace b200;
+
+// the kernel for columns that are whole scale blocks, or the other
+#define ACT8_LAUNCH(kernel, ...)                                                                                            \
+  do {                                                                                                                      \
+    if (s.vecs == s.padded_vecs)                                                                                            \
+      act8::kernel<true><<<act8_grid(s.padded), act8::THREADS, 0, (cudaStream_t)stream>>>(s, __VA_ARGS__);                   \
+    else                                                                                                                    \
+      act8::kernel<false><<<act8_grid(s.padded), act8::THREADS, 0, (cudaStream_t)stream>>>(s, __VA_ARGS__);                  \
+  } while (0)
 
 namespace {
 
@@ -281,8 +336,7 @@ extern "C" int b200_swiglu_act8(int fwd_dt, int n_rows, int n_cols, const void *
   B200_REQUIRE(x_w1 && x_w3 && b200_aligned16(x_w1) && b200_aligned16(x_w3) && b200_aligned16(out),
                "swiglu_act8: x_w1 and x_w3 must be given, and all tensors 16-byte aligned");
   if (act8_codes_ok("swiglu_act8", codes_w1, scales_w1, codes_w3, scales_w3)) return -1;
-  act8::keep_kernel<<<act8_grid(s.padded), act8::THREADS, 0, (cudaStream_t)stream>>>(
-      s, (const uint4 *)x_w1, (const uint4 *)x_w3, (uint4 *)out, (uint2 *)codes_w1, (uint8_t *)scales_w1, (uint2 *)codes_w3,
+  ACT8_LAUNCH(keep_kernel, (const uint4 *)x_w1, (const uint4 *)x_w3, (uint4 *)out, (uint2 *)codes_w1, (uint8_t *)scales_w1, (uint2 *)codes_w3,
       (uint8_t *)scales_w3);
   B200_CHECK_LAUNCH("swiglu_act8");
   return 0;
@@ -297,8 +351,7 @@ extern "C" int b200_swiglu_recompute_act8(int fwd_dt, int n_rows, int n_cols, co
   B200_REQUIRE((x_w1 || x_w3 || out) && b200_aligned16(x_w1) && b200_aligned16(x_w3) && b200_aligned16(out),
                "swiglu_recompute_act8: one output at least must be given, each 16-byte aligned");
   if (act8_codes_ok("swiglu_recompute_act8", codes_w1, scales_w1, codes_w3, scales_w3)) return -1;
-  act8::restore_kernel<<<act8_grid(s.padded), act8::THREADS, 0, (cudaStream_t)stream>>>(
-      s, (const uint2 *)codes_w1, (const uint8_t *)scales_w1, (const uint2 *)codes_w3, (const uint8_t *)scales_w3, (uint4 *)x_w1,
+  ACT8_LAUNCH(restore_kernel, (const uint2 *)codes_w1, (const uint8_t *)scales_w1, (const uint2 *)codes_w3, (const uint8_t *)scales_w3, (uint4 *)x_w1,
       (uint4 *)x_w3, (uint4 *)out);
   B200_CHECK_LAUNCH("swiglu_recompute_act8");
   return 0;
@@ -314,8 +367,7 @@ extern "C" int b200_swiglu_bwd_x_act8(int bwd_dt, int n_rows, int n_cols, const 
                    b200_aligned16(out),
                "swiglu_bwd_x_act8: the upstream gradient and both gradients must be given, and all tensors 16-byte aligned");
   if (act8_codes_ok("swiglu_bwd_x_act8", codes_w1, scales_w1, codes_w3, scales_w3)) return -1;
-  act8::backward_kernel<<<act8_grid(s.padded), act8::THREADS, 0, (cudaStream_t)stream>>>(
-      s, (const uint2 *)codes_w1, (const uint8_t *)scales_w1, (const uint2 *)codes_w3, (const uint8_t *)scales_w3,
+  ACT8_LAUNCH(backward_kernel, (const uint2 *)codes_w1, (const uint8_t *)scales_w1, (const uint2 *)codes_w3, (const uint8_t *)scales_w3,
       (const uint4 *)upstream_dX, (uint4 *)dX_w1, (uint4 *)dX_w3, (uint4 *)out);
   B200_CHECK_LAUNCH("swiglu_bwd_x_act8");
   return 0;

@@ -148,28 +148,6 @@ __device__ __forceinline__ bool all_seen(int base, int pos0, int last, int windo
   return base + TILE - 1 <= pos0 && (base >= last - window + 1 || base + TILE <= sinks);
 }
 
-// two fp32 operations in one instruction
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // x[j] = 2^(x[j] c + off). (A quarter of them by a polynomial on the FMA units, to relieve the special-function units, gave 1 % or took
 // 3 % in the backward and took 15 % in the forward.)
 template <int N>

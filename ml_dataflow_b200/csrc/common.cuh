@@ -63,6 +63,41 @@ __device__ __forceinline__ uint4 pack8(const float *f) {
   return v;
 }
 
+// Pairs of fp32 numbers, and two operations on them in one instruction (sm_100).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// a bf16x2 word as a pair of fp32
+__device__ __forceinline__ uint64_t widen2(uint32_t v) { return pack2(bf16lo(v), bf16hi(v)); }
+__device__ __forceinline__ uint32_t round2(uint64_t v) {
+  float a, b;
+  unpack2(v, a, b);
+  return pack_bf16(a, b);
+}
+__device__ __forceinline__ uint64_t swap2(uint64_t v) {
+  float a, b;
+  unpack2(v, a, b);
+  return pack2(b, a);
+}
+
 // 32-byte global accesses (sm_100): one full 32-byte sector per thread and instruction.
 __device__ __forceinline__ void ld_global_256(const void *p, uint4 &lo, uint4 &hi) {
   asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"

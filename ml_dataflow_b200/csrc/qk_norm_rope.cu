@@ -12,8 +12,9 @@
 // uses them for all heads of its warp.
 //
 // Layout: a head's row of 16-byte vectors lies on the next power of two of lanes (head_dim 128: 16 lanes, two heads per
-// warp at a time), so that the sums are shuffles. A warp takes one token and runs over its heads, four warp-wide vectors
-// in flight. Bound by memory: 4 bytes per element forward, 6 backward.
+// warp at a time), so that the sums are shuffles. A warp takes a token and runs over its heads in rounds of a few warp-wide
+// vectors. Bound by memory, 4 bytes per element forward, 6 backward: to keep enough of it in flight every lane copies the
+// vectors of the next two rounds into places of its own in shared memory (cp.async; registers hold no more than one round).
 #include <math.h>
 
 #include "common.cuh"
@@ -25,12 +26,14 @@ namespace qkn {
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_HEAD_DIM = 256;
-constexpr int BATCH = 4;  // warp-wide vectors in flight
+// Warp-wide vectors of a round, rounds in shared memory, blocks per SM.
+constexpr int BATCH = 4, STAGES = 3, FWD_BLOCKS = 3, BWD_BLOCKS = 2;
+constexpr size_t ring_bytes(bool bwd) { return (size_t)WARPS * STAGES * BATCH * (bwd ? 2 : 1) * 32 * sizeof(uint4); }
 
 struct Params {
   int tokens, q_heads, heads;  // heads = query + key heads
   int head_dim, head_vec;      // head_vec = head_dim / 8
-  int parts;                   // a token's heads are split over this many warps
+  bool spread;                 // a token's rounds of heads go to warps of their own
   float eps, inv_dim;
   double log2_theta;
   const int *pos;
@@ -41,11 +44,8 @@ struct Params {
   float *partial;              // backward with weights: [blocks][2][head_dim]
 };
 
-// plain loads: the output may lie over the input
-__device__ __forceinline__ uint4 ld_once(const uint4 *p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
+__device__ __forceinline__ void copy16(uint4 *dst, const uint4 *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ void turn_angles(double pos, const double *turns, float *cs, float *sn) {
@@ -56,110 +56,168 @@ __device__ __forceinline__ void turn_angles(double pos, const double *turns, flo
   }
 }
 
-// LANES: lanes that share a head (a power of two); BWD: the backward; the weights' gradients when p.partial is not null
+// LANES: lanes that share a head (a power of two); BWD: the backward, with the weights' gradients when p.partial is not null.
+// The query heads of a token come in rounds of AT_ONCE * BATCH, then the key heads. Arithmetic on pairs (2i, 2i + 1): both kernels are
+// as much bound by the instructions they issue as by memory, and packed ones halve them.
 template <int LANES, bool BWD>
-__global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const Params p) {
-  __shared__ double s_turns[MAX_HEAD_DIM / 2];
-  for (int i = threadIdx.x; i < p.head_dim / 2; i += THREADS)
-    s_turns[i] = exp2(-(double)(2 * i) / (double)p.head_dim * p.log2_theta) * 0.15915494309189533577;  // / (2 pi)
-  __syncthreads();
+__global__ void __launch_bounds__(THREADS, BWD ? BWD_BLOCKS : FWD_BLOCKS) qk_norm_rope_kernel(const __grid_constant__ Params p) {
   constexpr int AT_ONCE = 32 / LANES;  // heads
+  constexpr int ROUND = AT_ONCE * BATCH;
+  extern __shared__ uint4 s_ring[];  // [warp][stage][vector][x, dy][lane]
+  __shared__ double s_turns[MAX_HEAD_DIM / 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = lane % LANES, slot = lane / LANES;
   const bool on_row = c < p.head_vec;
-  const int rounds = (p.heads + AT_ONCE * BATCH - 1) / (AT_ONCE * BATCH);
-  const int kv_heads = p.heads - p.q_heads;
-  double turns[4];
-#pragma unroll
-  for (int j = 0; j < 4; j++) turns[j] = on_row ? s_turns[c * 4 + j] : 0.0;
-  float gq[8] = {0, 0, 0, 0, 0, 0, 0, 0}, gk[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const double *turns = s_turns + (on_row ? c * 4 : 0);
+  const int rounds_q = (p.q_heads + ROUND - 1) / ROUND, rounds = rounds_q + (p.heads - p.q_heads + ROUND - 1) / ROUND;
+  uint64_t gq[4] = {0, 0, 0, 0}, gk[4] = {0, 0, 0, 0};  // pairs of zeros
   const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-  const uint4 wq = p.wq && on_row ? __ldg(p.wq + c) : ones, wk = p.wk && on_row ? __ldg(p.wk + c) : ones;
-  const int64_t units = (int64_t)p.tokens * p.parts;
-  for (int64_t unit = (int64_t)blockIdx.x * WARPS + warp; unit < units; unit += (int64_t)gridDim.x * WARPS) {
-    const int64_t tok = unit / p.parts;
-    const int part = (int)(unit - tok * p.parts);
-    float cs[4], sn[4];
-    bool have_angles = false;
-    for (int rd = part; rd < rounds; rd += p.parts) {
-      uint4 x[BATCH], dy[BATCH];
-      int64_t at[BATCH];
+
+  // Many tokens: a warp takes every `stride`th token and all of its rounds. Few: one round of one token.
+  const int w = blockIdx.x * WARPS + warp, stride = gridDim.x * WARPS;
+  struct At {
+    int tok, rd;
+  };
+  const int only = p.spread ? w % rounds : 0;
+  At now = {p.spread ? w / rounds : w, only};
+  auto next = [&](At a) {
+    if (p.spread) return At{p.tokens, 0};
+    return a.rd + 1 < rounds ? At{a.tok, a.rd + 1} : At{a.tok + stride, 0};
+  };
+  struct Where {
+    bool is_q;
+    int heads, h0;
+    int64_t at;
+  };
+  const int step = AT_ONCE * p.head_vec;
+  auto where = [&](At a) {
+    Where r;
+    r.is_q = a.rd < rounds_q;
+    r.heads = r.is_q ? p.q_heads : p.heads - p.q_heads;
+    r.h0 = (r.is_q ? a.rd : a.rd - rounds_q) * ROUND + slot;
+    r.at = ((int64_t)a.tok * r.heads + r.h0) * p.head_vec + c;
+    return r;
+  };
+  constexpr int PER_STAGE = BATCH * (BWD ? 2 : 1) * 32;
+  uint4 *ring = s_ring + warp * STAGES * PER_STAGE + lane;
+  auto fetch = [&](At a, int stage) {
+    if (a.tok < p.tokens) {
+      const Where r = where(a);
+      const uint4 *px = (r.is_q ? p.q : p.k) + r.at, *pd = BWD ? (r.is_q ? p.dyq : p.dyk) + r.at : nullptr;
+      uint4 *to = ring + stage * PER_STAGE;
 #pragma unroll
-      for (int b = 0; b < BATCH; b++) {
-        const int h = (rd * BATCH + b) * AT_ONCE + slot;
-        x[b] = dy[b] = make_uint4(0, 0, 0, 0);
-        at[b] = h < p.q_heads ? (tok * p.q_heads + h) * p.head_vec + c : (tok * kv_heads + (h - p.q_heads)) * p.head_vec + c;
-        if (on_row && h < p.heads) {
-          x[b] = ld_once((h < p.q_heads ? p.q : p.k) + at[b]);
-          if (BWD) dy[b] = ld_once((h < p.q_heads ? p.dyq : p.dyk) + at[b]);
+      for (int b = 0; b < BATCH; b++)
+        if (on_row && r.h0 + b * AT_ONCE < r.heads) {
+          copy16(to + b * (BWD ? 64 : 32), px + b * step);
+          if (BWD) copy16(to + b * 64 + 32, pd + b * step);
         }
-      }
-      if (!have_angles) {  // while the loads are on their way
-        turn_angles((double)__ldg(p.pos + tok), turns, cs, sn);
-        have_angles = true;
-      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  At ahead = now;
 #pragma unroll
-      for (int b = 0; b < BATCH; b++) {
-        const int h = (rd * BATCH + b) * AT_ONCE + slot;
-        const bool is_q = h < p.q_heads;
-        float f[8], w[8];
-        unpack8(x[b], f);
-        unpack8(is_q ? wq : wk, w);
-        float ss = 0.0f;
+  for (int s = 0; s < STAGES - 1; s++) {
+    fetch(ahead, s);
+    if (ahead.tok < p.tokens) ahead = next(ahead);
+  }
+  int pos = now.tok < p.tokens ? __ldg(p.pos + now.tok) : 0;
+  for (int i = threadIdx.x; i < p.head_dim / 2; i += THREADS)  // while the first rounds are on their way
+    s_turns[i] = exp2(-(double)(2 * i) / (double)p.head_dim * p.log2_theta) * 0.15915494309189533577;  // / (2 pi)
+  __syncthreads();
+  float cs[4], sn[4];
+  for (int stage = 0; now.tok < p.tokens; now = next(now)) {
+    fetch(ahead, stage == 0 ? STAGES - 1 : stage - 1);
+    if (ahead.tok < p.tokens) ahead = next(ahead);
+    const Where r = where(now);
+    if (now.rd == only) {  // a new token
+      turn_angles((double)pos, turns, cs, sn);
+      if (!p.spread && now.tok + stride < p.tokens) pos = __ldg(p.pos + now.tok + stride);
+    }
+    const uint4 *weight = r.is_q ? p.wq : p.wk;
+    const uint4 wv = weight && on_row ? __ldg(weight + c) : ones;
+    const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
+    // y = r (keep o x + cross o x'), x' the pair the other way round; in the forward the weights lie in these coefficients
+    uint64_t wt[4], keep[4], cross[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss = fmaf(f[i], f[i], ss);
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = rsqrtf(fmaf(ss, p.inv_dim, p.eps));
-        if (!BWD) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float e = f[2 * j] * r * w[2 * j], o = f[2 * j + 1] * r * w[2 * j + 1];
-            f[2 * j] = cs[j] * e - sn[j] * o;
-            f[2 * j + 1] = cs[j] * o + sn[j] * e;
-          }
-        } else {
-          float g[8], dot = 0.0f;
-          unpack8(dy[b], g);
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float e = g[2 * j], o = g[2 * j + 1];
-            g[2 * j] = cs[j] * e + sn[j] * o;
-            g[2 * j + 1] = cs[j] * o - sn[j] * e;
-          }
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            f[i] *= r;
-            dot = fmaf(g[i] * w[i], f[i], dot);
-          }
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-          dot *= p.inv_dim;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float gn = g[i] * f[i];
-            if (is_q) gq[i] += gn;
-            else gk[i] += gn;
-            f[i] = r * (g[i] * w[i] - f[i] * dot);
-          }
-        }
-        if (on_row && h < p.heads) st_stream((is_q ? p.out_q : p.out_k) + at[b], pack8(f));
+    for (int j = 0; j < 4; j++) {
+      wt[j] = widen2(ww[j]);
+      keep[j] = pack2(cs[j], cs[j]);
+      cross[j] = BWD ? pack2(sn[j], -sn[j]) : pack2(-sn[j], sn[j]);
+      if (!BWD) {
+        keep[j] = mul2(keep[j], wt[j]);
+        cross[j] = mul2(cross[j], swap2(wt[j]));
       }
     }
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    const uint4 *from = ring + stage * PER_STAGE;
+    uint4 *po = (r.is_q ? p.out_q : p.out_k) + r.at;
+#pragma unroll
+    for (int b = 0; b < BATCH; b++) {
+      if (r.h0 - slot + b * AT_ONCE >= r.heads) break;  // the same for the whole warp
+      const bool on = on_row && r.h0 + b * AT_ONCE < r.heads;
+      const uint4 zero = make_uint4(0, 0, 0, 0), x = on ? from[b * (BWD ? 64 : 32)] : zero;
+      const uint32_t xv[4] = {x.x, x.y, x.z, x.w};
+      uint64_t f[4], ss2 = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        f[j] = widen2(xv[j]);
+        ss2 = fma2(f[j], f[j], ss2);
+      }
+      float ss, odd;
+      unpack2(ss2, ss, odd);
+      ss += odd;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float rn = rsqrtf(fmaf(ss, p.inv_dim, p.eps));
+      const uint64_t rr = pack2(rn, rn);
+      uint32_t out[4];
+      if (!BWD) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) out[j] = round2(mul2(rr, fma2(keep[j], f[j], mul2(cross[j], swap2(f[j])))));
+      } else {
+        const uint4 dy = on ? from[b * 64 + 32] : zero;
+        const uint32_t dv[4] = {dy.x, dy.y, dy.z, dy.w};
+        uint64_t a[4], dot2 = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint64_t d = widen2(dv[j]), g = fma2(keep[j], d, mul2(cross[j], swap2(d)));
+          f[j] = mul2(f[j], rr);
+          if (r.is_q) gq[j] = fma2(g, f[j], gq[j]);
+          else gk[j] = fma2(g, f[j], gk[j]);
+          a[j] = mul2(g, wt[j]);
+          dot2 = fma2(a[j], f[j], dot2);
+        }
+        float dot, odd2;
+        unpack2(dot2, dot, odd2);
+        dot += odd2;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        dot *= -p.inv_dim;
+        const uint64_t minus = pack2(dot, dot);
+#pragma unroll
+        for (int j = 0; j < 4; j++) out[j] = round2(mul2(rr, fma2(f[j], minus, a[j])));
+      }
+      if (on) st_stream(po + b * step, make_uint4(out[0], out[1], out[2], out[3]));
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   if (!BWD || p.partial == nullptr) return;
   // the block's share of the weight gradients: slots of a warp, then warps, each in a fixed order
   __shared__ float s_sum[WARPS][2][MAX_HEAD_DIM];
 #pragma unroll
   for (int i = 0; i < 8; i++) {
+    float q0, q1, k0, k1;
+    unpack2(gq[i >> 1], q0, q1);
+    unpack2(gk[i >> 1], k0, k1);
+    float q = i & 1 ? q1 : q0, k = i & 1 ? k1 : k0;
 #pragma unroll
     for (int o = LANES; o < 32; o <<= 1) {
-      gq[i] += __shfl_xor_sync(0xffffffffu, gq[i], o);
-      gk[i] += __shfl_xor_sync(0xffffffffu, gk[i], o);
+      q += __shfl_xor_sync(0xffffffffu, q, o);
+      k += __shfl_xor_sync(0xffffffffu, k, o);
     }
     if (slot == 0 && on_row) {
-      s_sum[warp][0][c * 8 + i] = gq[i];
-      s_sum[warp][1][c * 8 + i] = gk[i];
+      s_sum[warp][0][c * 8 + i] = q;
+      s_sum[warp][1][c * 8 + i] = k;
     }
   }
   __syncthreads();
@@ -172,24 +230,25 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const Params p) {
   }
 }
 
-// dw = (dw +) sum of the blocks' shares: a block takes 32 columns, its eight warps every eighth share, then the eight sums
-// in warp order
-__global__ void __launch_bounds__(256) qk_weight_grad_kernel(int head_dim, int blocks, const float *__restrict__ partial, bool accumulate,
-                                                             __nv_bfloat16 *dwq, __nv_bfloat16 *dwk) {
-  __shared__ float part[8][32];
+// dw = (dw +) sum of the blocks' shares: a block takes 32 columns, its 32 warps every 32nd share (all asked for at once: with eight warps
+// this took 7 us), then the warps' sums in order
+constexpr int JOIN_WARPS = 32;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) qk_weight_grad_kernel(int head_dim, int blocks, const float *__restrict__ partial,
+                                                                       bool accumulate, __nv_bfloat16 *dwq, __nv_bfloat16 *dwk) {
+  __shared__ float part[JOIN_WARPS][32];
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int i = blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (i < 2 * head_dim) {
-#pragma unroll 4
-    for (int b = grp; b < blocks; b += 8) s += partial[(int64_t)b * 2 * head_dim + i];
+#pragma unroll 8
+    for (int b = grp; b < blocks; b += JOIN_WARPS) s += partial[(int64_t)b * 2 * head_dim + i];
   }
   part[grp][lane] = s;
   __syncthreads();
   if (grp != 0 || i >= 2 * head_dim) return;
   float t = 0.0f;
 #pragma unroll
-  for (int g = 0; g < 8; g++) t += part[g][lane];
+  for (int g = 0; g < JOIN_WARPS; g++) t += part[g][lane];
   __nv_bfloat16 *dw = i < head_dim ? dwq : dwk;
   if (dw == nullptr) return;
   dw += i < head_dim ? i : i - head_dim;
@@ -215,33 +274,44 @@ int qkn_lanes(int head_dim) {
   return l;
 }
 
-// Warps per token: one, as long as the tokens alone give every SM 16 warps; else as many as there are rounds of heads, so that few
-// tokens spread over the GPU.
-constexpr int QKN_MANY_TOKENS = 148 * 16;
-int qkn_parts(int tokens, int heads, int head_dim) {
-  const int at_once = 32 / qkn_lanes(head_dim) * qkn::BATCH, rounds = (heads + at_once - 1) / at_once;
-  return tokens >= QKN_MANY_TOKENS ? 1 : rounds;
+// A warp takes whole tokens as long as these alone give every SM 16 warps (backward: 4; its blocks' shares of the weight gradients have to
+// be added up); below that every round of heads gets a warp, so that few tokens spread over the GPU.
+constexpr int QKN_SPREAD_FWD = 148 * 16, QKN_SPREAD_BWD = 148 * 4;
+bool qkn_spread(int tokens, bool bwd) { return tokens < (bwd ? QKN_SPREAD_BWD : QKN_SPREAD_FWD); }
+
+int qkn_blocks(int tokens, int q_heads, int heads, int head_dim, bool bwd) {
+  const int round = 32 / qkn_lanes(head_dim) * qkn::BATCH, rounds = (q_heads + round - 1) / round + (heads - q_heads + round - 1) / round;
+  if (qkn_spread(tokens, bwd)) return (int)(((int64_t)tokens * rounds + qkn::WARPS - 1) / qkn::WARPS);
+  const int want = (tokens - 1) / qkn::WARPS + 1, most = qkn_sms() * (bwd ? qkn::BWD_BLOCKS : qkn::FWD_BLOCKS);
+  return want < most ? want : most;
 }
 
-int qkn_blocks(int tokens, int heads, int head_dim, int per_sm) {
-  const int64_t units = (int64_t)tokens * qkn_parts(tokens, heads, head_dim);
-  const int64_t want = (units + qkn::WARPS - 1) / qkn::WARPS, most = (int64_t)qkn_sms() * per_sm;
-  return (int)(want < most ? want : most);
+template <int LANES, bool BWD>
+int qkn_launch_lanes(const char *op, const qkn::Params &p, int blocks, cudaStream_t s) {
+  static bool done[64];
+  int dev = -1;
+  B200_CUDA(cudaGetDevice(&dev));
+  B200_REQUIRE(dev >= 0 && dev < 64, "%s: device ordinal %d is out of range", op, dev);
+  constexpr size_t smem = qkn::ring_bytes(BWD);
+  if (!done[dev]) {
+    B200_CUDA(cudaFuncSetAttribute(qkn::qk_norm_rope_kernel<LANES, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    done[dev] = true;
+  }
+  qkn::qk_norm_rope_kernel<LANES, BWD><<<blocks, qkn::THREADS, smem, s>>>(p);
+  B200_CHECK_LAUNCH(op);
+  return 0;
 }
-constexpr int QKN_FWD_PER_SM = 8, QKN_BWD_PER_SM = 4;
 
 template <bool BWD>
 int qkn_launch(const char *op, const qkn::Params &p, int blocks, cudaStream_t s) {
   switch (qkn_lanes(p.head_dim)) {
-    case 1: qkn::qk_norm_rope_kernel<1, BWD><<<blocks, qkn::THREADS, 0, s>>>(p); break;
-    case 2: qkn::qk_norm_rope_kernel<2, BWD><<<blocks, qkn::THREADS, 0, s>>>(p); break;
-    case 4: qkn::qk_norm_rope_kernel<4, BWD><<<blocks, qkn::THREADS, 0, s>>>(p); break;
-    case 8: qkn::qk_norm_rope_kernel<8, BWD><<<blocks, qkn::THREADS, 0, s>>>(p); break;
-    case 16: qkn::qk_norm_rope_kernel<16, BWD><<<blocks, qkn::THREADS, 0, s>>>(p); break;
-    default: qkn::qk_norm_rope_kernel<32, BWD><<<blocks, qkn::THREADS, 0, s>>>(p); break;
+    case 1: return qkn_launch_lanes<1, BWD>(op, p, blocks, s);
+    case 2: return qkn_launch_lanes<2, BWD>(op, p, blocks, s);
+    case 4: return qkn_launch_lanes<4, BWD>(op, p, blocks, s);
+    case 8: return qkn_launch_lanes<8, BWD>(op, p, blocks, s);
+    case 16: return qkn_launch_lanes<16, BWD>(op, p, blocks, s);
+    default: return qkn_launch_lanes<32, BWD>(op, p, blocks, s);
   }
-  B200_CHECK_LAUNCH(op);
-  return 0;
 }
 
 int qkn_params(const char *op, qkn::Params *p, int dt, int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, float eps, int theta,
@@ -264,7 +334,6 @@ int qkn_params(const char *op, qkn::Params *p, int dt, int num_tokens, int num_q
   p->heads = num_q_heads + num_kv_heads;
   p->head_dim = head_dim;
   p->head_vec = head_dim / 8;
-  p->parts = qkn_parts(num_tokens, p->heads, head_dim);
   p->eps = eps;
   p->inv_dim = 1.0f / (float)head_dim;
   p->log2_theta = log2((double)theta);
@@ -288,14 +357,16 @@ extern "C" int b200_qk_norm_rope(int fwd_dt, int num_tokens, int num_q_heads, in
                  X_q, X_k, out_q, out_k))
     return -1;
   if (num_tokens == 0) return 0;
-  return qkn_launch<false>("qk_norm_rope", p, qkn_blocks(num_tokens, p.heads, head_dim, QKN_FWD_PER_SM), (cudaStream_t)stream);
+  p.spread = qkn_spread(num_tokens, false);
+  return qkn_launch<false>("qk_norm_rope", p, qkn_blocks(num_tokens, p.q_heads, p.heads, head_dim, false), (cudaStream_t)stream);
 }
 
 extern "C" uint64_t b200_qk_norm_rope_bwd_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, int head_dim) {
   if (num_tokens <= 0 || num_q_heads < 1 || num_kv_heads < 0 || head_dim < 8 || head_dim % 8 || head_dim > qkn::MAX_HEAD_DIM) return 0;
   // enough for every smaller number of tokens too: the most blocks may run just below the border between the two layouts
-  const int below = num_tokens < QKN_MANY_TOKENS ? num_tokens : QKN_MANY_TOKENS - 1, heads = num_q_heads + num_kv_heads;
-  const int a = qkn_blocks(num_tokens, heads, head_dim, QKN_BWD_PER_SM), b = qkn_blocks(below, heads, head_dim, QKN_BWD_PER_SM);
+  const int below = num_tokens < QKN_SPREAD_BWD ? num_tokens : QKN_SPREAD_BWD - 1, heads = num_q_heads + num_kv_heads;
+  const int a = qkn_blocks(num_tokens, num_q_heads, heads, head_dim, true),
+            b = qkn_blocks(below, num_q_heads, heads, head_dim, true);
   return (uint64_t)(a > b ? a : b) * 2 * head_dim * sizeof(float);
 }
 
@@ -316,7 +387,8 @@ extern "C" int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int
   }
   B200_REQUIRE(d_out_q && (num_kv_heads == 0 || d_out_k) && b200_aligned16(d_out_q) && b200_aligned16(d_out_k),
                "qk_norm_rope_bwd: the upstream gradients must be given and 16-byte aligned");
-  const int blocks = qkn_blocks(num_tokens, p.heads, head_dim, QKN_BWD_PER_SM);
+  p.spread = qkn_spread(num_tokens, true);
+  const int blocks = qkn_blocks(num_tokens, p.q_heads, p.heads, head_dim, true);
   if (want_dw) {
     const uint64_t need = (uint64_t)blocks * 2 * head_dim * sizeof(float);
     B200_REQUIRE(workspace && b200_aligned16(workspace) && workspace_bytes >= need,
@@ -328,7 +400,7 @@ extern "C" int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int
   p.dyk = (const uint4 *)d_out_k;
   if (qkn_launch<true>("qk_norm_rope_bwd", p, blocks, (cudaStream_t)stream)) return -1;
   if (!want_dw) return 0;
-  qkn::qk_weight_grad_kernel<<<(2 * head_dim + 31) / 32, 256, 0, (cudaStream_t)stream>>>(
+  qkn::qk_weight_grad_kernel<<<(2 * head_dim + 31) / 32, qkn::JOIN_WARPS * 32, 0, (cudaStream_t)stream>>>(
       head_dim, blocks, p.partial, accumulate != 0, (__nv_bfloat16 *)dq_weight, (__nv_bfloat16 *)dk_weight);
   B200_CHECK_LAUNCH("qk_norm_rope_bwd (weights)");
   return 0;
