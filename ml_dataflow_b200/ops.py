@@ -7,6 +7,7 @@ non-zero return from the library raises `RuntimeError` (the reference returns -1
 used for device memory and streams; every op runs a hand-written sm_100a kernel through ctypes.
 """
 import ctypes as C
+from array import array
 
 import torch
 
@@ -422,39 +423,51 @@ def attention_bwd(q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_head
 
 
 # ---- checks of the ops below: the library sees plain pointers, so shapes, types, devices and strides are checked here ----
-def _want(op, device, **tensors):
-    """tensors: name -> (tensor or None, number of elements it must hold, dtype). They must lie packed on `device`, which must
-    be the current one: the library launches there, on torch's current stream."""
-    if device.type != "cuda":
-        raise ValueError(f"{op}: the tensors are on {device}, not on a GPU")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"{op}: the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    for name, (t, n, dtype) in tensors.items():
-        if t is None:
-            continue
-        if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < n:
-            raise ValueError(f"{op}: {name} must be {n} contiguous values of {dtype} on {device}, got {tuple(t.shape)} of {t.dtype} "
-                             f"on {t.device}{'' if t.is_contiguous() else ', strided'}")
+def _here(op, t):
+    """The current device's index, where `t` has to be: the library launches there, on torch's current stream."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{op}: the tensors are on {t.device}, not on a GPU")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"{op}: the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return dev
 
 
-def _sizes(op, **values):
-    for name, v in values.items():
+def _ptr(op, name, t, n, dtype, dev, optional=False):
+    """The address of `t`, which has to hold at least n packed values of dtype on device dev."""
+    if t is None:
+        if optional or n == 0:
+            return None
+        raise ValueError(f"{op}: {name} is missing")
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{op}: {name} must be {n} contiguous values of {dtype} on cuda:{dev}, got {tuple(t.shape)} of {t.dtype} on "
+                         f"{t.device}{'' if t.is_contiguous() else ', strided'}")
+    return t.data_ptr()
+
+
+def _sizes(op, *values):
+    for v in values:
         if not 0 <= v < 1 << 31:  # ctypes would cut a larger number to 32 bits
-            raise ValueError(f"{op}: {name} must be at least 0 and below 2^31, got {v}")
+            raise ValueError(f"{op}: sizes must be at least 0 and below 2^31, got {v}")
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_BF, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
 
 # ---- RMSNorm of every query and key head, with the rotation -----------------------------------------------------------
 def qk_norm_rope(num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta, seq_positions, q_weight, k_weight, X_q, X_k, out_q,
                  out_k):
     """q_weight, k_weight: [head_dim] or None. out_q / out_k may be X_q / X_k where no backward follows."""
-    _sizes("qk_norm_rope", num_tokens=num_tokens, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads, head_dim=head_dim,
-           theta=theta)
-    nq, nk, bf = num_tokens * num_q_heads * head_dim, num_tokens * num_kv_heads * head_dim, torch.bfloat16
-    _want("qk_norm_rope", X_q.device, seq_positions=(seq_positions, num_tokens, torch.int32), q_weight=(q_weight, head_dim, bf),
-          k_weight=(k_weight, head_dim, bf), X_q=(X_q, nq, bf), X_k=(X_k, nk, bf), out_q=(out_q, nq, bf), out_k=(out_k, nk, bf))
-    _check(_lib.load().b200_qk_norm_rope(DT_BF16, num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta, _p(seq_positions),
-                                         _p(q_weight), _p(k_weight), _p(X_q), _p(X_k), _p(out_q), _p(out_k), _stream()),
-           "qk_norm_rope")
+    op = "qk_norm_rope"
+    _sizes(op, num_tokens, num_q_heads, num_kv_heads, head_dim, theta)
+    dev, nq, nk = _here(op, X_q), num_tokens * num_q_heads * head_dim, num_tokens * num_kv_heads * head_dim
+    _check(_lib.load().b200_qk_norm_rope(
+        DT_BF16, num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta, _ptr(op, "seq_positions", seq_positions, num_tokens, _I32, dev),
+        _ptr(op, "q_weight", q_weight, head_dim, _BF, dev, True), _ptr(op, "k_weight", k_weight, head_dim, _BF, dev, True),
+        _ptr(op, "X_q", X_q, nq, _BF, dev), _ptr(op, "X_k", X_k, nk, _BF, dev), _ptr(op, "out_q", out_q, nq, _BF, dev),
+        _ptr(op, "out_k", out_k, nk, _BF, dev), _raw_stream(dev)), op)
 
 
 def qk_norm_rope_bwd_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, head_dim):
@@ -465,19 +478,17 @@ def qk_norm_rope_bwd(num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta
                      d_out_q, d_out_k, dX_q, dX_k, dq_weight=None, dk_weight=None, accumulate=True, workspace=None):
     """X_q, X_k: the forward's inputs. The weight gradients are added to (accumulate) or written, and skipped when None; they need
     the workspace (uint8)."""
-    _sizes("qk_norm_rope_bwd", num_tokens=num_tokens, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads, head_dim=head_dim,
-           theta=theta)
-    nq, nk, bf = num_tokens * num_q_heads * head_dim, num_tokens * num_kv_heads * head_dim, torch.bfloat16
-    _want("qk_norm_rope_bwd", X_q.device, seq_positions=(seq_positions, num_tokens, torch.int32), q_weight=(q_weight, head_dim, bf),
-          k_weight=(k_weight, head_dim, bf), X_q=(X_q, nq, bf), X_k=(X_k, nk, bf), d_out_q=(d_out_q, nq, bf),
-          d_out_k=(d_out_k, nk, bf), dX_q=(dX_q, nq, bf), dX_k=(dX_k, nk, bf), dq_weight=(dq_weight, head_dim, bf),
-          dk_weight=(dk_weight, head_dim, bf), workspace=(workspace, 0, torch.uint8))
-    want_dw = dq_weight is not None or dk_weight is not None
-    _check(_lib.load().b200_qk_norm_rope_bwd(DT_BF16, DT_BF16, num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta,
-                                             _p(seq_positions), _p(q_weight), _p(k_weight), _p(X_q), _p(X_k), _p(d_out_q),
-                                             _p(d_out_k), _p(dX_q), _p(dX_k), _p(dq_weight), _p(dk_weight), int(bool(accumulate)),
-                                             0 if workspace is None else workspace.numel(), _p(workspace), _stream()),
-           "qk_norm_rope_bwd", 2 if want_dw else 1)
+    op = "qk_norm_rope_bwd"
+    _sizes(op, num_tokens, num_q_heads, num_kv_heads, head_dim, theta)
+    dev, nq, nk = _here(op, X_q), num_tokens * num_q_heads * head_dim, num_tokens * num_kv_heads * head_dim
+    _check(_lib.load().b200_qk_norm_rope_bwd(
+        DT_BF16, DT_BF16, num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta,
+        _ptr(op, "seq_positions", seq_positions, num_tokens, _I32, dev), _ptr(op, "q_weight", q_weight, head_dim, _BF, dev, True),
+        _ptr(op, "k_weight", k_weight, head_dim, _BF, dev, True), _ptr(op, "X_q", X_q, nq, _BF, dev), _ptr(op, "X_k", X_k, nk, _BF, dev),
+        _ptr(op, "d_out_q", d_out_q, nq, _BF, dev), _ptr(op, "d_out_k", d_out_k, nk, _BF, dev), _ptr(op, "dX_q", dX_q, nq, _BF, dev),
+        _ptr(op, "dX_k", dX_k, nk, _BF, dev), _ptr(op, "dq_weight", dq_weight, head_dim, _BF, dev, True),
+        _ptr(op, "dk_weight", dk_weight, head_dim, _BF, dev, True), 1 if accumulate else 0, 0 if workspace is None else workspace.numel(),
+        _ptr(op, "workspace", workspace, 0, _U8, dev), _raw_stream(dev)), op, 1 if dq_weight is None and dk_weight is None else 2)
 
 
 # ---- attention with a sliding window and sink tokens ---------------------------------------------------------------------
@@ -488,43 +499,41 @@ def attention_window_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_d
 
 def _window_args(op, q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v, x_attn_out, softmax_lse,
                  window, num_sinks):
+    """(device, host arrays to keep until the call, the C call's arguments from the datatype to softmax_lse, elements of x_q and x_k)"""
     n = len(q_lens)
     if not n == len(q_offsets) == len(k_offsets) == len(k_lens):
         raise ValueError(f"{op}: the four sequence lists have {len(q_offsets)}, {n}, {len(k_offsets)} and {len(k_lens)} entries")
     if x_q.dim() != 2 or x_k.dim() != 2:
         raise ValueError(f"{op}: x_q and x_k must be [rows][heads * head_dim], got {tuple(x_q.shape)} and {tuple(x_k.shape)}")
-    _sizes(op, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, window=window, num_sinks=num_sinks)
-    tq, tk, bf = x_q.shape[0], x_k.shape[0], torch.bfloat16
+    _sizes(op, num_q_heads, num_kv_heads, head_dim, window, num_sinks)
+    dev, tq, tk = _here(op, x_q), x_q.shape[0], x_k.shape[0]
     nq, nk = tq * num_q_heads * head_dim, tk * num_kv_heads * head_dim
-    _want(op, x_q.device, x_q=(x_q, nq, bf), x_k=(x_k, nk, bf), x_v=(x_v, nk, bf), x_attn_out=(x_attn_out, nq, bf),
-          softmax_lse=(softmax_lse, num_q_heads * tq, torch.float32))
-    return n, tq, tk, nq, nk
+    host = [array("i", v) for v in (q_offsets, q_lens, k_offsets, k_lens)]
+    return dev, host, (DT_BF16, n, tq, tk, *[a.buffer_info()[0] for a in host], num_q_heads, num_kv_heads, head_dim,
+                       _ptr(op, "x_q", x_q, nq, _BF, dev), _ptr(op, "x_k", x_k, nk, _BF, dev), _ptr(op, "x_v", x_v, nk, _BF, dev),
+                       _ptr(op, "x_attn_out", x_attn_out, nq, _BF, dev),
+                       _ptr(op, "softmax_lse", softmax_lse, num_q_heads * tq, _F32, dev)), nq, nk
 
 
 def attention_window_fwd(q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v, x_attn_out,
                          softmax_lse, window, num_sinks):
     """A query sees its own key, the window - 1 keys before it and the first num_sinks keys of its sequence."""
-    n, tq, tk, _, _ = _window_args("attention_window_fwd", q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim,
-                                   x_q, x_k, x_v, x_attn_out, softmax_lse, window, num_sinks)
-    _check(_lib.load().b200_attention_window_fwd(DT_BF16, n, tq, tk, _int_array(q_offsets), _int_array(q_lens), _int_array(k_offsets),
-                                                 _int_array(k_lens), num_q_heads, num_kv_heads, head_dim, _p(x_q), _p(x_k), _p(x_v),
-                                                 _p(x_attn_out), _p(softmax_lse), window, num_sinks, _stream()),
-           "attention_window_fwd", -(-n // 48))
+    op = "attention_window_fwd"
+    dev, host, args, _, _ = _window_args(op, q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v,
+                                         x_attn_out, softmax_lse, window, num_sinks)
+    _check(_lib.load().b200_attention_window_fwd(*args, window, num_sinks, _raw_stream(dev)), op, -(-len(q_lens) // 48))
 
 
 def attention_window_bwd(q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v, x_attn_out,
                          softmax_lse, dx_out, dx_q, dx_k, dx_v, window, num_sinks, workspace):
     """x_attn_out, softmax_lse: the forward's. workspace: uint8, attention_window_workspace_bytes of it."""
     op = "attention_window_bwd"
-    n, tq, tk, nq, nk = _window_args(op, q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v,
-                                     x_attn_out, softmax_lse, window, num_sinks)
-    bf = torch.bfloat16
-    _want(op, x_q.device, dx_out=(dx_out, nq, bf), dx_q=(dx_q, nq, bf), dx_k=(dx_k, nk, bf), dx_v=(dx_v, nk, bf),
-          workspace=(workspace, 0, torch.uint8))
-    _check(_lib.load().b200_attention_window_bwd(DT_BF16, n, tq, tk, _int_array(q_offsets), _int_array(q_lens), _int_array(k_offsets),
-                                                 _int_array(k_lens), num_q_heads, num_kv_heads, head_dim, _p(x_q), _p(x_k), _p(x_v),
-                                                 _p(x_attn_out), _p(softmax_lse), _p(dx_out), _p(dx_q), _p(dx_k), _p(dx_v), window,
-                                                 num_sinks, workspace.numel(), _p(workspace), _stream()), op, 2 * -(-n // 48))
+    dev, host, args, nq, nk = _window_args(op, q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v,
+                                           x_attn_out, softmax_lse, window, num_sinks)
+    _check(_lib.load().b200_attention_window_bwd(
+        *args, _ptr(op, "dx_out", dx_out, nq, _BF, dev), _ptr(op, "dx_q", dx_q, nq, _BF, dev), _ptr(op, "dx_k", dx_k, nk, _BF, dev),
+        _ptr(op, "dx_v", dx_v, nk, _BF, dev), window, num_sinks, workspace.numel(), _ptr(op, "workspace", workspace, 0, _U8, dev),
+        _raw_stream(dev)), op, 2 * -(-len(q_lens) // 48))
 
 
 # ---- SwiGLU activations held in 8 bits --------------------------------------------------------------------------------------
@@ -532,32 +541,35 @@ def act8_scales_bytes(n_rows, n_cols):
     return int(_lib.load().b200_act8_scales_bytes(n_rows, n_cols))
 
 
-def _act8_want(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, **tensors):
-    _sizes(op, n_rows=n_rows, n_cols=n_cols)
-    n, ns = n_rows * n_cols, n_rows * ((n_cols + 31) // 32)
-    _want(op, codes_w1.device, codes_w1=(codes_w1, n, torch.uint8), scales_w1=(scales_w1, ns, torch.uint8),
-          codes_w3=(codes_w3, n, torch.uint8), scales_w3=(scales_w3, ns, torch.uint8),
-          **{k: (t, n, torch.bfloat16) for k, t in tensors.items()})
+def _act8_args(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3):
+    _sizes(op, n_rows, n_cols)
+    dev, n, ns = _here(op, codes_w1), n_rows * n_cols, n_rows * ((n_cols + 31) // 32)
+    return dev, n, (_ptr(op, "codes_w1", codes_w1, n, _U8, dev), _ptr(op, "scales_w1", scales_w1, ns, _U8, dev),
+                    _ptr(op, "codes_w3", codes_w3, n, _U8, dev), _ptr(op, "scales_w3", scales_w3, ns, _U8, dev))
 
 
 def swiglu_act8(n_rows, n_cols, x_w1, x_w3, out, codes_w1, scales_w1, codes_w3, scales_w3):
     """out = silu(x_w1) * x_w3 (skipped when None), and x_w1, x_w3 in 8 bits: codes uint8 [n_rows][n_cols], scales uint8
     [n_rows][ceil(n_cols / 32)]."""
-    _act8_want("swiglu_act8", n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, x_w1=x_w1, x_w3=x_w3, out=out)
-    _check(_lib.load().b200_swiglu_act8(DT_BF16, n_rows, n_cols, _p(x_w1), _p(x_w3), _p(out), _p(codes_w1), _p(scales_w1),
-                                        _p(codes_w3), _p(scales_w3), _stream()), "swiglu_act8")
+    op = "swiglu_act8"
+    dev, n, held = _act8_args(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3)
+    _check(_lib.load().b200_swiglu_act8(DT_BF16, n_rows, n_cols, _ptr(op, "x_w1", x_w1, n, _BF, dev), _ptr(op, "x_w3", x_w3, n, _BF, dev),
+                                        _ptr(op, "out", out, n, _BF, dev, True), *held, _raw_stream(dev)), op)
 
 
 def swiglu_recompute_act8(n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, x_w1=None, x_w3=None, out=None):
     """The held x_w1, x_w3 and out = silu(x_w1) * x_w3 of them, each when given."""
-    _act8_want("swiglu_recompute_act8", n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, x_w1=x_w1, x_w3=x_w3, out=out)
-    _check(_lib.load().b200_swiglu_recompute_act8(DT_BF16, n_rows, n_cols, _p(codes_w1), _p(scales_w1), _p(codes_w3), _p(scales_w3),
-                                                  _p(x_w1), _p(x_w3), _p(out), _stream()), "swiglu_recompute_act8")
+    op = "swiglu_recompute_act8"
+    dev, n, held = _act8_args(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3)
+    _check(_lib.load().b200_swiglu_recompute_act8(DT_BF16, n_rows, n_cols, *held, _ptr(op, "x_w1", x_w1, n, _BF, dev, True),
+                                                  _ptr(op, "x_w3", x_w3, n, _BF, dev, True), _ptr(op, "out", out, n, _BF, dev, True),
+                                                  _raw_stream(dev)), op)
 
 
 def swiglu_bwd_x_act8(n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, upstream_dX, dX_w1, dX_w3, out=None):
     """swiglu_bwd_x on the held values; out, when given, receives silu(x_w1) * x_w3 of them."""
-    _act8_want("swiglu_bwd_x_act8", n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, upstream_dX=upstream_dX, dX_w1=dX_w1,
-               dX_w3=dX_w3, out=out)
-    _check(_lib.load().b200_swiglu_bwd_x_act8(DT_BF16, n_rows, n_cols, _p(codes_w1), _p(scales_w1), _p(codes_w3), _p(scales_w3),
-                                              _p(upstream_dX), _p(dX_w1), _p(dX_w3), _p(out), _stream()), "swiglu_bwd_x_act8")
+    op = "swiglu_bwd_x_act8"
+    dev, n, held = _act8_args(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3)
+    _check(_lib.load().b200_swiglu_bwd_x_act8(DT_BF16, n_rows, n_cols, *held, _ptr(op, "upstream_dX", upstream_dX, n, _BF, dev),
+                                              _ptr(op, "dX_w1", dX_w1, n, _BF, dev), _ptr(op, "dX_w3", dX_w3, n, _BF, dev),
+                                              _ptr(op, "out", out, n, _BF, dev, True), _raw_stream(dev)), op)
