@@ -423,6 +423,10 @@ int b200_moe_block_recompute(const B200MoeBlock *block, const void *Xn, int reco
 #define B200_SAVED_ACTIVATION_LEVEL_INP_ONLY 1
 #define B200_SAVED_ACTIVATION_LEVEL_INP_ATTN_ONLY 2
 #define B200_SAVED_ACTIVATION_LEVEL_FULL 3
+/* as FULL, with x1 and x3 in 8 bits (b200_swiglu_act8; no counterpart in the reference): half the bytes, gradients of the held values.
+ * The buffer must be memory of the current device or pinned host memory (kernels write and read it), 8-byte aligned. The restore
+ * writes x1, x3 and h; b200_moe_block_recompute_level then gathers the zone. */
+#define B200_SAVED_ACTIVATION_LEVEL_FULL_8BIT 4
 
 /* Bytes of the MoE part of a saved-activations buffer at `level` (0 for NONE or an unknown level): the tensors
  * above in the reference's order, each starting on a 256-byte boundary as in prep_seq_batch.c:230-283. */
@@ -872,7 +876,7 @@ int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, int total_k
  * b200_swiglu_act8: b200_swiglu (out = silu(x_w1) * x_w3; not formed when out is NULL) that also holds its inputs.
  * b200_swiglu_recompute_act8: the held x_w1, x_w3 as bf16 and h = silu(x_w1) * x_w3 of them, each when not NULL.
  * b200_swiglu_bwd_x_act8: b200_swiglu_bwd_x on the held values; out, when not NULL, receives h of them. dX_w1 or dX_w3 may be
- * upstream_dX itself. n_cols a multiple of 8; bf16 tensors and codes 16-byte aligned. No counterpart in the reference, which
+ * upstream_dX itself. n_cols a multiple of 8; bf16 tensors 16-byte aligned, codes 8-byte aligned. No counterpart in the reference, which
  * keeps them in 16 bits or not at all.
  */
 uint64_t b200_act8_scales_bytes(int n_rows, int n_cols);
@@ -931,6 +935,33 @@ int b200_transformer_block_fwd(const B200TransformerBlock *block, const void *x,
  * accumulated into (beta = 1), as by the reference's gradient GEMMs and norm kernels, unless grads->overwrite is set. */
 int b200_transformer_block_bwd(const B200TransformerBlock *block, const void *x, void *dx, const B200TransformerBlockGrads *grads,
                                const B200TransformerBlockScratch *scratch, void *stream);
+
+/*
+ * The same block with what a configuration may add to it; NULL options are the two calls above.
+ *  - qk_norm: queries and keys are normed per head before the rotation (b200_qk_norm_rope). q_raw, k_raw hold the projections (the
+ *    backward reads them; the shapes of q, k). q_norm, k_norm [head_dim] may be NULL; their gradients d_q_norm, d_k_norm, when not NULL,
+ *    are accumulated into or written as grads->overwrite says, through qk_workspace (b200_qk_norm_rope_bwd_workspace_bytes).
+ *  - window > 0: attention with a sliding window and num_sinks sink tokens (b200_attention_window_fwd); attn_workspace is then sized by
+ *    b200_attention_window_workspace_bytes(num_seqs, ..., total_tokens, num_sinks).
+ *  - codes_w1 ... scales_w3 (all or none): x1 and x3 are held there in 8 bits after the forward, and the backward takes them, h and the
+ *    gathered zone from what is held: moe.x1, x3, h, zone and Y may then be shared by every block of a model.
+ */
+typedef struct B200TransformerBlockOptions {
+  int qk_norm;
+  float qk_eps;
+  const void *q_norm, *k_norm;
+  void *q_raw, *k_raw;
+  void *d_q_norm, *d_k_norm;
+  void *qk_workspace;
+  uint64_t qk_workspace_bytes;
+  int window, num_sinks;
+  void *codes_w1, *scales_w1, *codes_w3, *scales_w3;
+} B200TransformerBlockOptions;
+
+int b200_transformer_block_fwd_options(const B200TransformerBlock *block, const B200TransformerBlockOptions *options, const void *x, void *out,
+                                       void *stream);
+int b200_transformer_block_bwd_options(const B200TransformerBlock *block, const B200TransformerBlockOptions *options, const void *x, void *dx,
+                                       const B200TransformerBlockGrads *grads, const B200TransformerBlockScratch *scratch, void *stream);
 
 #ifdef __cplusplus
 }

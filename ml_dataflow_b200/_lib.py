@@ -90,6 +90,8 @@ SIGNATURES = {
     "b200_transformer_block_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_scatter_row_weights": (_i, [_i, _i, _vp, _vp, _vp, _vp]),
     "b200_gather_router_grad": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "b200_transformer_block_fwd_options": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "b200_transformer_block_bwd_options": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_qk_norm_rope": (_i, [_i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_qk_norm_rope_bwd_workspace_bytes": (_u64, [_i, _i, _i, _i]),
     "b200_qk_norm_rope_bwd": (_i, [_i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i,
@@ -141,6 +143,15 @@ class TransformerBlockGrads(C.Structure):
 
 class TransformerBlockScratch(C.Structure):
     _fields_ = [(n, _vp) for n in ("dxn", "dattn", "dq", "dk", "dv", "norm_workspace")] + [("norm_workspace_bytes", _u64)]
+
+
+class TransformerBlockOptions(C.Structure):
+    """ctypes mirror of B200TransformerBlockOptions in include/b200_moe.h (same field order)."""
+    _fields_ = [
+        ("qk_norm", _i), ("qk_eps", C.c_float), ("q_norm", _vp), ("k_norm", _vp), ("q_raw", _vp), ("k_raw", _vp), ("d_q_norm", _vp),
+        ("d_k_norm", _vp), ("qk_workspace", _vp), ("qk_workspace_bytes", _u64), ("window", _i), ("num_sinks", _i),
+        ("codes_w1", _vp), ("scales_w1", _vp), ("codes_w3", _vp), ("scales_w3", _vp),
+    ]
 
 
 class EpMoeBlock(C.Structure):

@@ -136,7 +136,8 @@ struct SavedPiece {
   uint64_t offset;  // in the saved-activations buffer
 };
 
-// fills `pieces` (at most 9) and returns how many; *total = bytes of the buffer
+// fills `pieces` (at most 11) and returns how many; *total = bytes of the buffer. At FULL_8BIT the last four - codes and scales of x1,
+// then of x3 - have no tensor in the block (dev == NULL): kernels write and read them.
 int saved_pieces(const B200MoeBlock *b, int level, SavedPiece *pieces, uint64_t *total) {
   const uint64_t T = (uint64_t)b->total_tokens, E = (uint64_t)b->num_experts, k = (uint64_t)b->top_k,
                  f = (uint64_t)b->ffn_dim;
@@ -162,12 +163,17 @@ int saved_pieces(const B200MoeBlock *b, int level, SavedPiece *pieces, uint64_t 
     add(b->x1, R * f * 2);
     add(b->x3, R * f * 2);
   }
+  if (level == B200_SAVED_ACTIVATION_LEVEL_FULL_8BIT)
+    for (int i = 0; i < 2; i++) {
+      add(nullptr, R * f);
+      add(nullptr, R * ((f + 31) / 32));
+    }
   *total = at;
   return n;
 }
 
 int check_level(const char *op, int level) {
-  B200_REQUIRE(level >= B200_SAVED_ACTIVATION_LEVEL_NONE && level <= B200_SAVED_ACTIVATION_LEVEL_FULL,
+  B200_REQUIRE(level >= B200_SAVED_ACTIVATION_LEVEL_NONE && level <= B200_SAVED_ACTIVATION_LEVEL_FULL_8BIT,
                "%s: unknown saved-activation level %d", op, level);
   B200_REQUIRE(level != B200_SAVED_ACTIVATION_LEVEL_NONE, "%s: nothing is saved at level NONE, no backward can follow", op);
   return 0;
@@ -177,14 +183,14 @@ int check_level(const char *op, int level) {
 
 extern "C" uint64_t b200_moe_saved_activations_bytes(int total_tokens, int num_experts, int top_k, int ffn_dim,
                                                      int level) {
-  if (level <= B200_SAVED_ACTIVATION_LEVEL_NONE || level > B200_SAVED_ACTIVATION_LEVEL_FULL) return 0;
+  if (level <= B200_SAVED_ACTIVATION_LEVEL_NONE || level > B200_SAVED_ACTIVATION_LEVEL_FULL_8BIT) return 0;
   B200MoeBlock b;
   memset(&b, 0, sizeof(b));
   b.total_tokens = total_tokens;
   b.num_experts = num_experts;
   b.top_k = top_k;
   b.ffn_dim = ffn_dim;
-  SavedPiece pieces[9];
+  SavedPiece pieces[11];
   uint64_t total = 0;
   saved_pieces(&b, level, pieces, &total);
   return total;
@@ -194,14 +200,30 @@ static int copy_saved(const char *op, const B200MoeBlock *b, int level, void *bu
                       void *stream) {
   if (check_block(op, b) || check_level(op, level)) return -1;
   B200_REQUIRE(buffer != nullptr, "%s: null buffer", op);
-  SavedPiece pieces[9];
+  SavedPiece pieces[11];
   uint64_t total = 0;
   const int n = saved_pieces(b, level, pieces, &total);
   B200_REQUIRE(buffer_bytes >= total, "%s: the buffer holds %llu bytes, level %d needs %llu", op,
                (unsigned long long)buffer_bytes, level, (unsigned long long)total);
   unsigned char *base = static_cast<unsigned char *>(buffer);
+  if (level == B200_SAVED_ACTIVATION_LEVEL_FULL_8BIT) {
+    // kernels reach the buffer: it has to be this device's memory or pinned host memory
+    cudaPointerAttributes at;
+    int dev = -1;
+    B200_CUDA(cudaGetDevice(&dev));
+    B200_CUDA(cudaPointerGetAttributes(&at, buffer));
+    B200_REQUIRE(at.devicePointer != nullptr && at.type != cudaMemoryTypeUnregistered &&
+                     (at.type != cudaMemoryTypeDevice || at.device == dev) && (reinterpret_cast<uintptr_t>(at.devicePointer) & 7u) == 0,
+                 "%s: at level FULL_8BIT the buffer must be memory of the current device or pinned host memory, 8-byte aligned", op);
+    unsigned char *held = static_cast<unsigned char *>(at.devicePointer);
+    const int R = b->total_tokens * b->top_k, f = b->ffn_dim;
+    void *c1 = held + pieces[n - 4].offset, *e1 = held + pieces[n - 3].offset, *c3 = held + pieces[n - 2].offset, *e3 = held + pieces[n - 1].offset;
+    if (save ? b200_swiglu_act8(B200_DT_BF16, R, f, b->x1, b->x3, nullptr, c1, e1, c3, e3, stream)
+             : b200_swiglu_recompute_act8(B200_DT_BF16, R, f, c1, e1, c3, e3, b->x1, b->x3, b->h, stream))
+      return -1;
+  }
   for (int i = 0; i < n; i++) {
-    if (pieces[i].bytes == 0) continue;
+    if (pieces[i].bytes == 0 || pieces[i].dev == nullptr) continue;
     // the buffer may be device memory or pinned host memory: the copy kind is taken from the pointers
     if (save)
       B200_CUDA(cudaMemcpyAsync(base + pieces[i].offset, pieces[i].dev, pieces[i].bytes, cudaMemcpyDefault, (cudaStream_t)stream));
@@ -223,6 +245,11 @@ extern "C" int b200_moe_block_restore_activations(const B200MoeBlock *block, int
 
 extern "C" int b200_moe_block_recompute_level(const B200MoeBlock *block, const void *Xn, int level, void *stream) {
   if (check_level("moe_block_recompute_level", level)) return -1;
+  if (level == B200_SAVED_ACTIVATION_LEVEL_FULL_8BIT) {  // the restore has written x1, x3 and h
+    if (check_block("moe_block_recompute_level", block)) return -1;
+    B200_REQUIRE(Xn, "moe_block_recompute_level: Xn missing");
+    return b200_prepare_experts(block->total_tokens, block->model_dim, block->top_k, Xn, block->token_mapping, block->zone, stream);
+  }
   // FULL: x1 and x3 were kept, only the zone and h are formed again; below FULL they come back from the zone too
   return b200_moe_block_recompute(block, Xn, level == B200_SAVED_ACTIVATION_LEVEL_FULL ? 0 : 1, stream);
 }

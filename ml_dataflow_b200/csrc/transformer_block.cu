@@ -42,18 +42,37 @@ int check_block(const char *op, const B200TransformerBlock *b) {
   return 0;
 }
 
+// none of the options set: what a NULL pointer means
+const B200TransformerBlockOptions NO_OPTIONS = {};
+
+int check_options(const char *op, const B200TransformerBlockOptions *o) {
+  B200_REQUIRE(!o->qk_norm || (o->q_raw && o->k_raw && o->qk_eps >= 0.0f), "%s: q/k norm needs q_raw, k_raw and qk_eps >= 0", op);
+  B200_REQUIRE(o->window >= 0 && o->num_sinks >= 0 && (o->window > 0 || o->num_sinks == 0), "%s: bad window or sinks (%d, %d)", op, o->window,
+               o->num_sinks);
+  const int held = (o->codes_w1 != nullptr) + (o->scales_w1 != nullptr) + (o->codes_w3 != nullptr) + (o->scales_w3 != nullptr);
+  B200_REQUIRE(held == 0 || held == 4, "%s: codes and scales of both SwiGLU inputs, or none of them", op);
+  return 0;
+}
+
 }  // namespace
 
-extern "C" int b200_transformer_block_fwd(const B200TransformerBlock *b, const void *x, void *out, void *stream) {
-  if (check_block("transformer_block_fwd", b)) return -1;
+static int block_fwd(const B200TransformerBlock *b, const B200TransformerBlockOptions *o, const void *x, void *out, void *stream) {
+  if (check_block("transformer_block_fwd", b) || check_options("transformer_block_fwd", o)) return -1;
   B200_REQUIRE(x && out && x != out, "transformer_block_fwd: x and out must be two buffers");
   const int T = b->total_tokens, d = b->model_dim, Dq = b->num_q_heads * b->head_dim, Dk = b->num_kv_heads * b->head_dim;
   if (b200_rms_norm(BF, T, d, b->eps, b->attn_norm, x, b->xn, b->rms1, stream)) return -1;
-  if (linear(T, d, Dq, b->xn, b->wq, nullptr, b->q, stream)) return -1;
-  if (linear(T, d, Dk, b->xn, b->wk, nullptr, b->k, stream)) return -1;
+  if (linear(T, d, Dq, b->xn, b->wq, nullptr, o->qk_norm ? o->q_raw : b->q, stream)) return -1;
+  if (linear(T, d, Dk, b->xn, b->wk, nullptr, o->qk_norm ? o->k_raw : b->k, stream)) return -1;
   if (linear(T, d, Dk, b->xn, b->wv, nullptr, b->v, stream)) return -1;
-  if (b200_rope(BF, T, Dq, b->head_dim, b->num_kv_heads, b->theta, b->positions, b->q, b->k, stream)) return -1;
-  if (b200_attention_fwd(BF, b->num_seqs, T, T, b->seq_offsets, b->seq_lens, b->max_seqlen, b->seq_offsets, b->seq_lens,
+  if (o->qk_norm ? b200_qk_norm_rope(BF, T, b->num_q_heads, b->num_kv_heads, b->head_dim, o->qk_eps, b->theta, b->positions, o->q_norm,
+                                     o->k_norm, o->q_raw, o->k_raw, b->q, b->k, stream)
+                 : b200_rope(BF, T, Dq, b->head_dim, b->num_kv_heads, b->theta, b->positions, b->q, b->k, stream))
+    return -1;
+  if (o->window > 0) {
+    if (b200_attention_window_fwd(BF, b->num_seqs, T, T, b->seq_offsets, b->seq_lens, b->seq_offsets, b->seq_lens, b->num_q_heads,
+                                  b->num_kv_heads, b->head_dim, b->q, b->k, b->v, b->attn, b->lse, o->window, o->num_sinks, stream))
+      return -1;
+  } else if (b200_attention_fwd(BF, b->num_seqs, T, T, b->seq_offsets, b->seq_lens, b->max_seqlen, b->seq_offsets, b->seq_lens,
                          b->max_seqlen, b->num_q_heads, b->num_kv_heads, b->head_dim, b->q, b->k, b->v, b->attn, b->lse, 1,
                          b->attn_workspace_bytes, b->attn_workspace, stream))
     return -1;
@@ -61,12 +80,15 @@ extern "C" int b200_transformer_block_fwd(const B200TransformerBlock *b, const v
   if (b200_rms_norm(BF, T, d, b->eps, b->ffn_norm, b->x_mid, b->xn2, b->rms2, stream)) return -1;
   // the MoE combine accumulates onto the residual
   B200_CUDA(cudaMemcpyAsync(out, b->x_mid, (size_t)T * d * 2, cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
-  return b200_moe_block_fwd(&b->moe, b->xn2, out, stream);
+  if (b200_moe_block_fwd(&b->moe, b->xn2, out, stream)) return -1;
+  if (o->codes_w1 == nullptr) return 0;
+  return b200_swiglu_act8(BF, T * b->moe.top_k, b->moe.ffn_dim, b->moe.x1, b->moe.x3, nullptr, o->codes_w1, o->scales_w1, o->codes_w3,
+                          o->scales_w3, stream);
 }
 
-extern "C" int b200_transformer_block_bwd(const B200TransformerBlock *b, const void *x, void *dx, const B200TransformerBlockGrads *g,
-                                          const B200TransformerBlockScratch *s, void *stream) {
-  if (check_block("transformer_block_bwd", b)) return -1;
+static int block_bwd(const B200TransformerBlock *b, const B200TransformerBlockOptions *o, const void *x, void *dx,
+                     const B200TransformerBlockGrads *g, const B200TransformerBlockScratch *s, void *stream) {
+  if (check_block("transformer_block_bwd", b) || check_options("transformer_block_bwd", o)) return -1;
   B200_REQUIRE(x && dx && g && s, "transformer_block_bwd: null argument");
   B200_REQUIRE(g->attn_norm && g->wq && g->wk && g->wv && g->wo && g->ffn_norm && g->router && g->W1 && g->W3 && g->W2,
                "transformer_block_bwd: null gradient buffer");
@@ -76,6 +98,12 @@ extern "C" int b200_transformer_block_bwd(const B200TransformerBlock *b, const v
   if (!acc) {  // the norm-weight kernels only accumulate: start them from zero
     B200_CUDA(cudaMemsetAsync(g->attn_norm, 0, (size_t)d * 2, (cudaStream_t)stream));
     B200_CUDA(cudaMemsetAsync(g->ffn_norm, 0, (size_t)d * 2, (cudaStream_t)stream));
+  }
+  if (o->codes_w1 != nullptr) {  // x1, x3, h and the zone may have served other blocks since
+    if (b200_swiglu_recompute_act8(BF, T * b->moe.top_k, b->moe.ffn_dim, o->codes_w1, o->scales_w1, o->codes_w3, o->scales_w3, b->moe.x1,
+                                   b->moe.x3, b->moe.h, stream))
+      return -1;
+    if (b200_prepare_experts(T, d, b->moe.top_k, b->xn2, b->moe.token_mapping, b->moe.zone, stream)) return -1;
   }
   // MoE part: dx is the gradient at the block's output and also flows through the residual unchanged
   if ((acc ? b200_moe_block_bwd : b200_moe_block_bwd_overwrite)(&b->moe, b->xn2, dx, s->dxn, g->router, g->W1, g->W3, g->W2,
@@ -88,11 +116,20 @@ extern "C" int b200_transformer_block_bwd(const B200TransformerBlock *b, const v
   // attention part: x_mid = x + attn . wo^T
   if (linear_dw(T, Dq, d, dx, b->attn, g->wo, acc, stream)) return -1;
   if (linear_dx(T, Dq, d, dx, b->wo, s->dattn, false, stream)) return -1;
-  if (b200_attention_bwd(BF, b->num_seqs, T, T, b->seq_offsets, b->seq_lens, b->max_seqlen, b->seq_offsets, b->seq_lens,
+  if (o->window > 0) {
+    if (b200_attention_window_bwd(BF, b->num_seqs, T, T, b->seq_offsets, b->seq_lens, b->seq_offsets, b->seq_lens, b->num_q_heads,
+                                  b->num_kv_heads, b->head_dim, b->q, b->k, b->v, b->attn, b->lse, s->dattn, s->dq, s->dk, s->dv, o->window,
+                                  o->num_sinks, b->attn_workspace_bytes, b->attn_workspace, stream))
+      return -1;
+  } else if (b200_attention_bwd(BF, b->num_seqs, T, T, b->seq_offsets, b->seq_lens, b->max_seqlen, b->seq_offsets, b->seq_lens,
                          b->max_seqlen, b->num_q_heads, b->num_kv_heads, b->head_dim, b->q, b->k, b->v, b->attn, b->lse,
                          s->dattn, s->dq, s->dk, s->dv, 1, b->attn_workspace_bytes, b->attn_workspace, stream))
     return -1;
-  if (b200_rope_bwd_x(BF, T, Dq, b->head_dim, b->num_kv_heads, b->theta, b->positions, s->dq, s->dk, stream)) return -1;
+  if (o->qk_norm ? b200_qk_norm_rope_bwd(BF, BF, T, b->num_q_heads, b->num_kv_heads, b->head_dim, o->qk_eps, b->theta, b->positions, o->q_norm,
+                                         o->k_norm, o->q_raw, o->k_raw, s->dq, s->dk, s->dq, s->dk, o->d_q_norm, o->d_k_norm, acc,
+                                         o->qk_workspace_bytes, o->qk_workspace, stream)
+                 : b200_rope_bwd_x(BF, T, Dq, b->head_dim, b->num_kv_heads, b->theta, b->positions, s->dq, s->dk, stream))
+    return -1;
   if (b200_rms_norm_recompute(BF, T, d, b->attn_norm, b->rms1, x, b->xn, stream)) return -1;
   if (linear_dw(T, d, Dq, s->dq, b->xn, g->wq, acc, stream)) return -1;
   if (linear_dw(T, d, Dk, s->dk, b->xn, g->wk, acc, stream)) return -1;
@@ -104,4 +141,24 @@ extern "C" int b200_transformer_block_bwd(const B200TransformerBlock *b, const v
                           stream))
     return -1;
   return b200_rms_norm_bwd_x(BF, BF, T, d, b->eps, b->rms1, b->attn_norm, x, s->dxn, dx, nullptr, stream);
+}
+
+extern "C" int b200_transformer_block_fwd(const B200TransformerBlock *b, const void *x, void *out, void *stream) {
+  return block_fwd(b, &NO_OPTIONS, x, out, stream);
+}
+
+extern "C" int b200_transformer_block_bwd(const B200TransformerBlock *b, const void *x, void *dx, const B200TransformerBlockGrads *g,
+                                          const B200TransformerBlockScratch *s, void *stream) {
+  return block_bwd(b, &NO_OPTIONS, x, dx, g, s, stream);
+}
+
+extern "C" int b200_transformer_block_fwd_options(const B200TransformerBlock *b, const B200TransformerBlockOptions *options, const void *x,
+                                                  void *out, void *stream) {
+  return block_fwd(b, options ? options : &NO_OPTIONS, x, out, stream);
+}
+
+extern "C" int b200_transformer_block_bwd_options(const B200TransformerBlock *b, const B200TransformerBlockOptions *options, const void *x,
+                                                  void *dx, const B200TransformerBlockGrads *g, const B200TransformerBlockScratch *s,
+                                                  void *stream) {
+  return block_bwd(b, options ? options : &NO_OPTIONS, x, dx, g, s, stream);
 }

@@ -8,7 +8,9 @@ dataflow_transformer.c: embedding 2283-2342, block forward 2343-2584 and 2588-29
 the buffers. Like moe_layer.py it is the test and benchmark harness of the ops, not a second implementation: the
 parity test (tests/test_gpu_decoder.py) compares a small model against float32 torch autograd with the routing held
 fixed. No activation offload or recompute: every layer keeps what its backward reads (the memory planner of the
-reference is out of scope).
+reference is out of scope). What a configuration may add: an RMSNorm of every query and key head before the rotation
+(qk_norm), attention with a sliding window and sink tokens (window, num_sinks), and the SwiGLU's inputs held in 8 bits
+with one MoE working set for all layers (act8).
 
 Weight layouts are the reference's (models/init_model.py:279-306): projections [out_features][in_features], experts
 W1 / W3 [E][f][d], W2 [E][d][f], embedding and head [vocab][d], all bf16.
@@ -35,6 +37,11 @@ class DecoderConfig:
     vocab: int
     eps: float = 1e-5
     theta: int = 500000
+    qk_norm: bool = False         # RMSNorm of every query and key head, with weights unless qk_norm_weights is False
+    qk_norm_weights: bool = True
+    window: int = 0               # keys a query sees, its own included; 0: all before it
+    num_sinks: int = 0            # first keys of a sequence that stay visible
+    act8: bool = False            # x1 and x3 of the MoE layers in 8 bits between forward and backward
 
 
 def _randn(gen, shape, std, dev):
@@ -64,6 +71,8 @@ class Decoder:
                 wv=_randn(gen, (Dk, c.d), std, dev), wo=_randn(gen, (c.d, Dq), std, dev), ffn_norm=ones(c.d),
                 router=_randn(gen, (c.n_experts, c.d), std, dev), W1=_randn(gen, (c.n_experts, c.ffn, c.d), std, dev),
                 W3=_randn(gen, (c.n_experts, c.ffn, c.d), std, dev), W2=_randn(gen, (c.n_experts, c.d, c.ffn), std, dev)))
+            if c.qk_norm and c.qk_norm_weights:
+                self.layers[-1].update(q_norm=ones(c.head_dim), k_norm=ones(c.head_dim))
         self.embed = _randn(gen, (c.vocab, c.d), std, dev)
         self.final_norm = ones(c.d)
         self.head = _randn(gen, (c.vocab, c.d), std, dev)
@@ -78,8 +87,13 @@ class Decoder:
         # stream after the attention residual, the normed input of the MoE part; the MoE layer keeps its own set
         self.saved = [dict(x=buf((T, c.d)), rms1=buf((T,), f32), q=buf((T, Dq)), k=buf((T, Dk)), v=buf((T, Dk)),
                            attn=buf((T, Dq)), lse=buf((c.n_heads, T), f32), x_mid=buf((T, c.d)), rms2=buf((T,), f32),
-                           xn2=buf((T, c.d)), moe=MoELayer(T, c.d, c.n_experts, c.top_k, c.ffn, device=dev))
+                           xn2=buf((T, c.d)))
                       for _ in range(c.n_layers)]
+        for li, S in enumerate(self.saved):
+            S["moe"] = MoELayer(T, c.d, c.n_experts, c.top_k, c.ffn, device=dev, held8=c.act8,
+                                share=self.saved[0]["moe"] if c.act8 and li > 0 else None)
+            if c.qk_norm:  # the projections before the norm
+                S.update(q_raw=buf((T, Dq)), k_raw=buf((T, Dk)))
         self.x_final = buf((T, c.d))
         self.rms_f = buf((T,), f32)
         self.xn = buf((T, c.d))
@@ -88,8 +102,13 @@ class Decoder:
         # backward scratch shared by the layers
         self.dx, self.dxn, self.dattn = buf((T, c.d)), buf((T, c.d)), buf((T, Dq))
         self.dq, self.dk, self.dv = buf((T, Dq)), buf((T, Dk)), buf((T, Dk))
-        self.attn_ws = torch.empty(max(256, ops.attention_workspace_bytes(True, c.n_heads, c.n_kv_heads, c.head_dim, T, max_seqlen, max_seqlen)), dtype=torch.uint8,
-                                   device=dev)
+        # a batch has at most one sequence per token
+        attn_bytes = (ops.attention_window_workspace_bytes(T, c.n_heads, c.n_kv_heads, c.head_dim, T, c.num_sinks) if c.window else
+                      ops.attention_workspace_bytes(True, c.n_heads, c.n_kv_heads, c.head_dim, T, max_seqlen, max_seqlen))
+        self.attn_ws = torch.empty(max(256, attn_bytes), dtype=torch.uint8, device=dev)
+        self.qk_ws = None
+        if c.qk_norm and c.qk_norm_weights:
+            self.qk_ws = torch.empty(ops.qk_norm_rope_bwd_workspace_bytes(T, c.n_heads, c.n_kv_heads, c.head_dim), dtype=torch.uint8, device=dev)
         self.norm_ws = torch.empty(ops.rms_norm_bwd_w_workspace_bytes(T, c.d), dtype=torch.uint8, device=dev)
 
     def _c_structs(self):
@@ -103,7 +122,7 @@ class Decoder:
         n = len(self.seq_lens)
         self._seq_arrays = ((C.c_int * n)(*self.seq_offs), (C.c_int * n)(*self.seq_lens))  # kept alive with the structs
         offs, lens = (C.cast(a, C.c_void_p) for a in self._seq_arrays)
-        blocks, grads = [], []
+        blocks, grads, options = [], [], []
         for L, S, G in zip(self.layers, self.saved, self.grads):
             moe = S["moe"].block(L["router"], L["W1"], L["W3"], L["W2"])
             blocks.append(_lib.TransformerBlock(
@@ -113,9 +132,28 @@ class Decoder:
                 p(S["xn2"]), p(self.xn), p(self.attn_ws), self.attn_ws.numel(), moe))
             # one batch per step here: the blocks write their weight gradients, so nothing has to be zeroed first
             grads.append(_lib.TransformerBlockGrads(*[p(G[k]) for k in self.PARAMS], 1))
+            options.append(self._options(L, S, G))
         scratch = _lib.TransformerBlockScratch(p(self.dxn), p(self.dattn), p(self.dq), p(self.dk), p(self.dv), p(self.norm_ws),
                                                self.norm_ws.numel())
-        return blocks, grads, scratch
+        return blocks, grads, scratch, options
+
+    def _options(self, L, S, G):
+        """A layer's _lib.TransformerBlockOptions, or None where the configuration adds nothing."""
+        from . import _lib
+
+        c = self.cfg
+        if not (c.qk_norm or c.window or c.act8):
+            return None
+        p = lambda t: None if t is None else t.data_ptr()
+        o = _lib.TransformerBlockOptions(window=c.window, num_sinks=c.num_sinks)
+        if c.qk_norm:
+            o.qk_norm, o.qk_eps, o.q_raw, o.k_raw = 1, c.eps, p(S["q_raw"]), p(S["k_raw"])
+        if self.qk_ws is not None:
+            o.q_norm, o.k_norm, o.d_q_norm, o.d_k_norm = p(L["q_norm"]), p(L["k_norm"]), p(G["q_norm"]), p(G["k_norm"])
+            o.qk_workspace, o.qk_workspace_bytes = p(self.qk_ws), self.qk_ws.numel()
+        if c.act8:
+            o.codes_w1, o.scales_w1, o.codes_w3, o.scales_w3 = (p(t) for t in S["moe"].held8)
+        return o
 
     # ------------------------------------------------------------------------------------------------ helpers
     @staticmethod
@@ -160,20 +198,28 @@ class Decoder:
         x = self.saved[0]["x"]
         ops.embedding_table(nu, c.d, sid, smap, starts, self.embed, x)
         if self.c_blocks:
-            self._blocks, self._block_grads, self._block_scratch = self._c_structs()
+            self._blocks, self._block_grads, self._block_scratch, self._block_options = self._c_structs()
         for li, (L, S) in enumerate(zip(self.layers, self.saved)):
             x = S["x"]
             if self.c_blocks:
                 out = self.saved[li + 1]["x"] if li + 1 < c.n_layers else self.x_final
-                ops.transformer_block_fwd(self._blocks[li], x, out)
+                ops.transformer_block_fwd(self._blocks[li], x, out, self._block_options[li])
                 continue
             ops.rms_norm(T, c.d, c.eps, L["attn_norm"], x, self.xn, S["rms1"])
-            self._linear(self.xn, L["wq"], S["q"])
-            self._linear(self.xn, L["wk"], S["k"])
+            self._linear(self.xn, L["wq"], S["q_raw" if c.qk_norm else "q"])
+            self._linear(self.xn, L["wk"], S["k_raw" if c.qk_norm else "k"])
             self._linear(self.xn, L["wv"], S["v"])
-            ops.rope(T, self.Dq, c.head_dim, c.n_kv_heads, c.theta, self.positions, S["q"], S["k"])
-            ops.attention_fwd(self.seq_offs, self.seq_lens, self.seq_offs, self.seq_lens, c.n_heads, c.n_kv_heads, c.head_dim,
-                              S["q"], S["k"], S["v"], S["attn"], S["lse"], True, self.attn_ws)
+            if c.qk_norm:
+                ops.qk_norm_rope(T, c.n_heads, c.n_kv_heads, c.head_dim, c.eps, c.theta, self.positions, L.get("q_norm"), L.get("k_norm"),
+                                 S["q_raw"], S["k_raw"], S["q"], S["k"])
+            else:
+                ops.rope(T, self.Dq, c.head_dim, c.n_kv_heads, c.theta, self.positions, S["q"], S["k"])
+            attn = (self.seq_offs, self.seq_lens, self.seq_offs, self.seq_lens, c.n_heads, c.n_kv_heads, c.head_dim, S["q"], S["k"],
+                    S["v"], S["attn"], S["lse"])
+            if c.window:
+                ops.attention_window_fwd(*attn, c.window, c.num_sinks)
+            else:
+                ops.attention_fwd(*attn, True, self.attn_ws)
             self._linear(S["attn"], L["wo"], S["x_mid"], residual=x)
             ops.rms_norm(T, c.d, c.eps, L["ffn_norm"], S["x_mid"], S["xn2"], S["rms2"])
             out = self.saved[li + 1]["x"] if li + 1 < c.n_layers else self.x_final
@@ -202,7 +248,7 @@ class Decoder:
             L, S, G = self.layers[li], self.saved[li], self.grads[li]
             x, moe = S["x"], S["moe"]
             if self.c_blocks:
-                ops.transformer_block_bwd(self._blocks[li], x, self.dx, self._block_grads[li], self._block_scratch)
+                ops.transformer_block_bwd(self._blocks[li], x, self.dx, self._block_grads[li], self._block_scratch, self._block_options[li])
                 continue
             # MoE part: dx is the gradient at the block's output; it also flows through the residual unchanged
             moe.backward(S["xn2"], L["router"], L["W1"], L["W3"], L["W2"], self.dx, self.dxn, G["router"], G["W1"], G["W3"],
@@ -212,10 +258,18 @@ class Decoder:
             # attention part: x_mid = x + attn . wo^T
             self._linear_dw(self.dx, S["attn"], G["wo"])
             self._linear_dx(self.dx, L["wo"], self.dattn, accumulate=False)
-            ops.attention_bwd(self.seq_offs, self.seq_lens, self.seq_offs, self.seq_lens, c.n_heads, c.n_kv_heads, c.head_dim,
-                              S["q"], S["k"], S["v"], S["attn"], S["lse"], self.dattn, self.dq, self.dk, self.dv, True,
-                              self.attn_ws)
-            ops.rope_bwd_x(T, self.Dq, c.head_dim, c.n_kv_heads, c.theta, self.positions, self.dq, self.dk)
+            attn = (self.seq_offs, self.seq_lens, self.seq_offs, self.seq_lens, c.n_heads, c.n_kv_heads, c.head_dim, S["q"], S["k"],
+                    S["v"], S["attn"], S["lse"], self.dattn, self.dq, self.dk, self.dv)
+            if c.window:
+                ops.attention_window_bwd(*attn, c.window, c.num_sinks, self.attn_ws)
+            else:
+                ops.attention_bwd(*attn, True, self.attn_ws)
+            if c.qk_norm:
+                ops.qk_norm_rope_bwd(T, c.n_heads, c.n_kv_heads, c.head_dim, c.eps, c.theta, self.positions, L.get("q_norm"),
+                                     L.get("k_norm"), S["q_raw"], S["k_raw"], self.dq, self.dk, self.dq, self.dk, G.get("q_norm"),
+                                     G.get("k_norm"), True, self.qk_ws)
+            else:
+                ops.rope_bwd_x(T, self.Dq, c.head_dim, c.n_kv_heads, c.theta, self.positions, self.dq, self.dk)
             ops.rms_norm_recompute(T, c.d, L["attn_norm"], S["rms1"], x, self.xn)
             self._linear_dw(self.dq, self.xn, G["wq"])
             self._linear_dw(self.dk, self.xn, G["wk"])
@@ -231,7 +285,7 @@ class Decoder:
     # ------------------------------------------------------------------------------------------------ optimizer
     def _all_params(self):
         for L, G in zip(self.layers, self.grads):
-            for name in self.PARAMS:
+            for name in L:
                 yield L[name], G[name]
         yield self.embed, self.g_embed
         yield self.final_norm, self.g_final_norm

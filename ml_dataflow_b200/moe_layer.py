@@ -13,6 +13,9 @@ Two drivers over the same buffers:
 
 Shapes: Xn [T, d] bf16, Wr [E, d], W1/W3 [E, f, d], W2 [E, d, f] bf16 (the reference's weight
 layouts, models/init_model.py:279-306). All buffers are allocated once in the constructor.
+
+With held8 the layer keeps x1 and x3 in 8 bits between forward and backward (ops.swiglu_act8), and its working set - everything the
+backward can form again or overwrites - may be that of another layer (share).
 """
 import torch
 
@@ -20,7 +23,7 @@ from . import ops
 
 
 class MoELayer:
-    def __init__(self, T, d, E, k, f, device="cuda"):
+    def __init__(self, T, d, E, k, f, device="cuda", held8=False, share=None):
         self.T, self.d, self.E, self.k, self.f = T, d, E, k, f
         R = T * k
         self.R = R
@@ -42,6 +45,19 @@ class MoELayer:
         self.token_mapping = buf((T, k), i32)
         self.map_ws = torch.empty(ops.build_expert_mapping_workspace_bytes(T, E, k), dtype=torch.uint8, device=dev)
         self.mm_ws = torch.empty(16 << 20, dtype=torch.uint8, device=dev)  # split-K scratch of the router GEMMs
+        self.held8 = None
+        if held8:
+            u8, blocks = torch.uint8, (f + 31) // 32
+            self.held8 = (buf((R, f), u8), buf((R, blocks), u8), buf((R, f), u8), buf((R, blocks), u8))  # codes, scales of x1, of x3
+        self.dh = None  # [R, f], allocated on first use by the reference-order backward only
+        self.profile = None  # list of (name, event) when a caller wants per-op timing (see mark())
+        self.keep_pre_gate = False  # tests set this to look at dX_routed before the gate Jacobian is applied
+        self.dX_routed_pre = None
+        if share is not None:
+            assert held8 and share.held8 is not None and (share.T, share.d, share.E, share.k, share.f) == (T, d, E, k, f)
+            for name in ("zone", "x1", "x3", "h", "Y", "dYz", "row_w", "dP", "dx1", "dx3", "hs", "dZ", "dX_routed"):
+                setattr(self, name, getattr(share, name))
+            return
         self.zone = buf((R, d), bf)
         self.x1 = buf((R, f), bf)
         self.x3 = buf((R, f), bf)
@@ -54,12 +70,8 @@ class MoELayer:
         self.dx1 = buf((R, f), bf)
         self.dx3 = buf((R, f), bf)
         self.hs = buf((R, f), bf)
-        self.dh = None  # [R, f], allocated on first use by the reference-order backward only
         self.dZ = buf((R, d), bf)
         self.dX_routed = buf((T, E), bf)
-        self.profile = None  # list of (name, event) when a caller wants per-op timing (see mark())
-        self.keep_pre_gate = False  # tests set this to look at dX_routed before the gate Jacobian is applied
-        self.dX_routed_pre = None
 
     def mark(self, name):
         """Records a CUDA event labelled `name` on the current stream when profiling is switched on."""
@@ -111,12 +123,19 @@ class MoELayer:
                             self.x1, self.x3, self.h, self.Y)
         self.mark("merge_experts")
         ops.merge_experts(T, d, k, self.Y, self.token_mapping, self.weights, out)
+        if self.held8 is not None:
+            self.mark("hold8")
+            ops.swiglu_act8(R, f, self.x1, self.x3, None, *self.held8)
         self.mark("fwd_end")
         return out
 
     def backward(self, Xn, Wr, W1, W3, W2, dOut, dXn, dWr, dW1, dW3, dW2):
         """dXn is overwritten; dWr, dW1, dW3, dW2 (bf16) are accumulated into, like the reference's beta=1 GEMMs."""
         T, d, E, k, f, R = self.T, self.d, self.E, self.k, self.f, self.R
+        if self.held8 is not None:  # another layer may have used the working set since
+            self.mark("restore8")
+            ops.swiglu_recompute_act8(R, f, *self.held8, self.x1, self.x3, self.h)
+            ops.prepare_experts(T, d, k, Xn, self.token_mapping, self.zone)
         # dY rows = w * dOut in expert order (what the reference's router_bwd_x leaves in the zone)
         self.mark("prepare_experts_weighted")
         ops.prepare_experts_weighted(T, d, k, dOut, self.token_mapping, self.weights, self.dYz)
@@ -163,6 +182,8 @@ class MoELayer:
             ops.matmul(1, 0, d, f, n, 1.0, 0.0, W2[e], h, None, self.Y[base:base + n])
             base += n
         ops.merge_experts(T, d, k, self.Y, self.token_mapping, self.weights, out)
+        if self.held8 is not None:
+            ops.swiglu_act8(self.R, f, self.x1, self.x3, None, *self.held8)
         return out
 
     def backward_reference_order(self, Xn, Wr, W1, W3, W2, dOut, dXn, dWr, dW1, dW3, dW2):
@@ -176,7 +197,11 @@ class MoELayer:
                 continue
             sl = slice(base, base + n)
             x1, x3, tmp = self.x1[sl], self.x3[sl], self.hs[sl]
-            ops.swiglu(n, f, x1, x3, tmp)  # recompute h, then the expert output
+            held = None if self.held8 is None else [t[sl] for t in self.held8]
+            if held is None:
+                ops.swiglu(n, f, x1, x3, tmp)  # recompute h, then the expert output
+            else:
+                ops.swiglu_recompute_act8(n, f, *held, out=tmp)
             ops.matmul(1, 0, d, f, n, 1.0, 0.0, W2[e], tmp, None, zone[sl])
             ops.router_bwd_x(n, d, E, k, e, self.cumsum, self.expert_mapping, self.chosen, self.weights, zone[sl],
                              dOut, self.dX_routed, zone[sl])
@@ -185,7 +210,10 @@ class MoELayer:
                 self.dh = torch.empty_like(self.h)
             dh = self.dh[sl]
             ops.matmul(0, 0, f, d, n, 1.0, 0.0, W2[e], zone[sl], None, dh)  # dh = dY W2
-            ops.swiglu_bwd_x(n, f, x1, x3, dh, self.dx1[sl], self.dx3[sl])
+            if held is None:
+                ops.swiglu_bwd_x(n, f, x1, x3, dh, self.dx1[sl], self.dx3[sl])
+            else:
+                ops.swiglu_bwd_x_act8(n, f, *held, dh, self.dx1[sl], self.dx3[sl])
             ops.matmul(0, 0, d, f, n, 1.0, 0.0, W1[e], self.dx1[sl], None, zone[sl])
             ops.matmul(0, 0, d, f, n, 1.0, 1.0, W3[e], self.dx3[sl], zone[sl], zone[sl])
             base += n

@@ -385,13 +385,21 @@ def _int_array(values):
     return (C.c_int * len(values))(*[int(v) for v in values])
 
 
-def transformer_block_fwd(block, x, out):
-    """block: _lib.TransformerBlock; out = block(x)."""
+def transformer_block_fwd(block, x, out, options=None):
+    """block: _lib.TransformerBlock; out = block(x). options: _lib.TransformerBlockOptions (q/k norm, window, 8-bit activations)."""
+    if options is not None:
+        _check(_lib.load().b200_transformer_block_fwd_options(C.byref(block), C.byref(options), _p(x), _p(out), _stream()),
+               "transformer_block_fwd_options", 20 + (options.codes_w1 is not None))
+        return
     _check(_lib.load().b200_transformer_block_fwd(C.byref(block), _p(x), _p(out), _stream()), "transformer_block_fwd", 20)
 
 
-def transformer_block_bwd(block, x, dx, grads, scratch):
+def transformer_block_bwd(block, x, dx, grads, scratch, options=None):
     """dx: the gradient at the block's output on entry, at its input on return; grads are accumulated into."""
+    if options is not None:
+        _check(_lib.load().b200_transformer_block_bwd_options(C.byref(block), C.byref(options), _p(x), _p(dx), C.byref(grads),
+                                                              C.byref(scratch), _stream()), "transformer_block_bwd_options", 45)
+        return
     _check(_lib.load().b200_transformer_block_bwd(C.byref(block), _p(x), _p(dx), C.byref(grads), C.byref(scratch), _stream()),
            "transformer_block_bwd", 45)
 

@@ -17,7 +17,7 @@ def _ints(*v):
 
 BF, F32 = 5, 3
 P = ctypes.c_void_p(1 << 20)  # an aligned address that is never read: the refusal comes first
-ODD = ctypes.c_void_p((1 << 20) + 8)
+ODD = ctypes.c_void_p((1 << 20) + 4)
 
 
 def test_qk_norm_rope_refusals():
@@ -113,3 +113,35 @@ def test_the_front_end_refuses_tensors_that_are_not_on_the_current_device():
         ops.attention_window_fwd([0], [4, 1], [0], [4], 1, 1, 64, x, x, x, x, torch.zeros(1, 4), 4, 0)
     with pytest.raises(ValueError):
         ops.attention_window_fwd([0], [4], [0], [4], 1, 1, 64, x, x, x, x, torch.zeros(1, 4), 1 << 32, 0)
+
+
+def test_block_options_mirror_and_refusals():
+    """The structure as ctypes sees it; inconsistent options are refused before any CUDA call; unknown levels have no size."""
+    import test_abi_exports as abi
+
+    from ml_dataflow_b200 import _lib
+
+    assert abi._struct_fields("B200TransformerBlockOptions") == [f[0] for f in _lib.TransformerBlockOptions._fields_]
+    lib = _lib.load()
+    assert lib.b200_transformer_block_fwd_options(None, None, None, None, None) == -1
+    blk = _lib.TransformerBlock()  # all zeros: bad dimensions
+    assert lib.b200_transformer_block_bwd_options(ctypes.byref(blk), None, None, None, None, None, None) == -1
+    p = P.value
+    m = _lib.MoeBlock(8, 64, 4, 2, 32, *[p] * 4, 2048, 2048, 2048, *[p] * 5, None, *[p] * 8, 1 << 20, p, 1 << 20, *[p] * 7)
+    one = _ints(0)
+    seqs = ctypes.cast(one, ctypes.c_void_p)
+    blk = _lib.TransformerBlock(8, 64, 2, 1, 32, 10000, 1e-5, 1, 8, seqs, seqs, *[p] * 7, *[p] * 11, 1 << 20, m)
+    for bad in (dict(qk_norm=1, q_raw=p), dict(qk_norm=1, q_raw=p, k_raw=p, qk_eps=-1.0), dict(window=-1), dict(num_sinks=3), dict(window=4, num_sinks=-1),
+                dict(codes_w1=p), dict(codes_w1=p, scales_w1=p, codes_w3=p)):
+        o = _lib.TransformerBlockOptions(**bad)
+        assert lib.b200_transformer_block_fwd_options(ctypes.byref(blk), ctypes.byref(o), P, ctypes.c_void_p(p + 4096), None) == -1, bad
+
+
+def test_saved_set_in_8_bits_is_the_stated_layout():
+    lib = _lib()
+    for T, E, k, f in ((300, 16, 4, 192), (8192, 64, 8, 1408), (1, 2, 1, 8), (5, 4, 2, 40)):
+        R, at = T * k, 0
+        for s in [4 * T * E, 2 * R, 4 * R, 4 * (E + 1), 4 * E, 4 * R, 4 * R, R * f, R * ((f + 31) // 32), R * f, R * ((f + 31) // 32)]:
+            at = (at + 255) // 256 * 256 + s
+        assert lib.b200_moe_saved_activations_bytes(T, E, k, f, 4) == at
+        assert lib.b200_moe_saved_activations_bytes(T, E, k, f, 5) == 0
