@@ -250,6 +250,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](uint64_t *b) { return ptx::smem_u32(b); };
   auto wait = [&](uint64_t *b, uint32_t par, int code) { return ptx::mbar_wait<false>(bar(b), par & 1u, abort_flag, p.status, code); };
+  // every thread arrives for itself (one arrival per warp measured the same)
+  auto arrive = [&](uint64_t *b) { ptx::mbar_arrive(bar(b)); };
 
   if (tid == 0) {
     for (int g = 0; g < 2; g++) {
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         uint32_t s[TILE];
         load_columns<TILE>(s_addr, s);
         ptx::tc_fence_before();
-        ptx::mbar_arrive(bar(&st->s_read[g]));
+        arrive(&st->s_read[g]);
         if (!all_seen(kb * TILE, tile_pos, last_pos, p.window, p.sinks)) {
           const int base = kb * TILE, hi = min(pos, u.sp.Tk - 1) - base, lo = pos - p.window + 1 - base, sk = p.sinks - base;
 #pragma unroll
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         store_packed<8>(p_addr + SLAB, trow, 0, pk + 32);
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
-        ptx::mbar_arrive(bar(&st->p_ready[g]));
+        arrive(&st->p_ready[g]);
         first = false;
         t++;
       }
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
       uint32_t r[HD];
       load_columns<HD>(o_addr, r);
       ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(&st->o_empty[g]));
+      arrive(&st->o_empty[g]);
       if (row < u.sp.Tq) {
         const float inv = 1.0f / l;
         __nv_bfloat16 *o = p.O + ((int64_t)(u.sp.q_off + row) * p.q_heads + x.h) * HD;
@@ -631,6 +633,8 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](uint64_t *b) { return ptx::smem_u32(b); };
   auto wait = [&](uint64_t *b, uint32_t par, int code) { return ptx::mbar_wait<false>(bar(b), par & 1u, abort_flag, p.status, code); };
+  // every thread arrives for itself (one arrival per warp measured the same)
+  auto arrive = [&](uint64_t *b) { ptx::mbar_arrive(bar(b)); };
 
   if (tid == 0) {
     ptx::mbar_init(bar(&st->q_full), 1);
@@ -821,7 +825,7 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
           if (r < rows) p.delta[(int64_t)u.x.h * p.total_q + row0 + r] = d;
         }
       }
-      ptx::mbar_arrive(bar(&st->stat_full[set]));
+      arrive(&st->stat_full[set]);
       return true;
     };
     uint32_t units = 0;
@@ -841,7 +845,7 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
         load_columns<32>(lane_addr + COL_DQ + (units & 1) * TILE + q * 32, r);
         if (q == HD / 32 - 1) {
           ptx::tc_fence_before();
-          ptx::mbar_arrive(bar(&st->acc_empty[units & 1]));
+          arrive(&st->acc_empty[units & 1]);
         }
         if (row < u.sp.Tq) {
           store16(o + q * 32, r, p.scale);
@@ -866,7 +870,7 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
       const float lse2 = row < u.sp.Tq ? p.lse[(int64_t)u.x.h * p.total_q + u.sp.q_off + row] * LOG2E : 0.0f;
       if (!wait(&st->stat_full[units & 1], units / 2, ST_BQ_STAT)) goto teardown;
       const float delta = st->delta[units & 1][trow];
-      ptx::mbar_arrive(bar(&st->stat_empty[units & 1]));
+      arrive(&st->stat_empty[units & 1]);
       for (int i = 0; i < u.n; i++, t++) {
         const int kb = u.block(i);
         uint32_t s[32], d[32];
@@ -874,13 +878,13 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
         ptx::tc_fence_after();
         load_columns<32>(lane_addr + COL_S, s);
         ptx::tc_fence_before();
-        ptx::mbar_arrive(bar(&st->s_read));
+        arrive(&st->s_read);
         probabilities<32>(s, c, -lse2);
         if (!wait(&st->dp_full, t, ST_BQ_DP)) goto teardown;
         ptx::tc_fence_after();
         load_columns<32>(lane_addr + COL_DP, d);
         ptx::tc_fence_before();
-        ptx::mbar_arrive(bar(&st->dp_read));
+        arrive(&st->dp_read);
         score_gradients<32>(d, s, delta);
         if (!all_seen(kb * TILE, pos0, last_pos, p.window, p.sinks)) {
           const int base = kb * TILE + cols * 32;
@@ -893,7 +897,7 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
         store_chunks<4>(ds_addr, trow, (cols & 1) * 4, d);
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
-        ptx::mbar_arrive(bar(&st->ds_ready));
+        arrive(&st->ds_ready);
       }
     }
   }
@@ -971,6 +975,8 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](uint64_t *b) { return ptx::smem_u32(b); };
   auto wait = [&](uint64_t *b, uint32_t par, int code) { return ptx::mbar_wait<false>(bar(b), par & 1u, abort_flag, p.status, code); };
+  // every thread arrives for itself (one arrival per warp measured the same)
+  auto arrive = [&](uint64_t *b) { ptx::mbar_arrive(bar(b)); };
 
   if (tid == 0) {
     ptx::mbar_init(bar(&st->kv_full), 1);
@@ -1173,7 +1179,7 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
       ptx::tc_fence_after();
       load_columns<32>(lane_addr + COL_S + cols * 32, x);
       ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(&st->s_read));
+      arrive(&st->s_read);
       probabilities<32>(x, c, -lse2);
       if (masked) {
 #pragma unroll
@@ -1183,12 +1189,12 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
       store_chunks<4>(p_addr, trow, (cols & 1) * 4, x);
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(&st->p_ready));
+      arrive(&st->p_ready);
       if (!wait(&st->dp_full, (uint32_t)i, ST_BK_DP)) goto teardown;
       ptx::tc_fence_after();
       load_columns<32>(lane_addr + COL_DP + cols * 32, d);
       ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(&st->dp_read));
+      arrive(&st->dp_read);
       score_gradients<32>(d, x, delta);
       if (masked) {  // a masked product may be anything
 #pragma unroll
@@ -1198,7 +1204,7 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
       store_chunks<4>(ds_addr, trow, (cols & 1) * 4, d);
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(&st->ds_ready));
+      arrive(&st->ds_ready);
     }
     if (n > 0) {
       if (!wait(&st->dk_done, (uint32_t)(n - 1), ST_BK_DK) || !wait(&st->dv_done, (uint32_t)(n - 1), ST_BK_DV)) goto teardown;
@@ -1248,27 +1254,26 @@ teardown:
   }
 }
 
-// dK and dV of the sink rows: the shares of a block's units, in order. Grid: (blocks with sinks * kv heads, sequences); a thread per
-// (row, dimension).
+// dK and dV of the sink rows: the shares of a block's units, in order. Grid: (blocks with sinks * kv heads, sequences, elements of a
+// block's rows / 256); a thread per element.
 __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ BwdParams p, int head_dim) {
   const int s = blockIdx.y, kb = blockIdx.x / p.kv_heads, kvh = blockIdx.x % p.kv_heads;
   const Span sp = span_of(p.seqs, s);
   if (kb >= split_blocks(sp.Tk, p.sinks)) return;
   const int chunks = key_walk(sp.Tq, sp.Tk, kb, p.window, p.sinks).chunks, most = key_walk(sp.Tq, sp.Tk, 0, p.window, p.sinks).chunks;
-  if (chunks == 0) return;
-  const int rows = min(min(p.sinks, sp.Tk) - kb * TILE, TILE);
+  const int rows = min(min(p.sinks, sp.Tk) - kb * TILE, TILE), i = blockIdx.z * 256 + threadIdx.x;
+  if (chunks == 0 || i >= rows * 2 * head_dim) return;
   const int64_t step = (int64_t)p.kv_heads * p.slot_rows * 2 * head_dim;
-  const float *first = p.shares + ((int64_t)(p.slot[s] + kb * (most + 1)) * p.kv_heads + kvh) * p.slot_rows * 2 * head_dim;
-  for (int i = threadIdx.x; i < rows * 2 * head_dim; i += 256) {
-    float sum = 0.0f;
-    for (int c = 0; c <= chunks; c++) sum += first[c * step + i];
-    const int row = i / (2 * head_dim), d = i - row * 2 * head_dim;
-    const int64_t at = ((int64_t)(sp.k_off + kb * TILE + row) * p.kv_heads + kvh) * head_dim;
-    if (d < head_dim)
-      p.dk[at + d] = __float2bfloat16_rn(sum);
-    else
-      p.dv[at + d - head_dim] = __float2bfloat16_rn(sum);
-  }
+  const float *share = p.shares + ((int64_t)(p.slot[s] + kb * (most + 1)) * p.kv_heads + kvh) * p.slot_rows * 2 * head_dim + i;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int c = 0; c <= chunks; c++) sum += share[c * step];
+  const int row = i / (2 * head_dim), d = i - row * 2 * head_dim;
+  const int64_t at = ((int64_t)(sp.k_off + kb * TILE + row) * p.kv_heads + kvh) * head_dim;
+  if (d < head_dim)
+    p.dk[at + d] = __float2bfloat16_rn(sum);
+  else
+    p.dv[at + d - head_dim] = __float2bfloat16_rn(sum);
 }
 
 bool sm100_supported(int head_dim) { return head_dim == 64 || head_dim == 128; }
@@ -1419,7 +1424,8 @@ int sm100_bwd(const Call &c) {
     p.units = p.main_units + p.far[p.seqs.n];
     if (c.head_dim == 128 ? launch_bwd_kv<128>(p, d, c.stream) : launch_bwd_kv<64>(p, d, c.stream)) return -1;
     if (blocks == 0) continue;
-    window_join_kernel<<<dim3((unsigned)(blocks * c.kv_heads), (unsigned)p.seqs.n), 256, 0, c.stream>>>(p, c.head_dim);
+    window_join_kernel<<<dim3((unsigned)(blocks * c.kv_heads), (unsigned)p.seqs.n, (unsigned)(p.slot_rows * 2 * c.head_dim + 255) / 256), 256, 0,
+                         c.stream>>>(p, c.head_dim);
     B200_CHECK_LAUNCH("attention_window_bwd (sinks)");
   }
   return 0;
