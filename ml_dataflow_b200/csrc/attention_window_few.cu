@@ -3,8 +3,9 @@
 // Such a call reads every visible key and value once and computes next to nothing: memory bounds it, and, in small batches, latency. The
 // query heads of a group are the rows of one 16-row tile, so K and V are read once for all of them. A unit is such a tile of one
 // sequence and key/value head; its visible keys - the sinks, then the window - are numbered through and cut into blocks of 64, which the
-// CTAs of a cluster take in turn. There are as many CTAs per unit (1, 2, 4 or 8) as it takes to give every SM two; they join their
-// partial sums through each other's shared memory, so that a call is one launch and needs no workspace.
+// CTAs of a cluster take in turn. There are as many CTAs per unit (1, 2, 4 or 8) as every SM can hold two of at once (32 sequences of up
+// to 4100 visible keys, 128 units: 2 CTAs each 37 us, 4 each 44 to 49); they join their partial sums through each other's shared memory, so
+// that a call is one launch and needs no workspace.
 //
 // A CTA: 4 warps, 16 keys of a block each, three blocks of K and V in flight (cp.async, 96 KB at head size 128, two CTAs per SM). Products
 // with m16n8k16 warp-level MMAs: a 128-row tcgen05 tile would be seven eighths empty and wait for tensor memory first. Online
@@ -378,7 +379,7 @@ int few_fwd(const Call &c) {
     if (p.n == 0) return 0;
     const int units = p.first[p.n];
     p.cluster = 1;
-    while (p.cluster < MAX_CLUSTER && units * p.cluster < 2 * 148 && (int64_t)p.cluster * KEYS < most) p.cluster *= 2;
+    while (p.cluster < MAX_CLUSTER && units * p.cluster <= 148 && (int64_t)p.cluster * KEYS < most) p.cluster *= 2;
     if (c.head_dim == 128 ? launch_few<128>(p, units, c.stream) : launch_few<64>(p, units, c.stream)) return -1;
   }
   return 0;
