@@ -849,6 +849,12 @@ int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int num_q_head
  * zero gradient, and keys of a sequence that none of its queries sees, like rows outside the sequences, may hold anything.
  * head_dim a multiple of 8 up to 256, tensors 16-byte aligned, bf16 only. The reference has no window: no counterpart.
  *
+ * Head sizes 64 and 128 run on the tensor cores (csrc/attention_window_sm100.cu; sequences with few queries, up to 32 rows of a group, in
+ * csrc/attention_window_few.cu), the others on the fp32 units. All sums have a fixed order: two runs give the same bits. Rounding as in
+ * b200_attention_fwd / _bwd, but dS is formed from the fp32 probabilities; delta is formed from x_attn_out as it is stored, in bf16. A
+ * value of infinity or NaN reaches the queries of the 128-row tiles that see it. A wait inside the kernels that runs out raises the word
+ * that b200_attention_status reads. As with the other entry points, the first call on a device comes before any stream capture.
+ *
  * The forward needs no workspace. The backward's is sized by b200_attention_window_workspace_bytes(max_num_seqs, ...,
  * max_total_q, num_sinks), which covers every smaller batch. dx_q / dx_k / dx_v are overwritten.
  */
@@ -873,7 +879,8 @@ int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, int total_k
  * An infinity or NaN is held as NaN and does not touch the others of its block; numbers above 240 * 2^120 (3.19e38) are held
  * as that, the largest multiple that bf16 has.
  *
- * b200_swiglu_act8: b200_swiglu (out = silu(x_w1) * x_w3; not formed when out is NULL) that also holds its inputs.
+ * b200_swiglu_act8: b200_swiglu (out = silu(x_w1) * x_w3; not formed when out is NULL) that also holds its inputs; out may be x_w1 or
+ * x_w3 itself.
  * b200_swiglu_recompute_act8: the held x_w1, x_w3 as bf16 and h = silu(x_w1) * x_w3 of them, each when not NULL.
  * b200_swiglu_bwd_x_act8: b200_swiglu_bwd_x on the held values; out, when not NULL, receives h of them. dX_w1 or dX_w3 may be
  * upstream_dX itself. n_cols a multiple of 8; bf16 tensors 16-byte aligned, codes 8-byte aligned. No counterpart in the reference, which

@@ -65,6 +65,13 @@ struct Places {
   }
 };
 
+// bypasses L1; not a read-only load, because h may be written over x1 or x3
+__device__ __forceinline__ uint4 ld_once(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // exponent of the block's unit, biased by 127, from the bf16 bits of its largest finite magnitude
 __device__ __forceinline__ int unit_of(uint32_t top) {
   const int e = (int)(top >> 7) - 135 + ((top & 0x7f) > 0x60);  // 448 = 1.75 * 2^8
@@ -174,8 +181,8 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(Shape s, const uint4 *x1,
       const Place p = places(s, u * THREADS + threadIdx.x);
       a[u] = b[u] = make_uint4(0, 0, 0, 0);
       if (p.on) {
-        a[u] = ld_stream(x1 + p.vec);
-        b[u] = ld_stream(x3 + p.vec);
+        a[u] = ld_once(x1 + p.vec);
+        b[u] = ld_once(x3 + p.vec);
       }
     }
 #pragma unroll

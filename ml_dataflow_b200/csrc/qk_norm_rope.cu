@@ -74,14 +74,15 @@ __global__ void __launch_bounds__(THREADS, BWD ? BWD_BLOCKS : FWD_BLOCKS) qk_nor
   const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
 
   // Many tokens: a warp takes every `stride`th token and all of its rounds. Few: one round of one token.
-  const int w = blockIdx.x * WARPS + warp, stride = gridDim.x * WARPS;
+  const uint32_t w = blockIdx.x * WARPS + warp, stride = gridDim.x * WARPS, tokens = p.tokens;  // unsigned: a sum may pass 2^31
   struct At {
-    int tok, rd;
+    uint32_t tok;
+    int rd;
   };
-  const int only = p.spread ? w % rounds : 0;
-  At now = {p.spread ? w / rounds : w, only};
+  const int only = p.spread ? (int)(w % (uint32_t)rounds) : 0;
+  At now = {p.spread ? w / (uint32_t)rounds : w, only};
   auto next = [&](At a) {
-    if (p.spread) return At{p.tokens, 0};
+    if (p.spread) return At{tokens, 0};
     return a.rd + 1 < rounds ? At{a.tok, a.rd + 1} : At{a.tok + stride, 0};
   };
   struct Where {
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(THREADS, BWD ? BWD_BLOCKS : FWD_BLOCKS) qk_nor
   constexpr int PER_STAGE = BATCH * (BWD ? 2 : 1) * 32;
   uint4 *ring = s_ring + warp * STAGES * PER_STAGE + lane;
   auto fetch = [&](At a, int stage) {
-    if (a.tok < p.tokens) {
+    if (a.tok < tokens) {
       const Where r = where(a);
       const uint4 *px = (r.is_q ? p.q : p.k) + r.at, *pd = BWD ? (r.is_q ? p.dyq : p.dyk) + r.at : nullptr;
       uint4 *to = ring + stage * PER_STAGE;
@@ -118,20 +119,20 @@ __global__ void __launch_bounds__(THREADS, BWD ? BWD_BLOCKS : FWD_BLOCKS) qk_nor
 #pragma unroll
   for (int s = 0; s < STAGES - 1; s++) {
     fetch(ahead, s);
-    if (ahead.tok < p.tokens) ahead = next(ahead);
+    if (ahead.tok < tokens) ahead = next(ahead);
   }
-  int pos = now.tok < p.tokens ? __ldg(p.pos + now.tok) : 0;
+  int pos = now.tok < tokens ? __ldg(p.pos + now.tok) : 0;
   for (int i = threadIdx.x; i < p.head_dim / 2; i += THREADS)  // while the first rounds are on their way
     s_turns[i] = exp2(-(double)(2 * i) / (double)p.head_dim * p.log2_theta) * 0.15915494309189533577;  // / (2 pi)
   __syncthreads();
   float cs[4], sn[4];
-  for (int stage = 0; now.tok < p.tokens; now = next(now)) {
+  for (int stage = 0; now.tok < tokens; now = next(now)) {
     fetch(ahead, stage == 0 ? STAGES - 1 : stage - 1);
-    if (ahead.tok < p.tokens) ahead = next(ahead);
+    if (ahead.tok < tokens) ahead = next(ahead);
     const Where r = where(now);
     if (now.rd == only) {  // a new token
       turn_angles((double)pos, turns, cs, sn);
-      if (!p.spread && now.tok + stride < p.tokens) pos = __ldg(p.pos + now.tok + stride);
+      if (!p.spread && now.tok + stride < tokens) pos = __ldg(p.pos + now.tok + stride);
     }
     const uint4 *weight = r.is_q ? p.wq : p.wk;
     const uint4 wv = weight && on_row ? __ldg(weight + c) : ones;

@@ -540,8 +540,8 @@ def attention_window_bwd(q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_
                                            x_attn_out, softmax_lse, window, num_sinks)
     _check(_lib.load().b200_attention_window_bwd(
         *args, _ptr(op, "dx_out", dx_out, nq, _BF, dev), _ptr(op, "dx_q", dx_q, nq, _BF, dev), _ptr(op, "dx_k", dx_k, nk, _BF, dev),
-        _ptr(op, "dx_v", dx_v, nk, _BF, dev), window, num_sinks, workspace.numel(), _ptr(op, "workspace", workspace, 0, _U8, dev),
-        _raw_stream(dev)), op, 2 * -(-len(q_lens) // 48))
+        _ptr(op, "dx_v", dx_v, nk, _BF, dev), window, num_sinks, 0 if workspace is None else workspace.numel(),
+        _ptr(op, "workspace", workspace, 0, _U8, dev), _raw_stream(dev)), op, 2 * -(-len(q_lens) // 48))
 
 
 # ---- SwiGLU activations held in 8 bits --------------------------------------------------------------------------------------

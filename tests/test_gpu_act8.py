@@ -81,6 +81,11 @@ def test_keep_restore_backward(R, f):
     c2 = _codes(R, f)
     ops.swiglu_act8(R, f, x1, x3, None, *c2)
     assert all(torch.equal(s, t) for s, t in zip(c, c2))
+    for which in (0, 1):  # h over either input
+        ins = [x1.clone(), x3.clone()]
+        c3 = _codes(R, f)
+        ops.swiglu_act8(R, f, *ins, ins[which], *c3)
+        assert torch.equal(ins[which], h) and all(torch.equal(s, t) for s, t in zip(c, c3))
     for which in (0, 1):
         up, other = dh.clone(), torch.empty_like(dh)
         out = (up, other) if which == 0 else (other, up)

@@ -29,6 +29,10 @@ CASES = [
     ([1, 1, 5, 1], [33, 3000, 2000, 7], 8, 1, 64, 1000, 40),
     (list(range(1, 61)), [n + (n % 3) * 50 for n in range(1, 61)], 4, 2, 128, 24, 2),
     ([1] * 70, [3 * n + 1 for n in range(70)], 4, 1, 64, 40, 4),
+    ([1, 1, 2], [700, 3, 260], 24, 1, 128, 300, 5),     # few queries: more rows than one 16-row tile of a group; 48 rows go to the tiles
+    ([1, 2], [500, 900], 40, 1, 64, 1000, 0),           # a group of 40 heads
+    ([1, 3, 1], [2000, 130, 77], 21, 3, 128, 90, 2),    # an odd group
+    ([2] * 200, [2 + 5 * n for n in range(200)], 2, 1, 64, 64, 3),  # more sequences than one launch of the few-query form takes
 ]
 
 
