@@ -172,6 +172,8 @@ __device__ __forceinline__ void swiglu(const uint64_t *x, const uint64_t *y, uin
 template <bool WHOLE>
 __global__ void __launch_bounds__(THREADS) keep_kernel(Shape s, const uint4 *x1, const uint4 *x3, uint4 *out, uint2 *c1, uint8_t *e1,
                                                        uint2 *c3, uint8_t *e3) {
+  pdl_release();
+  pdl_wait();
   const int64_t step = (int64_t)gridDim.x * THREADS * UNROLL;
   for (int64_t base = (int64_t)blockIdx.x * THREADS * UNROLL; base < s.padded; base += step) {
     const Places<WHOLE> places(s, base);
@@ -212,6 +214,8 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(Shape s, const uint4 *x1,
 template <bool WHOLE>
 __global__ void __launch_bounds__(THREADS) restore_kernel(Shape s, const uint2 *c1, const uint8_t *e1, const uint2 *c3, const uint8_t *e3,
                                                           uint4 *x1, uint4 *x3, uint4 *out) {
+  pdl_release();
+  pdl_wait();
   const int64_t step = (int64_t)gridDim.x * THREADS * UNROLL;
   for (int64_t base = (int64_t)blockIdx.x * THREADS * UNROLL; base < s.padded; base += step) {
     const Places<WHOLE> places(s, base);
@@ -249,6 +253,8 @@ __global__ void __launch_bounds__(THREADS) restore_kernel(Shape s, const uint2 *
 template <bool WHOLE>
 __global__ void __launch_bounds__(THREADS) backward_kernel(Shape s, const uint2 *c1, const uint8_t *e1, const uint2 *c3, const uint8_t *e3,
                                                            const uint4 *dh, uint4 *dx1, uint4 *dx3, uint4 *out) {
+  pdl_release();
+  pdl_wait();
   const int64_t step = (int64_t)gridDim.x * THREADS * UNROLL;
   for (int64_t base = (int64_t)blockIdx.x * THREADS * UNROLL; base < s.padded; base += step) {
     const Places<WHOLE> places(s, base);
@@ -295,13 +301,9 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(Shape s, const uint2 
 using namespace b200;
 
 // the kernel for columns that are whole scale blocks, or the other
-#define ACT8_LAUNCH(kernel, ...)                                                                                            \
-  do {                                                                                                                      \
-    if (s.vecs == s.padded_vecs)                                                                                            \
-      act8::kernel<true><<<act8_grid(s.padded), act8::THREADS, 0, (cudaStream_t)stream>>>(s, __VA_ARGS__);                   \
-    else                                                                                                                    \
-      act8::kernel<false><<<act8_grid(s.padded), act8::THREADS, 0, (cudaStream_t)stream>>>(s, __VA_ARGS__);                  \
-  } while (0)
+#define ACT8_LAUNCH(kernel, ...)                                                                                                   \
+  B200_CUDA(b200_launch_overlapped(s.vecs == s.padded_vecs ? act8::kernel<true> : act8::kernel<false>, dim3(act8_grid(s.padded)),   \
+                                   dim3(act8::THREADS), 0, (cudaStream_t)stream, 1, s, __VA_ARGS__))
 
 namespace {
 

@@ -141,6 +141,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) window_few_kernel(const __grid
       cp16(dst + Sh::TILE + place(r, chunk), V + at, on);
     }
   };
+  pdl_release();
+  pdl_wait();
 #pragma unroll
   for (int i = 0; i < STAGES - 1; i++) {
     if (i < mine) fetch(rank + i * p.cluster, i);
@@ -323,18 +325,8 @@ int launch_few(const window::FewParams &p, int units, cudaStream_t s) {
     B200_CUDA(cudaFuncSetAttribute(window::window_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     done[dev] = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * p.cluster));
-  cfg.blockDim = dim3(window::FEW_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)p.cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  B200_CUDA(cudaLaunchKernelEx(&cfg, window::window_few_kernel<HD>, p));
+  B200_CUDA(b200_launch_overlapped(window::window_few_kernel<HD>, dim3((unsigned)(units * p.cluster)), dim3(window::FEW_THREADS), smem, s,
+                                   (unsigned)p.cluster, p));
   B200_CHECK_LAUNCH("attention_window_fwd (few queries)");
   return 0;
 }

@@ -285,6 +285,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = st->tmem_base;
+  pdl_release();
+  pdl_wait();
 
   // The ring: step t of the CTA (counted through its units) uses K at place max(0, 2 t - 1) and V at place 2 t + 2: a unit's first K
   // goes before the last unit's last V.
@@ -678,6 +680,8 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = st->tmem_base;
+  pdl_release();
+  pdl_wait();
 
   if (warp < 4) {
     ptx::reg_dec<REGS_BWD_Q_OTHER>();
@@ -1015,6 +1019,8 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = st->tmem_base;
+  pdl_release();
+  pdl_wait();
 
   // the unit: a block of keys of one key/value head, and the query tiles it walks for every query head of the group
   const int unit = blockIdx.x;
@@ -1257,6 +1263,8 @@ teardown:
 // dK and dV of the sink rows: the shares of a block's units, in order. Grid: (blocks with sinks * kv heads, sequences, elements of a
 // block's rows / 256); a thread per element.
 __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ BwdParams p, int head_dim) {
+  pdl_release();
+  pdl_wait();
   const int s = blockIdx.y, kb = blockIdx.x / p.kv_heads, kvh = blockIdx.x % p.kv_heads;
   const Span sp = span_of(p.seqs, s);
   if (kb >= split_blocks(sp.Tk, p.sinks)) return;
@@ -1323,7 +1331,7 @@ int launch_fwd(window::FwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
   constexpr size_t smem = window::FwdShape<HD>::smem;
   if (allow_smem(window::window_fwd_kernel<HD>, smem, &done[d.dev])) return -1;
-  window::window_fwd_kernel<HD><<<p.units < d.sms ? p.units : d.sms, window::FWD_THREADS, smem, s>>>(p);
+  B200_CUDA(b200_launch_overlapped(window::window_fwd_kernel<HD>, dim3(p.units < d.sms ? p.units : d.sms), dim3(window::FWD_THREADS), smem, s, 1, p));
   B200_CHECK_LAUNCH("attention_window_fwd");
   return 0;
 }
@@ -1333,7 +1341,7 @@ int launch_bwd_q(const window::BwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
   constexpr size_t smem = window::BwdQShape<HD>::smem;
   if (allow_smem(window::window_bwd_q_kernel<HD>, smem, &done[d.dev])) return -1;
-  window::window_bwd_q_kernel<HD><<<p.units < d.sms ? p.units : d.sms, window::BWD_Q_THREADS, smem, s>>>(p);
+  B200_CUDA(b200_launch_overlapped(window::window_bwd_q_kernel<HD>, dim3(p.units < d.sms ? p.units : d.sms), dim3(window::BWD_Q_THREADS), smem, s, 1, p));
   B200_CHECK_LAUNCH("attention_window_bwd (dQ)");
   return 0;
 }
@@ -1343,7 +1351,7 @@ int launch_bwd_kv(const window::BwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
   constexpr size_t smem = window::BwdKShape<HD>::smem;
   if (allow_smem(window::window_bwd_kv_kernel<HD>, smem, &done[d.dev])) return -1;
-  window::window_bwd_kv_kernel<HD><<<p.units, window::BWD_KV_THREADS, smem, s>>>(p);
+  B200_CUDA(b200_launch_overlapped(window::window_bwd_kv_kernel<HD>, dim3(p.units), dim3(window::BWD_KV_THREADS), smem, s, 1, p));
   B200_CHECK_LAUNCH("attention_window_bwd (dK, dV)");
   return 0;
 }
@@ -1424,8 +1432,8 @@ int sm100_bwd(const Call &c) {
     p.units = p.main_units + p.far[p.seqs.n];
     if (c.head_dim == 128 ? launch_bwd_kv<128>(p, d, c.stream) : launch_bwd_kv<64>(p, d, c.stream)) return -1;
     if (blocks == 0) continue;
-    window_join_kernel<<<dim3((unsigned)(blocks * c.kv_heads), (unsigned)p.seqs.n, (unsigned)(p.slot_rows * 2 * c.head_dim + 255) / 256), 256, 0,
-                         c.stream>>>(p, c.head_dim);
+    const dim3 grid((unsigned)(blocks * c.kv_heads), (unsigned)p.seqs.n, (unsigned)(p.slot_rows * 2 * c.head_dim + 255) / 256);
+    B200_CUDA(b200_launch_overlapped(window_join_kernel, grid, dim3(256), 0, c.stream, 1, p, c.head_dim));
     B200_CHECK_LAUNCH("attention_window_bwd (sinks)");
   }
   return 0;

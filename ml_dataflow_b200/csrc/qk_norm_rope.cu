@@ -115,6 +115,8 @@ __global__ void __launch_bounds__(THREADS, BWD ? BWD_BLOCKS : FWD_BLOCKS) qk_nor
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  pdl_release();
+  pdl_wait();
   At ahead = now;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; s++) {
@@ -237,6 +239,8 @@ constexpr int JOIN_WARPS = 32;
 __global__ void __launch_bounds__(JOIN_WARPS * 32) qk_weight_grad_kernel(int head_dim, int blocks, const float *__restrict__ partial,
                                                                        bool accumulate, __nv_bfloat16 *dwq, __nv_bfloat16 *dwk) {
   __shared__ float part[JOIN_WARPS][32];
+  pdl_release();
+  pdl_wait();
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int i = blockIdx.x * 32 + lane;
   float s = 0.0f;
@@ -298,7 +302,7 @@ int qkn_launch_lanes(const char *op, const qkn::Params &p, int blocks, cudaStrea
     B200_CUDA(cudaFuncSetAttribute(qkn::qk_norm_rope_kernel<LANES, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     done[dev] = true;
   }
-  qkn::qk_norm_rope_kernel<LANES, BWD><<<blocks, qkn::THREADS, smem, s>>>(p);
+  B200_CUDA(b200_launch_overlapped(qkn::qk_norm_rope_kernel<LANES, BWD>, dim3(blocks), dim3(qkn::THREADS), smem, s, 1, p));
   B200_CHECK_LAUNCH(op);
   return 0;
 }
@@ -401,8 +405,9 @@ extern "C" int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int
   p.dyk = (const uint4 *)d_out_k;
   if (qkn_launch<true>("qk_norm_rope_bwd", p, blocks, (cudaStream_t)stream)) return -1;
   if (!want_dw) return 0;
-  qkn::qk_weight_grad_kernel<<<(2 * head_dim + 31) / 32, qkn::JOIN_WARPS * 32, 0, (cudaStream_t)stream>>>(
-      head_dim, blocks, p.partial, accumulate != 0, (__nv_bfloat16 *)dq_weight, (__nv_bfloat16 *)dk_weight);
+  B200_CUDA(b200_launch_overlapped(qkn::qk_weight_grad_kernel, dim3((2 * head_dim + 31) / 32), dim3(qkn::JOIN_WARPS * 32), 0, (cudaStream_t)stream, 1,
+                                   head_dim, blocks, (const float *)p.partial, accumulate != 0, (__nv_bfloat16 *)dq_weight,
+                                   (__nv_bfloat16 *)dk_weight));
   B200_CHECK_LAUNCH("qk_norm_rope_bwd (weights)");
   return 0;
 }
