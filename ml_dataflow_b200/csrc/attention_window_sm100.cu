@@ -560,7 +560,8 @@ teardown:
 // its keys, K and V stay in shared memory. Per tile
 //     S = Q K^T,  dP = dO V^T,   dV += P^T dO,   dK += dS^T Q      (P and dS are read by the tensor cores with the rows as reduction)
 // Blocks that hold sinks are seen by every later query: tiles behind the block's window are cut into further units that sum their
-// share of the sink rows into the workspace, and a last kernel adds the shares in order.
+// share of the sink rows into the workspace, and a last kernel adds the shares in order. In batches too small to fill the GPU the heads of a
+// group are split over units the same way (45 - 391 keys, 8 heads on one: 30 -> 13 us).
 //
 // Rounding: P and dS to bf16 once each (dS from the fp32 P), accumulators fp32, one rounding per output.
 // What bounds both: shared memory. A 128 x 128 x 128 product reads 64 KB of operands in the 512 cycles that it takes, all that
@@ -580,8 +581,9 @@ struct BwdParams {
   float *delta;  // [q_heads][total_q]
   __nv_bfloat16 *dq, *dk, *dv;
   int window, sinks, group, q_heads, kv_heads, total_q, units;
-  // dK, dV: units from main_units on are shares of the sink rows; share[s]: the first slot of sequence s in the workspace
-  int main_units, slot_rows;
+  // dK, dV: units from main_units on are shares of the sink rows; slot[s]: the first slot of sequence s in the workspace. Or, with
+  // parts > 1: every block's heads are split over so many units, whose shares cover all rows
+  int main_units, slot_rows, parts;
   int far[MAX_SEQS + 1], slot[MAX_SEQS];
   float *shares;  // [slots][kv_heads][slot_rows][2][head_dim]
   float scale;
@@ -926,8 +928,9 @@ struct KeyWalk {
   int t0, t1, tiles, chunk, chunks;
 };
 constexpr int MIN_CHUNK = 8;         // tiles of such a unit: at least this many, and as many as a block's window spans
+constexpr int MAX_SPLIT_UNITS = 148;   // units that the heads of a small batch are split into, at most
 constexpr int MAX_SPLIT_SINKS = 1024;  // more sinks than this fill the GPU with blocks of their own: their units walk every tile
-__host__ __device__ inline KeyWalk key_walk(int Tq, int Tk, int kb, int window, int sinks) {
+__host__ __device__ inline KeyWalk key_walk(int Tq, int Tk, int kb, int window, int sinks, bool split = true) {
   KeyWalk w;
   const int shift = Tk - Tq;
   w.tiles = (Tq + TILE - 1) / TILE;
@@ -938,7 +941,7 @@ __host__ __device__ inline KeyWalk key_walk(int Tq, int Tk, int kb, int window, 
   w.chunk = window / TILE + 1 > MIN_CHUNK ? window / TILE + 1 : MIN_CHUNK;
   w.chunks = 0;
   if ((int64_t)kb * TILE < sinks) {
-    if (sinks > MAX_SPLIT_SINKS)
+    if (!split || sinks > MAX_SPLIT_SINKS)
       w.t1 = w.tiles;
     else
       w.chunks = (w.tiles - w.t1 + w.chunk - 1) / w.chunk;
@@ -1023,7 +1026,8 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
   pdl_wait();
 
   // the unit: a block of keys of one key/value head, and the query tiles it walks for every query head of the group
-  const int unit = blockIdx.x;
+  const int unit = blockIdx.x / p.parts, head_part = blockIdx.x % p.parts;
+  const int h0 = head_part * p.group / p.parts, heads = (head_part + 1) * p.group / p.parts - h0;  // of the group
   int s = 0, kb, kvh, t0, t1, share = -1;  // share: the slot of the workspace that takes the sink rows
   if (unit < p.main_units) {
     while (unit >= p.seqs.first[s + 1]) s++;
@@ -1036,7 +1040,7 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
     kb = 0;
   }
   const Span sp = span_of(p.seqs, s);
-  const int most = key_walk(sp.Tq, sp.Tk, 0, p.window, p.sinks).chunks;
+  const int most = key_walk(sp.Tq, sp.Tk, 0, p.window, p.sinks, p.parts == 1).chunks;
   int part = 0;
   if (unit >= p.main_units) {
     const int rel = (unit - p.main_units - p.far[s]) / p.kv_heads;  // block, then chunk
@@ -1044,13 +1048,15 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
     part = 1 + rel % most;
   }
   {
-    const KeyWalk w = key_walk(sp.Tq, sp.Tk, kb, p.window, p.sinks);
+    const KeyWalk w = key_walk(sp.Tq, sp.Tk, kb, p.window, p.sinks, p.parts == 1);
     t0 = part == 0 ? w.t0 : w.t1 + (part - 1) * w.chunk;
     t1 = part == 0 ? w.t1 : min(w.tiles, t0 + w.chunk);
     if (w.chunks > 0) share = p.slot[s] + kb * (most + 1) + part;
     if (part > w.chunks) share = -1;  // this block is split into fewer units than the first: nothing to do
   }
-  const int tiles = max(0, t1 - t0), n = tiles * p.group;
+  if (p.parts > 1) share = blockIdx.x;
+  const int share_rows = p.parts > 1 ? sp.Tk : p.sinks;  // keys below this go to the share
+  const int tiles = max(0, t1 - t0), n = tiles * heads;
 
   if (n > 0 && warp == 0) {
     // ================= loads: the whole warp walks, one lane issues =================
@@ -1062,7 +1068,7 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
       ptx::tma_load_3d(ptx::smem_u32(sK), &p.tmK, bar(&st->kv_full), 0, sp.k_off + kb * TILE, kvh * KSL);
       ptx::tma_load_3d(ptx::smem_u32(sV), &p.tmV, bar(&st->kv_full), 0, sp.k_off + kb * TILE, kvh * KSL);
     }
-    for (int i = 0, tile_at = t0, h = kvh * p.group; ok && i < n; i++) {
+    for (int i = 0, tile_at = t0, h = kvh * p.group + h0; ok && i < n; i++) {
       const int row = tile_at * TILE;
       const bool fix = row + TILE > sp.Tq;  // rows past the sequence's end are zeroed: dO and Q multiply P and dS
 #pragma unroll
@@ -1154,7 +1160,7 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
     const float c = p.scale * LOG2E;
     // a step's statistics are fetched while the step before computes: `ahead` is its tile, stat_at its row in the arrays
     int ahead = t0;
-    int64_t stat_at = (int64_t)(kvh * p.group) * p.total_q + sp.q_off + t0 * TILE + trow;
+    int64_t stat_at = (int64_t)(kvh * p.group + h0) * p.total_q + sp.q_off + t0 * TILE + trow;
     float lse2 = 0.0f, delta = 0.0f, next_lse = 0.0f, next_delta = 0.0f;
     auto fetch = [&]() {
       if (ahead * TILE + trow < sp.Tq) {
@@ -1220,8 +1226,9 @@ __global__ void __launch_bounds__(BWD_KV_THREADS, 1) window_bwd_kv_kernel(const 
       // the accumulators' lanes are keys
       constexpr int DIMS = HD / 4;
       const int key = kb * TILE + trow;
-      const bool to_share = share >= 0 && key < p.sinks;
-      float *sh = to_share ? p.shares + (((int64_t)share * p.kv_heads + kvh) * p.slot_rows + trow) * 2 * HD + cols * DIMS : nullptr;
+      const bool to_share = share >= 0 && key < share_rows;
+      const int64_t slot = p.parts > 1 ? share : (int64_t)share * p.kv_heads + kvh;
+      float *sh = to_share ? p.shares + (slot * p.slot_rows + trow) * 2 * HD + cols * DIMS : nullptr;
       const int64_t at = ((int64_t)(sp.k_off + key) * p.kv_heads + kvh) * HD + cols * DIMS;
 #pragma unroll
       for (int which = 0; which < 2; which++) {
@@ -1278,6 +1285,28 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   for (int c = 0; c <= chunks; c++) sum += share[c * step];
   const int row = i / (2 * head_dim), d = i - row * 2 * head_dim;
   const int64_t at = ((int64_t)(sp.k_off + kb * TILE + row) * p.kv_heads + kvh) * head_dim;
+  if (d < head_dim)
+    p.dk[at + d] = __float2bfloat16_rn(sum);
+  else
+    p.dv[at + d - head_dim] = __float2bfloat16_rn(sum);
+}
+
+// dK and dV of blocks whose heads were split: their shares, in order. Grid: (blocks of keys * kv heads, elements of a block / 256).
+__global__ void __launch_bounds__(256) window_join_heads_kernel(const __grid_constant__ BwdParams p, int head_dim) {
+  pdl_release();
+  pdl_wait();
+  int s = 0;
+  while ((int)blockIdx.x >= p.seqs.first[s + 1]) s++;
+  const Span sp = span_of(p.seqs, s);
+  const int rel = blockIdx.x - p.seqs.first[s], kvh = rel % p.kv_heads, kb = rel / p.kv_heads, i = blockIdx.y * 256 + threadIdx.x;
+  const int row = i / (2 * head_dim), d = i - row * 2 * head_dim, key = kb * TILE + row;
+  if (key >= sp.Tk) return;
+  const int64_t step = (int64_t)TILE * 2 * head_dim;
+  const float *share = p.shares + (int64_t)blockIdx.x * p.parts * step + i;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int c = 0; c < p.parts; c++) sum += share[c * step];
+  const int64_t at = ((int64_t)(sp.k_off + key) * p.kv_heads + kvh) * head_dim;
   if (d < head_dim)
     p.dk[at + d] = __float2bfloat16_rn(sum);
   else
@@ -1365,16 +1394,18 @@ int slot_rows(int sinks) { return sinks < window::TILE ? sinks : window::TILE; }
 namespace b200 {
 namespace window {
 
-// delta, then the shares of the sink rows. A block's shares: its own and those of at most ceil(tiles / MIN_CHUNK) further units, that is
+// delta, then the shares: those of split heads or those of the sink rows. A block's sink shares: its own and those of at most ceil(tiles / MIN_CHUNK) further units, that is
 // Tq / 1024 + 3 at most.
 uint64_t sm100_bwd_workspace(int num_seqs, int q_heads, int kv_heads, int head_dim, int total_q, int sinks) {
   static_assert(TILE * MIN_CHUNK == 1024, "the bound on a sequence's shares");
-  uint64_t n = up256((uint64_t)total_q * q_heads * sizeof(float));
+  uint64_t n = 0;
+  if (q_heads > kv_heads) n = (uint64_t)MAX_SPLIT_UNITS * TILE * 2 * head_dim * sizeof(float);
   if (sinks > 0 && sinks <= MAX_SPLIT_SINKS) {
     const uint64_t seqs = num_seqs < MAX_SEQS ? num_seqs : MAX_SEQS;  // of one launch
-    n += (uint64_t)((sinks + TILE - 1) / TILE) * ((uint64_t)total_q / 1024 + 3 * seqs) * kv_heads * slot_rows(sinks) * 2 * head_dim * sizeof(float);
+    const uint64_t shares = (uint64_t)((sinks + TILE - 1) / TILE) * ((uint64_t)total_q / 1024 + 3 * seqs) * kv_heads * slot_rows(sinks) * 2 * head_dim * sizeof(float);
+    if (shares > n) n = shares;
   }
-  return n;
+  return up256((uint64_t)total_q * q_heads * sizeof(float)) + n;
 }
 
 int sm100_bwd(const Call &c) {
@@ -1407,8 +1438,8 @@ int sm100_bwd(const Call &c) {
   p.kv_heads = c.kv_heads;
   p.total_q = c.total_q;
   p.scale = c.scale;
-  p.slot_rows = slot_rows(c.sinks);
   p.main_units = 0;
+  p.parts = 1;
   p.status = attn_status_ptr();
   B200_REQUIRE(p.status != nullptr, "attention_window: the status word of this device is not reachable");
   for (int next = 0; next < c.num_seqs;) {
@@ -1419,18 +1450,27 @@ int sm100_bwd(const Call &c) {
   for (int next = 0; next < c.num_seqs;) {
     p.main_units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.k_len[s] + TILE - 1) / TILE * c.kv_heads; });
     if (p.main_units == 0) continue;
+    // as many units as there are SMs, if the heads of a group give them
+    p.parts = p.main_units < MAX_SPLIT_UNITS ? MAX_SPLIT_UNITS / p.main_units : 1;
+    if (p.parts > p.group) p.parts = p.group;
+    p.slot_rows = p.parts > 1 ? TILE : slot_rows(c.sinks);
     int slots = 0, blocks = 0;
     p.far[0] = 0;
     for (int s = 0; s < p.seqs.n; s++) {
       const int split = split_blocks(p.seqs.Tk[s], c.sinks), chunks = key_walk(p.seqs.Tq[s], p.seqs.Tk[s], 0, c.window, c.sinks).chunks;
-      const bool any = split > 0 && chunks > 0;
+      const bool any = split > 0 && chunks > 0 && p.parts == 1;
       p.slot[s] = slots;
       p.far[s + 1] = p.far[s] + (any ? split * chunks * c.kv_heads : 0);
       if (any) slots += split * (chunks + 1);
       if (any && split > blocks) blocks = split;
     }
-    p.units = p.main_units + p.far[p.seqs.n];
+    p.units = p.parts > 1 ? p.main_units * p.parts : p.main_units + p.far[p.seqs.n];
     if (c.head_dim == 128 ? launch_bwd_kv<128>(p, d, c.stream) : launch_bwd_kv<64>(p, d, c.stream)) return -1;
+    if (p.parts > 1) {
+      const dim3 all((unsigned)p.main_units, (unsigned)(TILE * 2 * c.head_dim / 256));
+      B200_CUDA(b200_launch_overlapped(window_join_heads_kernel, all, dim3(256), 0, c.stream, 1, p, c.head_dim));
+      B200_CHECK_LAUNCH("attention_window_bwd (heads)");
+    }
     if (blocks == 0) continue;
     const dim3 grid((unsigned)(blocks * c.kv_heads), (unsigned)p.seqs.n, (unsigned)(p.slot_rows * 2 * c.head_dim + 255) / 256);
     B200_CUDA(b200_launch_overlapped(window_join_kernel, grid, dim3(256), 0, c.stream, 1, p, c.head_dim));

@@ -29,6 +29,12 @@ CASES = [
     ([1, 1, 5, 1], [33, 3000, 2000, 7], 8, 1, 64, 1000, 40),
     (list(range(1, 61)), [n + (n % 3) * 50 for n in range(1, 61)], 4, 2, 128, 24, 2),
     ([1] * 70, [3 * n + 1 for n in range(70)], 4, 1, 64, 40, 4),
+    # enough blocks of keys to fill the GPU: heads of a group on one unit, the sinks' far tiles on others
+    ([2600], [2600], 8, 4, 128, 300, 4),
+    ([4000], [4500], 8, 4, 64, 128, 130),
+    ([2000, 0, 700], [2100, 300, 700], 12, 4, 128, 200, 17),
+    ([1700, 900], [1700, 900], 8, 8, 64, 1, 1),
+    ([3000], [3000], 6, 6, 128, 2000, 1100),            # more sinks than are split off
     ([1, 1, 2], [700, 3, 260], 24, 1, 128, 300, 5),     # few queries: more rows than one 16-row tile of a group; 48 rows go to the tiles
     ([1, 2], [500, 900], 40, 1, 64, 1000, 0),           # a group of 40 heads
     ([1, 3, 1], [2000, 130, 77], 21, 3, 128, 90, 2),    # an odd group
