@@ -284,7 +284,7 @@ unsigned blocks_for(int64_t warps) { return (unsigned)((warps + window::WARPS - 
 int rows_fwd(const window::Call &c) {
   window::Params p = rows_params(c);
   for (int next = 0; next < c.num_seqs;) {
-    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.q_len[s]; });
+    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.q_len[s]; }, [](int) { return 0; });
     if (rows == 0) continue;
     window::rows_fwd_kernel<<<blocks_for(rows * c.q_heads), window::THREADS, 0, c.stream>>>(p);
     B200_CHECK_LAUNCH("attention_window_fwd");
@@ -295,13 +295,13 @@ int rows_fwd(const window::Call &c) {
 int rows_bwd(const window::Call &c) {
   window::Params p = rows_params(c);
   for (int next = 0; next < c.num_seqs;) {
-    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.q_len[s]; });
+    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.q_len[s]; }, [](int) { return 0; });
     if (rows == 0) continue;
     window::rows_bwd_q_kernel<<<blocks_for(rows * c.q_heads), window::THREADS, 0, c.stream>>>(p);
     B200_CHECK_LAUNCH("attention_window_bwd (dQ)");
   }
   for (int next = 0; next < c.num_seqs;) {
-    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.k_len[s]; });
+    const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.k_len[s]; }, [](int) { return 0; });
     if (rows == 0) continue;
     window::rows_bwd_kv_kernel<<<blocks_for(rows * c.kv_heads), window::THREADS, 0, c.stream>>>(p);
     B200_CHECK_LAUNCH("attention_window_bwd (dK, dV)");

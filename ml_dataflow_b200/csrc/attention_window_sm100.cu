@@ -1387,6 +1387,12 @@ int launch_bwd_kv(const window::BwdParams &p, const Device &d, cudaStream_t s) {
 
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
+// blocks of 128 keys that a tile of queries sees, at most (of 128 queries that see a block of keys, with the queries' number)
+int blocks_seen(const window::Call &c, int s, int rows) {
+  const int64_t span = (int64_t)c.window + 2 * window::TILE + (c.sinks < c.k_len[s] ? c.sinks : c.k_len[s]);
+  return (int)(((span < rows ? span : rows) + window::TILE - 1) / window::TILE);
+}
+
 int slot_rows(int sinks) { return sinks < window::TILE ? sinks : window::TILE; }
 
 }  // namespace
@@ -1443,12 +1449,14 @@ int sm100_bwd(const Call &c) {
   p.status = attn_status_ptr();
   B200_REQUIRE(p.status != nullptr, "attention_window: the status word of this device is not reachable");
   for (int next = 0; next < c.num_seqs;) {
-    p.units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.q_len[s] + TILE - 1) / TILE * c.q_heads; });
+    p.units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.q_len[s] + TILE - 1) / TILE * c.q_heads; },
+                             [&](int s) { return blocks_seen(c, s, c.k_len[s]); });
     if (p.units == 0) continue;
     if (c.head_dim == 128 ? launch_bwd_q<128>(p, d, c.stream) : launch_bwd_q<64>(p, d, c.stream)) return -1;
   }
   for (int next = 0; next < c.num_seqs;) {
-    p.main_units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.k_len[s] + TILE - 1) / TILE * c.kv_heads; });
+    p.main_units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.k_len[s] + TILE - 1) / TILE * c.kv_heads; },
+                                  [&](int s) { return blocks_seen(c, s, c.q_len[s]); });
     if (p.main_units == 0) continue;
     // as many units as there are SMs, if the heads of a group give them
     p.parts = p.main_units < MAX_SPLIT_UNITS ? MAX_SPLIT_UNITS / p.main_units : 1;
@@ -1503,10 +1511,13 @@ int sm100_fwd(const Call &c) {
   p.status = attn_status_ptr();
   B200_REQUIRE(p.status != nullptr, "attention_window: the status word of this device is not reachable");
   for (int next = 0; next < c.num_seqs;) {
-    p.units = next_sequences(p.seqs, &next, c, [&](int s) {
-      const int tiles = is_few(c, s) ? 0 : (c.q_len[s] + TILE - 1) / TILE;
-      return p.pair_heads ? tiles * (c.q_heads / 2) : (tiles + 1) / 2 * c.q_heads;
-    });
+    p.units = next_sequences(
+        p.seqs, &next, c,
+        [&](int s) {
+          const int tiles = is_few(c, s) ? 0 : (c.q_len[s] + TILE - 1) / TILE;
+          return p.pair_heads ? tiles * (c.q_heads / 2) : (tiles + 1) / 2 * c.q_heads;
+        },
+        [&](int s) { return blocks_seen(c, s, c.k_len[s]); });
     if (p.units == 0) continue;
     if (c.head_dim == 128 ? launch_fwd<128>(p, d, c.stream) : launch_fwd<64>(p, d, c.stream)) return -1;
   }
