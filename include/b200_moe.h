@@ -809,7 +809,8 @@ int b200_attention_bwd(int bwd_dt, int num_seqs, int total_q, int total_k, const
                        void *dx_v, int is_causal, uint64_t workspaceBytes, void *workspace, void *stream);
 
 /* The fused attention kernels (head_dim 64 and 128) bound every wait on a barrier to two seconds; one that runs out
- * records a code (21-26: which hand-over gave up) and the launch ends early with wrong results. Synchronises the device,
+ * records a code (which hand-over gave up: 21-26, with a window 51-60 forward, 61-72 dQ, 81-94 dK and dV) and the launch ends early
+ * with wrong results. Synchronises the device,
  * returns the recorded code through status_out (0 = none) and clears it. No counterpart in the reference. */
 int b200_attention_status(int *status_out);
 
@@ -825,7 +826,7 @@ int b200_attention_status(int *status_out);
  * bf16 only. It stands where the reference submits rms_norm_noscale per head and rope (no fused counterpart there).
  *
  * Backward: dX_q, dX_k are overwritten (and may be d_out_q / d_out_k themselves). dq_weight, dk_weight [head_dim], either
- * may be NULL: accumulate != 0 adds to them, 0 writes them. Their sums run in a fixed order (fp32 shares of the blocks in
+ * may be NULL, not the same array: accumulate != 0 adds to them, 0 writes them. Their sums run in a fixed order (fp32 shares of the blocks in
  * the workspace, then their sum): two runs give the same bits. The workspace is needed only for weight gradients;
  * b200_qk_norm_rope_bwd_workspace_bytes(num_tokens, ...) covers every smaller number of tokens too.
  */
@@ -847,7 +848,7 @@ int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int num_q_head
  * visible keys. The query ranges of the sequences must not overlap, nor, in the backward, their key ranges. Rows of
  * x_attn_out, softmax_lse, dx_q, dx_k, dx_v outside every sequence are left as they were; a key that no query sees gets a
  * zero gradient, and keys of a sequence that none of its queries sees, like rows outside the sequences, may hold anything.
- * head_dim a multiple of 8 up to 256, tensors 16-byte aligned, bf16 only. The reference has no window: no counterpart.
+ * Outputs and workspace must not overlap the inputs or one another. head_dim a multiple of 8 up to 256, tensors 16-byte aligned, bf16 only. The reference has no window: no counterpart.
  *
  * Head sizes 64 and 128 run on the tensor cores (csrc/attention_window_sm100.cu; sequences with few queries, up to 32 rows of a group, in
  * csrc/attention_window_few.cu), the others on the fp32 units. All sums have a fixed order: two runs give the same bits. Rounding as in

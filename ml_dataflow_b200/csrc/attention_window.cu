@@ -230,6 +230,22 @@ int disjoint(const char *op, const char *what, int num_seqs, const int *off, con
   return 0;
 }
 
+// The outputs, first n_out of the tensors, must lie apart from one another and from the inputs behind them: units of a launch, and the launches
+// of a backward, read rows that others have written by then.
+struct Range {
+  const void *at;
+  uint64_t bytes;
+};
+int apart(const char *op, const Range *t, int n_out, int n) {
+  for (int i = 0; i < n_out; i++)
+    for (int j = i + 1; j < n; j++) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(t[i].at), b = reinterpret_cast<uintptr_t>(t[j].at);
+      B200_REQUIRE(t[i].bytes == 0 || t[j].bytes == 0 || (a < b ? a + t[i].bytes <= b : b + t[j].bytes <= a),
+                   "%s: an output overlaps another tensor", op);
+    }
+  return 0;
+}
+
 int window_check(const char *op, int dt, int num_seqs, int total_q, int total_k, const int *q_off, const int *q_len, const int *k_off,
                  const int *k_len, int num_q_heads, int num_kv_heads, int head_dim, int window, int num_sinks) {
   B200_REQUIRE(dt == B200_DT_BF16, "%s: only bf16 is implemented (datatype code %d)", op, dt);
@@ -322,8 +338,10 @@ void fill_call(window::Call *c, int num_seqs, int total_q, int total_k, const in
   c->q_heads = num_q_heads;
   c->kv_heads = num_kv_heads;
   c->head_dim = head_dim;
-  c->window = window_;
-  c->sinks = num_sinks;
+  // More than all keys changes nothing, and positions plus these stay within 32 bits. (The sinks stay above what decides on the workspace.)
+  c->window = window_ < total_k ? window_ : total_k;
+  const int most_sinks = total_k > (1 << 20) ? total_k : 1 << 20;
+  c->sinks = num_sinks < most_sinks ? num_sinks : most_sinks;
   c->scale = 1.0f / sqrtf((float)head_dim);
   c->q = (const __nv_bfloat16 *)x_q;
   c->k = (const __nv_bfloat16 *)x_k;
@@ -346,10 +364,15 @@ extern "C" int b200_attention_window_fwd(int fwd_dt, int num_seqs, int total_q, 
   if (window_check("attention_window_fwd", fwd_dt, num_seqs, total_q, total_k, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens,
                    num_q_heads, num_kv_heads, head_dim, window, num_sinks))
     return -1;
-  if (num_seqs == 0 || total_q == 0) return 0;
+  bool any = false;
+  for (int s = 0; s < num_seqs && !any; s++) any = q_seq_lens[s] > 0;
+  if (!any) return 0;
   B200_REQUIRE(x_q && x_k && x_v && x_attn_out && softmax_lse, "attention_window_fwd: null tensor");
   B200_REQUIRE(b200_aligned16(x_q) && b200_aligned16(x_k) && b200_aligned16(x_v) && b200_aligned16(x_attn_out),
                "attention_window_fwd: tensors must be 16-byte aligned");
+  const uint64_t nq = (uint64_t)total_q * num_q_heads, nk = (uint64_t)total_k * num_kv_heads, row = (uint64_t)head_dim * 2;
+  const Range t[] = {{x_attn_out, nq * row}, {softmax_lse, nq * 4}, {x_q, nq * row}, {x_k, nk * row}, {x_v, nk * row}};
+  if (apart("attention_window_fwd", t, 2, 5)) return -1;
   window::Call c{};
   fill_call(&c, num_seqs, total_q, total_k, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens, num_q_heads, num_kv_heads, head_dim, x_q,
             x_k, x_v, window, num_sinks, stream);
@@ -368,7 +391,8 @@ extern "C" int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, 
     return -1;
   if (disjoint("attention_window_bwd", "key", num_seqs, k_seq_offsets, k_seq_lens)) return -1;
   if (num_seqs == 0 || total_k == 0) return 0;
-  B200_REQUIRE(x_q && x_k && x_v && x_attn_out && softmax_lse && dx_out && dx_q && dx_k && dx_v, "attention_window_bwd: null tensor");
+  B200_REQUIRE(x_k && x_v && dx_k && dx_v && (total_q == 0 || (x_q && x_attn_out && softmax_lse && dx_out && dx_q)),
+               "attention_window_bwd: null tensor");
   B200_REQUIRE(b200_aligned16(x_q) && b200_aligned16(x_k) && b200_aligned16(x_v) && b200_aligned16(x_attn_out) && b200_aligned16(dx_out) &&
                    b200_aligned16(dx_q) && b200_aligned16(dx_k) && b200_aligned16(dx_v),
                "attention_window_bwd: tensors must be 16-byte aligned");
@@ -376,6 +400,10 @@ extern "C" int b200_attention_window_bwd(int bwd_dt, int num_seqs, int total_q, 
   B200_REQUIRE(total_q == 0 || (workspace && b200_aligned16(workspace) && workspaceBytes >= need),
                "attention_window_bwd: the workspace holds %llu bytes, %llu are needed (b200_attention_window_workspace_bytes)",
                (unsigned long long)workspaceBytes, (unsigned long long)need);
+  const uint64_t nq = (uint64_t)total_q * num_q_heads, nk = (uint64_t)total_k * num_kv_heads, row = (uint64_t)head_dim * 2;
+  const Range t[] = {{dx_q, nq * row}, {dx_k, nk * row}, {dx_v, nk * row},       {workspace, total_q ? need : 0}, {x_q, nq * row},
+                     {x_k, nk * row},  {x_v, nk * row},  {x_attn_out, nq * row}, {softmax_lse, nq * 4},           {dx_out, nq * row}};
+  if (apart("attention_window_bwd", t, 4, 10)) return -1;
   window::Call c{};
   fill_call(&c, num_seqs, total_q, total_k, q_seq_offsets, q_seq_lens, k_seq_offsets, k_seq_lens, num_q_heads, num_kv_heads, head_dim, x_q,
             x_k, x_v, window, num_sinks, stream);

@@ -204,32 +204,34 @@ __global__ void __launch_bounds__(THREADS, BWD ? BWD_BLOCKS : FWD_BLOCKS) qk_nor
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
-  if (!BWD || p.partial == nullptr) return;
-  // the block's share of the weight gradients: slots of a warp, then warps, each in a fixed order
-  __shared__ float s_sum[WARPS][2][MAX_HEAD_DIM];
+  if constexpr (BWD) {
+    if (p.partial == nullptr) return;
+    // the block's share of the weight gradients: slots of a warp, then warps, each in a fixed order
+    __shared__ float s_sum[WARPS][2][MAX_HEAD_DIM];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    float q0, q1, k0, k1;
-    unpack2(gq[i >> 1], q0, q1);
-    unpack2(gk[i >> 1], k0, k1);
-    float q = i & 1 ? q1 : q0, k = i & 1 ? k1 : k0;
+    for (int i = 0; i < 8; i++) {
+      float q0, q1, k0, k1;
+      unpack2(gq[i >> 1], q0, q1);
+      unpack2(gk[i >> 1], k0, k1);
+      float q = i & 1 ? q1 : q0, k = i & 1 ? k1 : k0;
 #pragma unroll
-    for (int o = LANES; o < 32; o <<= 1) {
-      q += __shfl_xor_sync(0xffffffffu, q, o);
-      k += __shfl_xor_sync(0xffffffffu, k, o);
+      for (int o = LANES; o < 32; o <<= 1) {
+        q += __shfl_xor_sync(0xffffffffu, q, o);
+        k += __shfl_xor_sync(0xffffffffu, k, o);
+      }
+      if (slot == 0 && on_row) {
+        s_sum[warp][0][c * 8 + i] = q;
+        s_sum[warp][1][c * 8 + i] = k;
+      }
     }
-    if (slot == 0 && on_row) {
-      s_sum[warp][0][c * 8 + i] = q;
-      s_sum[warp][1][c * 8 + i] = k;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.head_dim; i += THREADS) {
-    const int which = i / p.head_dim, d = i - which * p.head_dim;
-    float t = 0.0f;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * p.head_dim; i += THREADS) {
+      const int which = i / p.head_dim, d = i - which * p.head_dim;
+      float t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) t += s_sum[w][which][d];
-    p.partial[(int64_t)blockIdx.x * 2 * p.head_dim + i] = t;
+      for (int w = 0; w < WARPS; w++) t += s_sum[w][which][d];
+      p.partial[(int64_t)blockIdx.x * 2 * p.head_dim + i] = t;
+    }
   }
 }
 
@@ -385,6 +387,9 @@ extern "C" int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int
                  k_weight, X_q, X_k, dX_q, dX_k))
     return -1;
   const bool want_dw = dq_weight != nullptr || dk_weight != nullptr;
+  // one vector for both would be written by two threads
+  const uintptr_t wa = reinterpret_cast<uintptr_t>(dq_weight), wb = reinterpret_cast<uintptr_t>(dk_weight), wn = (uintptr_t)head_dim * 2;
+  B200_REQUIRE(!wa || !wb || (wa < wb ? wa + wn <= wb : wb + wn <= wa), "qk_norm_rope_bwd: dq_weight and dk_weight overlap");
   if (num_tokens == 0) {  // the sums over no tokens
     if (dq_weight && !accumulate) B200_CUDA(cudaMemsetAsync(dq_weight, 0, (size_t)head_dim * 2, (cudaStream_t)stream));
     if (dk_weight && !accumulate) B200_CUDA(cudaMemsetAsync(dk_weight, 0, (size_t)head_dim * 2, (cudaStream_t)stream));

@@ -66,6 +66,33 @@ def test_attention_window_refusals():
         assert bwd(**b) == -1, b
 
 
+def test_overlapping_outputs_are_refused(capfd):
+    """Outputs over inputs or one another; weight gradients in one array."""
+    lib = _lib()
+    at = lambda i: ctypes.c_void_p((i + 1) << 20)  # 1 MB apart, more than any of these tensors
+    error = lambda: capfd.readouterr().err
+    one, n8 = _ints(0), _ints(8)
+
+    def fwd(**same):
+        a = {n: at(i) for i, n in enumerate(("q", "k", "v", "o", "lse"))}
+        a |= {n: a[m] for n, m in same.items()}
+        return lib.b200_attention_window_fwd(BF, 1, 8, 8, one, n8, one, n8, 2, 1, 128, a["q"], a["k"], a["v"], a["o"], a["lse"], 4, 0, None)
+
+    def bwd(**same):
+        a = {n: at(i) for i, n in enumerate(("q", "k", "v", "o", "lse", "do", "dq", "dk", "dv", "ws"))}
+        a |= {n: a[m] for n, m in same.items()}
+        return lib.b200_attention_window_bwd(BF, 1, 8, 8, one, n8, one, n8, 2, 1, 128, a["q"], a["k"], a["v"], a["o"], a["lse"], a["do"], a["dq"],
+                                             a["dk"], a["dv"], 4, 0, 1 << 40, a["ws"], None)
+
+    for call, pairs in ((fwd, (("o", "q"), ("o", "v"), ("lse", "o"), ("lse", "k"))),
+                        (bwd, (("dq", "q"), ("dq", "do"), ("dk", "k"), ("dv", "dk"), ("dk", "dq"), ("ws", "dv"), ("ws", "lse"), ("dv", "o")))):
+        for a, b in pairs:
+            assert call(**{a: b}) == -1 and "overlaps" in error(), (a, b)
+    assert lib.b200_qk_norm_rope_bwd(BF, BF, 4, 2, 1, 64, 1e-5, 10000, at(0), None, None, at(1), at(2), at(3), at(4), at(5), at(6), at(7),
+                                     ctypes.c_void_p((8 << 20) + 64), 1, 1 << 30, at(9), None) == -1
+    assert "overlap" in error()
+
+
 def test_attention_window_workspace_covers_smaller_batches():
     ws = _lib().b200_attention_window_workspace_bytes
     assert ws(0, 4, 2, 128, 10, 0) == ws(1, 0, 2, 128, 10, 0) == ws(1, 4, 2, 128, 0, 0) == ws(1, 4, 2, 128, 5, -1) == 0

@@ -244,3 +244,40 @@ def test_gradient_against_differences():
     # a gradient carries its own rounding and those of the probabilities, dS and the output that delta is formed from: three more of
     # like size; independent signs, six standard deviations
     assert abs(terms.sum().item() - want) <= 6 * 2 * HALF * terms.norm().item()
+
+
+@pytest.mark.parametrize("hd", [128, 64, 40])
+def test_more_window_or_sinks_than_there_are_keys(hd):
+    """The largest numbers that the arguments take: every key before a query is seen, as with a window of the whole sequence."""
+    import torch
+
+    from operator_reference import window_attention
+
+    q_lens, k_lens, hq, hkv = [400, 2, 90], [520, 300, 90], 4, 2
+    q_offs, k_offs, q, k, v, do = _setup(q_lens, k_lens, hq, hkv, hd, 0, 0, 5)
+    run = lambda w, s: _run(q_offs, q_lens, k_offs, k_lens, hq, hkv, hd, q, k, v, do, w, s)
+    want = run(520, 0)
+    for w, s in ((2 ** 31 - 1, 2 ** 31 - 1), (520, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 100)):
+        got = run(w, s)
+        assert all(torch.equal(got[n], want[n]) for n in want), (w, s)
+    got, args = run(1, 2 ** 31 - 1), (q_offs, q_lens, k_offs, k_lens, hq, hkv, hd, q, k, v)  # sinks only
+    _compare(got, window_attention(*args, 1, 2 ** 31 - 1, do, got["o"]))
+
+
+@pytest.mark.parametrize("hd", [128, 32])
+def test_sequences_without_queries(hd):
+    """No query at all: nothing is written forward, keys and values get zeros."""
+    import torch
+
+    hq, hkv = 4, 2
+    for q_lens, k_lens, pad in (([0, 0], [130, 7], 0), ([0, 0], [130, 7], 5)):
+        k_offs, tk = _offs(k_lens, 2)
+        q = torch.full((pad, hq * hd), math.nan, dtype=torch.bfloat16, device="cuda")
+        k = torch.randn((tk, hkv * hd), device="cuda").to(torch.bfloat16)
+        got = _run([0, 0], q_lens, k_offs, k_lens, hq, hkv, hd, q, k, k.clone(), q.clone(), 9, 3)
+        inside = torch.zeros(tk, dtype=torch.bool, device="cuda")
+        for o, n in zip(k_offs, k_lens):
+            inside[o:o + n] = True
+        assert torch.all(got["o"] == 7.0) and torch.all(got["lse"] == 7.0) and torch.all(got["dq"] == 7.0)
+        for n in ("dk", "dv"):
+            assert torch.all(got[n][inside] == 0) and torch.all(got[n][~inside] == 7.0), n
