@@ -15,7 +15,8 @@
 // share a scale block, and the maximum costs two shuffles; two groups of eight per thread are in flight. What bounds them besides
 // memory is the number of instructions: hence arithmetic on pairs, the special-function units' reciprocal in the sigmoid (2^-22
 // relative, far below the outputs' 2^-9), special values looked for once per group, and no index divisions where the columns are whole
-// scale blocks.
+// scale blocks. Measured at 65536 x 1408, 744 MB a call: h and the codes 126 us (5.9 TB/s), x1, x3 and h restored 117 us (6.4), the
+// backward's two gradients 116 us (6.4); a plain copy reaches 6.5.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -326,7 +327,8 @@ int act8_codes_ok(const char *op, const void *c1, const void *e1, const void *c3
 int act8_grid(int64_t units) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t want = (units + act8::THREADS * act8::UNROLL - 1) / (act8::THREADS * act8::UNROLL), most = (int64_t)sms * 32;
+  const int64_t want = (units + act8::THREADS * act8::UNROLL - 1) / (act8::THREADS * act8::UNROLL), most = (int64_t)sms * 64;
+  // four blocks run on an SM: at 16 times as many the last ones end together (at 8 times, 2 % more time; at one, 2 to 16 %)
   return (int)(want < most ? want : most);
 }
 

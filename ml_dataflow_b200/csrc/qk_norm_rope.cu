@@ -15,6 +15,8 @@
 // warp at a time), so that the sums are shuffles. A warp takes a token and runs over its heads in rounds of a few warp-wide
 // vectors. Bound by memory, 4 bytes per element forward, 6 backward: to keep enough of it in flight every lane copies the
 // vectors of the next two rounds into places of its own in shared memory (cp.async; registers hold no more than one round).
+// Measured with 16 + 4 heads of 128: 8192 tokens forward 18 us, backward 32 us and 5 for the weights' join; 65536 tokens 110 us (6.1 TB/s)
+// and 180 us (5.6 TB/s).
 #include <math.h>
 
 #include "common.cuh"
