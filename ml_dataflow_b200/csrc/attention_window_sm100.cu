@@ -1,7 +1,7 @@
 // Windowed attention with sinks on the tensor cores, head sizes 64 and 128.
 //
 // Forward. A work unit is a pair of 128-row query tiles that read the same keys: two query heads of one key/value head over
-// the same rows (or, where the group is odd, two neighbouring tiles of one head). Key blocks of 128 that no row of the pair
+// the same rows (or, where the group is odd, two neighbouring tiles of one head); in the last round, one of them. Key blocks of 128 that no row of the pair
 // sees are never touched: the unit walks the blocks that hold sinks, then those of its window. A persistent CTA (one per SM)
 // takes units in turn: while one unit's last products and its output are under way, the next one's queries and keys load.
 //   warp 0     TMA loads: the query tiles, and K_0, K_1, V_0, K_2, V_1, ... through a ring, in the order they are used
@@ -22,7 +22,7 @@
 // What bounds it: neither unit alone. A 128 x 128 x 128 product takes 727 cycles (both operands from shared memory), so a step of a pair has
 // 2900 cycles of tensor work and 2 x 128 x 128 exponentials (2050 cycles of the special-function units); a step takes 4000: products and
 // exponentials of the two tiles alternate, but the waits between them (250 cycles each) stay. Measured with 16 query heads on 4 of 128 and 8192
-// tokens: window 1024 100 us (65 GFLOP of visible pairs: 650 TFLOP/s; 86 with the masked parts of the blocks), window 4096 203 us, no window 250 us (1100 TFLOP/s;
+// tokens: window 1024 97 us (65 GFLOP of visible pairs: 670 TFLOP/s; 86 with the masked parts of the blocks), window 4096 203 us, no window 250 us (1100 TFLOP/s;
 // the causal kernel without windows 330 us). Tried and slower: the second half of the scores' rows on 8 more warps that exchange maxima (127 us),
 // sink blocks in a form of 32 columns (their step is shorter, the others' longer: 107 us).
 //
@@ -65,6 +65,7 @@ struct FwdParams {
   __nv_bfloat16 *O;
   float *lse;  // [q_heads][total_q]
   int window, sinks, group, q_heads, total_q, pair_heads, units;
+  int whole;  // units from this one on are one tile of a pair each
   float scale;
   int *status;
 };
@@ -120,6 +121,8 @@ __device__ __forceinline__ Tile tile_of(const Span &sp, int window, int h, int r
 }
 __device__ __forceinline__ Unit unit_of(const FwdParams &p, int unit) {
   Unit u;
+  const int half = unit < p.whole ? 0 : 1 + ((unit - p.whole) & 1);  // 1, 2: the pair's first tile, its second
+  if (half) unit = p.whole + ((unit - p.whole) >> 1);
   int s = 0;
   while (unit >= p.seqs.first[s + 1]) s++;
   u.sp = span_of(p.seqs, s);
@@ -133,9 +136,13 @@ __device__ __forceinline__ Unit unit_of(const FwdParams &p, int unit) {
     u.a = tile_of(u.sp, p.window, rel % p.q_heads, row);
     u.b = tile_of(u.sp, p.window, rel % p.q_heads, row + TILE);
   }
+  if (half) {
+    if (half == 2) u.a = u.b;
+    u.b.exists = false;
+  }
   u.first = u.a.lo;
   u.n_sink = min((p.sinks + TILE - 1) / TILE, u.first);
-  u.n = u.n_sink + (u.b.exists ? u.b.hi : u.a.hi) - u.first + 1;
+  u.n = u.a.exists ? u.n_sink + (u.b.exists ? u.b.hi : u.a.hi) - u.first + 1 : 0;  // a second tile that is not there
   return u;
 }
 
@@ -443,7 +450,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
     const uint32_t p_addr = ptx::smem_u32(sP + g * Sh::P_TILE + trow * 128);
     const float c = p.scale * LOG2E;
     uint32_t t = 0;  // steps of this tile so far
-    if (g == 1 && !wait(&st->p_ready[0], 0, ST_P)) goto teardown;  // the first tile of a CTA's first unit always exists
+    if (g == 1 && unit_of(p, unit_at(0)).b.exists && !wait(&st->p_ready[0], 0, ST_P)) goto teardown;
     for (int round = 0, unit = unit_at(0); unit < p.units; unit = unit_at(++round)) {
       const Unit u = unit_of(p, unit);
       const Tile x = g ? u.b : u.a;
@@ -1531,6 +1538,12 @@ int sm100_fwd(const Call &c) {
         },
         [&](int s) { return blocks_seen(c, s, c.k_len[s]); });
     if (p.units == 0) continue;
+    // In the last round, pairs are given to two CTAs as long as there are CTAs without one (8192 tokens, window 1024, 512 pairs: 103 -> 97
+    // us; 400 tokens of 8 heads, 16 pairs: 14 -> 11). Not where the units of a long sequence run from one block to all: the last round's are
+    // its short ones, and two halves take longer than a pair (no window: 246 -> 250 us).
+    const int last = p.units % d.sms, split = p.units > d.sms && c.window > p.seqs.Tk[0] / 2 ? 0 : (last < d.sms - last ? last : d.sms - last);
+    p.whole = p.units - split;
+    p.units += split;
     if (c.head_dim == 128 ? launch_fwd<128>(p, d, c.stream) : launch_fwd<64>(p, d, c.stream)) return -1;
   }
   return 0;
