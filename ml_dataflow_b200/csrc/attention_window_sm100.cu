@@ -31,6 +31,8 @@
 #include <math.h>
 #include <stddef.h>
 
+#include <algorithm>
+
 #include "attention_sm100.cuh"
 #include "attention_window.cuh"
 #include "common.cuh"
@@ -59,9 +61,45 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 enum { ST_Q_EMPTY = 51, ST_KV_EMPTY, ST_Q_FULL, ST_KV_FULL, ST_S_FREE, ST_P, ST_O_FREE, ST_S, ST_PV, ST_FIX };
 
+// Which units a persistent CTA takes, one after the other.
+// Without a schedule: c, 2 G - 1 - c, 2 G + c, ... for G CTAs; units are numbered from the longest of a sequence on, so that a CTA that took a
+// long one of a round takes a short one of the next.
+// The forward of several sequences: the host deals the units out, the longest first, each to the CTA with the least work so far, and writes that
+// down in runs: CTAs cta .. cta + n - 1 take units unit .. unit + n - 1. (16 heads on 4 of 128: eight sequences of 1024 tokens, window 512, 68 -> 59
+// us; six of 700 to 2000, no window, 94 -> 79; the three chunks of prompts 61.5 -> 59.6. One sequence has nothing to gain, and the longer walk
+// costs it 2 %, hence two kernels; dQ gained nothing.)
+constexpr int MAX_RUNS = 160;
+struct Schedule {
+  int n;
+  struct Run {
+    int unit;
+    unsigned short cta, n;
+  } run[MAX_RUNS];
+};
+__device__ __forceinline__ int unit_at(int round) {
+  return (round & 1) ? (round + 1) * (int)gridDim.x - 1 - (int)blockIdx.x : round * (int)gridDim.x + (int)blockIdx.x;
+}
+template <bool DEALT>
+struct Walk {
+  int at = 0;
+  // the CTA's next unit; `units` or more: no more
+  __device__ __forceinline__ int next(const Schedule &s, int units) {
+    if constexpr (!DEALT) {
+      return unit_at(at++);
+    } else {
+      while (at < s.n) {
+        const Schedule::Run r = s.run[at++];
+        if ((unsigned)((int)blockIdx.x - r.cta) < (unsigned)r.n) return r.unit + (int)blockIdx.x - r.cta;
+      }
+      return units;
+    }
+  }
+};
+
 struct FwdParams {
   CUtensorMap tmQ, tmK, tmV;  // [rows][heads * HD] bf16, boxes of 64 columns x 128 rows, 128-byte swizzle
   SeqTable seqs;
+  Schedule schedule;
   __nv_bfloat16 *O;
   float *lse;  // [q_heads][total_q]
   int window, sinks, group, q_heads, total_q, pair_heads, units;
@@ -83,17 +121,11 @@ struct FwdShape {
   static_assert(smem <= 232448, "more shared memory than a CTA can be given");
 };
 
-// The units of a persistent CTA: c, 2 G - 1 - c, 2 G + c, ... for G CTAs. Units are numbered from the longest of a sequence on, so
-// that a CTA that took a long one of a round takes a short one of the next.
-__device__ __forceinline__ int unit_at(int round) {
-  return (round & 1) ? (round + 1) * (int)gridDim.x - 1 - (int)blockIdx.x : round * (int)gridDim.x + (int)blockIdx.x;
-}
-
 // Which keys a sequence's rows see.
 struct Span {
   int q_off, Tq, k_off, Tk, shift;
 };
-__device__ __forceinline__ Span span_of(const SeqTable &t, int s) {
+__host__ __device__ __forceinline__ Span span_of(const SeqTable &t, int s) {
   return Span{t.q_off[s], t.Tq[s], t.k_off[s], t.Tk[s], t.Tk[s] - t.Tq[s]};
 }
 
@@ -110,7 +142,7 @@ struct Unit {
   int n, n_sink, first;
   __device__ __forceinline__ int block(int i) const { return i < n_sink ? i : first + i - n_sink; }
 };
-__device__ __forceinline__ Tile tile_of(const Span &sp, int window, int h, int row) {
+__host__ __device__ __forceinline__ Tile tile_of(const Span &sp, int window, int h, int row) {
   Tile t;
   t.h = h;
   t.row = row;
@@ -119,7 +151,7 @@ __device__ __forceinline__ Tile tile_of(const Span &sp, int window, int h, int r
   t.exists = row < sp.Tq;
   return t;
 }
-__device__ __forceinline__ Unit unit_of(const FwdParams &p, int unit) {
+__host__ __device__ __forceinline__ Unit unit_of(const FwdParams &p, int unit) {
   Unit u;
   const int half = unit < p.whole ? 0 : 1 + ((unit - p.whole) & 1);  // 1, 2: the pair's first tile, its second
   if (half) unit = p.whole + ((unit - p.whole) >> 1);
@@ -251,7 +283,7 @@ __device__ __forceinline__ void zero_dead(uint32_t tile, const Span &sp, int kb,
   }
 }
 
-template <int HD>
+template <int HD, bool DEALT>
 __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid_constant__ FwdParams p) {
   using Sh = FwdShape<HD>;
   constexpr int SLOTS = Sh::SLOTS;
@@ -337,7 +369,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
       auto load_last_v = [&]() {
         load(&p.tmV, v_at(t - 1), last_sp, last_kvh, last_kb, has_dead(last_sp, last_kb, p.window, p.sinks));
       };
-      for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
+      Walk<DEALT> walk;
+      for (int unit = walk.next(p.schedule, p.units); ok && unit < p.units; unit = walk.next(p.schedule, p.units)) {
         const Unit u = unit_of(p, unit);
         const int kvh = u.a.h / p.group;
         for (int i = 0; ok && i < u.n; i++) {
@@ -371,7 +404,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         const uint32_t q_base = ptx::smem_u32(sQ), kv_base = ptx::smem_u32(sKV);
         uint32_t t = 0, uq[2] = {0, 0}, ts[2] = {0, 0};  // steps; units and S products of either tile
         bool ok = true;
-        for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
+        Walk<DEALT> walk;
+        for (int unit = walk.next(p.schedule, p.units); ok && unit < p.units; unit = walk.next(p.schedule, p.units)) {
           const Unit u = unit_of(p, unit);
           if (u.a.exists) ok = wait(&st->q_full[0], uq[0]++, ST_Q_FULL);
           if (ok && u.b.exists) ok = wait(&st->q_full[1], uq[1]++, ST_Q_FULL);
@@ -410,7 +444,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         const uint32_t p_base = ptx::smem_u32(sP + g * Sh::P_TILE), kv_base = ptx::smem_u32(sKV), o_col = tmem_base + COL_O + (uint32_t)(g * HD);
         uint32_t t = 0, units = 0, tp = 0;  // steps; units and products of this tile
         bool ok = true;
-        for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round)) {
+        Walk<DEALT> walk;
+        for (int unit = walk.next(p.schedule, p.units); ok && unit < p.units; unit = walk.next(p.schedule, p.units)) {
           const Unit u = unit_of(p, unit);
           const Tile x = g ? u.b : u.a;
           bool begun = false;
@@ -450,8 +485,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
     const uint32_t p_addr = ptx::smem_u32(sP + g * Sh::P_TILE + trow * 128);
     const float c = p.scale * LOG2E;
     uint32_t t = 0;  // steps of this tile so far
-    if (g == 1 && unit_of(p, unit_at(0)).b.exists && !wait(&st->p_ready[0], 0, ST_P)) goto teardown;
-    for (int round = 0, unit = unit_at(0); unit < p.units; unit = unit_at(++round)) {
+    if (g == 1 && unit_of(p, Walk<DEALT>().next(p.schedule, p.units)).b.exists && !wait(&st->p_ready[0], 0, ST_P)) goto teardown;
+    Walk<DEALT> walk;
+    for (int unit = walk.next(p.schedule, p.units); unit < p.units; unit = walk.next(p.schedule, p.units)) {
       const Unit u = unit_of(p, unit);
       const Tile x = g ? u.b : u.a;
       if (!x.exists) continue;
@@ -1374,14 +1410,66 @@ int tile_map(CUtensorMap *m, const void *base, int rows, uint64_t cols, int head
   return 0;
 }
 
-template <int HD>
-int launch_fwd(window::FwdParams &p, const Device &d, cudaStream_t s) {
+// Deals the units of a launch out to `ctas` CTAs; no runs where there are too many, or nothing to deal. cost(unit) in any measure; next(unit): the
+// first unit behind it that may cost something else.
+template <typename F, typename G>
+void deal(window::Schedule *s, int sequences, int units, int ctas, F cost, G next) {
+  constexpr int MAX_CLASSES = 128;
+  struct Class {
+    int cost, unit, n;
+  } cls[MAX_CLASSES];
+  struct Group {  // CTAs cta .. cta + n - 1 have the same load
+    int load, cta, n;
+  } grp[MAX_CLASSES + window::MAX_RUNS];
+  s->n = 0;
+  if (units <= ctas || sequences == 1) return;
+  int classes = 0;
+  for (int unit = 0; unit < units;) {
+    const int end = next(unit), c = cost(unit);
+    if (classes > 0 && cls[classes - 1].cost == c && cls[classes - 1].unit + cls[classes - 1].n == unit) {
+      cls[classes - 1].n += end - unit;
+    } else {
+      if (classes == MAX_CLASSES) return;
+      cls[classes++] = Class{c, unit, end - unit};
+    }
+    unit = end;
+  }
+  std::stable_sort(cls, cls + classes, [](const Class &a, const Class &b) { return a.cost > b.cost; });
+  int groups = 1, runs = 0;
+  grp[0] = Group{0, 0, ctas};
+  for (int i = 0; i < classes; i++)
+    while (cls[i].n > 0) {
+      int least = 0;
+      for (int g = 1; g < groups; g++)
+        if (grp[g].load < grp[least].load) least = g;
+      Group &from = grp[least];
+      const int n = from.n < cls[i].n ? from.n : cls[i].n;
+      if (runs == window::MAX_RUNS) return;
+      s->run[runs++] = window::Schedule::Run{cls[i].unit, (unsigned short)from.cta, (unsigned short)n};
+      cls[i].unit += n;
+      cls[i].n -= n;
+      const Group to = {from.load + cls[i].cost, from.cta, n};
+      from.cta += n;
+      from.n -= n;
+      if (from.n == 0) from = to;
+      else grp[groups++] = to;
+    }
+  s->n = runs;
+}
+
+template <int HD, bool DEALT>
+int launch_fwd(const window::FwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
   constexpr size_t smem = window::FwdShape<HD>::smem;
-  if (allow_smem(window::window_fwd_kernel<HD>, smem, &done[d.dev])) return -1;
-  B200_CUDA(b200_launch_overlapped(window::window_fwd_kernel<HD>, dim3(p.units < d.sms ? p.units : d.sms), dim3(window::FWD_THREADS), smem, s, 1, p));
+  if (allow_smem(window::window_fwd_kernel<HD, DEALT>, smem, &done[d.dev])) return -1;
+  B200_CUDA(b200_launch_overlapped(window::window_fwd_kernel<HD, DEALT>, dim3(p.units < d.sms ? p.units : d.sms), dim3(window::FWD_THREADS), smem, s, 1,
+                                   p));
   B200_CHECK_LAUNCH("attention_window_fwd");
   return 0;
+}
+template <int HD>
+int launch_fwd(const window::FwdParams &p, const Device &d, cudaStream_t s) {
+  return p.schedule.n > 0 ? launch_fwd<HD, true>(p, d, s) : launch_fwd<HD, false>(p, d, s);
 }
 
 template <int HD>
@@ -1544,6 +1632,20 @@ int sm100_fwd(const Call &c) {
     const int last = p.units % d.sms, split = p.units > d.sms && c.window > p.seqs.Tk[0] / 2 ? 0 : (last < d.sms - last ? last : d.sms - last);
     p.whole = p.units - split;
     p.units += split;
+    // in quarters of a pair's step: a single tile's step takes three, a unit's begin and end five
+    deal(
+        &p.schedule, p.seqs.n, p.units, d.sms,
+        [&](int unit) {
+          const window::Unit u = window::unit_of(p, unit);
+          return u.n * (u.b.exists ? 4 : 3) + 5;
+        },
+        [&](int unit) {
+          if (unit >= p.whole) return unit + 1;
+          int s = 0;
+          while (unit >= p.seqs.first[s + 1]) s++;
+          const int row = p.pair_heads ? c.q_heads / 2 : c.q_heads, end = p.seqs.first[s] + ((unit - p.seqs.first[s]) / row + 1) * row;
+          return end < p.whole ? end : p.whole;
+        });
     if (c.head_dim == 128 ? launch_fwd<128>(p, d, c.stream) : launch_fwd<64>(p, d, c.stream)) return -1;
   }
   return 0;
