@@ -599,12 +599,13 @@ teardown:
 // query rows on the tensor-memory lanes, so that a thread's log-sum-exp and delta are its own two numbers.
 //
 // dQ: one query tile of one head per unit, persistent CTAs. Per key block
-//     S = Q K^T,  dP = dO V^T,   dS = P o (dP - delta) as bf16 through shared memory,   dQ += dS K
+//     S = Q K^T,  dP = dO V^T,   dS = P o (dP - delta) as bf16 through tensor memory,   dQ += dS K
 // S and dP of a block are issued while the threads still work on the block before, and a unit's first products before the last
 // unit's dQ is finished. delta = rowsum(dO o O) is formed here, in fp32, and written for the other kernel. Four warps of their own
-// form it for the next unit and write the last one's dQ (two accumulators in tensor memory): with these in the computing
-// threads' way a unit of ten blocks spent 10 of its 43 thousand cycles between the blocks. K is needed from S to dQ, V for dP only:
-// three slots of shared memory for K, one for V.
+// form it for the next unit and write the last one's dQ: with these in the computing threads' way a unit of ten blocks spent 10 of its 43
+// thousand cycles between the blocks. dS lies in tensor memory, where the product takes its rows from, in two places by turns: through shared
+// memory, which bounds this kernel, 8 % more time, though tensor memory then held an accumulator for the next unit. K is needed from S to dQ, V
+// for dP only: three slots of shared memory for K, two for V.
 //
 // dK, dV: one block of 128 keys of one key/value head per unit; it walks the query heads of the group and the query tiles that see
 // its keys, K and V stay in shared memory. Per tile
@@ -648,15 +649,16 @@ struct BwdParams {
 template <int HD>
 struct BwdQShape {
   static constexpr int Q_TILE = TILE * HD * 2, KV_TILE = TILE * HD * 2;
-  static constexpr int KS = HD == 128 ? 3 : 5, VS = HD == 128 ? 1 : 3;
+  static constexpr int KS = HD == 128 ? 3 : 5, VS = HD == 128 ? 2 : 3;
+  static constexpr int ACCS = 128 / HD;  // accumulators
   struct Tail {
-    uint64_t q_full, q_empty, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full, s_read, dp_full, dp_read, ds_ready, dq_done, acc_full[2],
-        acc_empty[2], stat_full[2], stat_empty[2], fixed;
+    uint64_t q_full, q_empty, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full, s_read, dp_full, dp_read, ds_ready[2], dq_done[2], acc_full[ACCS],
+        acc_empty[ACCS], stat_full[2], stat_empty[2], fixed;
     uint32_t tmem_base;
     int abort_flag;
     float delta[2][TILE];  // of even and odd units
   };
-  static constexpr size_t smem = 1024 + 2 * (size_t)Q_TILE + DS_TILE + (KS + VS) * (size_t)KV_TILE + sizeof(Tail);
+  static constexpr size_t smem = 1024 + 2 * (size_t)Q_TILE + (KS + VS) * (size_t)KV_TILE + sizeof(Tail);
   static_assert(smem <= 232448, "more shared memory than a CTA can be given");
 };
 
@@ -682,11 +684,12 @@ __device__ __forceinline__ QUnit q_unit_of(const BwdParams &p, int unit) {
 template <int HD>
 __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __grid_constant__ BwdParams p) {
   using Sh = BwdQShape<HD>;
-  constexpr int KS = Sh::KS, VS = Sh::VS;
-  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256;  // dQ of even and odd units: 128 columns each
+  constexpr int KS = Sh::KS, VS = Sh::VS, ACCS = Sh::ACCS;
+  // dQ: an accumulator of 128 columns or two of 64; dS of even and odd steps as bf16, 64 columns each
+  constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_DP = 128, COL_DQ = 256, COL_DS = 384;
   extern __shared__ unsigned char window_smem[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(window_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  unsigned char *sQ = smem, *sDO = sQ + Sh::Q_TILE, *sDS = sDO + Sh::Q_TILE, *sK = sDS + DS_TILE, *sV = sK + KS * Sh::KV_TILE;
+  unsigned char *sQ = smem, *sDO = sQ + Sh::Q_TILE, *sK = sDO + Sh::Q_TILE, *sV = sK + KS * Sh::KV_TILE;
   auto *st = reinterpret_cast<typename Sh::Tail *>(sV + VS * Sh::KV_TILE);
   volatile int *abort_flag = &st->abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -710,11 +713,13 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
     ptx::mbar_init(bar(&st->s_read), 512);
     ptx::mbar_init(bar(&st->dp_full), 1);
     ptx::mbar_init(bar(&st->dp_read), 512);
-    ptx::mbar_init(bar(&st->ds_ready), 512);
-    ptx::mbar_init(bar(&st->dq_done), 1);
-    for (int s = 0; s < 2; s++) {
+    for (int s = 0; s < ACCS; s++) {
       ptx::mbar_init(bar(&st->acc_full[s]), 1);
       ptx::mbar_init(bar(&st->acc_empty[s]), TILE);
+    }
+    for (int s = 0; s < 2; s++) {
+      ptx::mbar_init(bar(&st->ds_ready[s]), 512);
+      ptx::mbar_init(bar(&st->dq_done[s]), 1);
       ptx::mbar_init(bar(&st->stat_full[s]), TILE);
       ptx::mbar_init(bar(&st->stat_empty[s]), 512);
     }
@@ -820,25 +825,25 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
       // ================= dQ += dS K =================
       if (lane == 0) {
         const uint32_t idesc = ptx::make_idesc_bf16(TILE, HD, 0, 1);  // K is read with its head dimension contiguous
-        const uint32_t ds_base = ptx::smem_u32(sDS), k_base = ptx::smem_u32(sK);
+        const uint32_t k_base = ptx::smem_u32(sK);
         uint32_t t = 0, units = 0;
         bool ok = true;
         for (int round = 0, unit = unit_at(0); ok && unit < p.units; unit = unit_at(++round), units++) {
           const int steps = q_unit_of(p, unit).n;
-          const uint32_t acc = units & 1;
-          // the unit before the last one has been read out of this accumulator
-          if (units > 1) ok = wait(&st->acc_empty[acc], units / 2 - 1, ST_BQ_ACC);
+          const uint32_t acc = units % ACCS;
+          // the unit before in this accumulator has been read out
+          if (units >= ACCS) ok = wait(&st->acc_empty[acc], units / ACCS - 1, ST_BQ_ACC);
           for (int i = 0; ok && i < steps; i++, t++) {
             const uint32_t slot = t % KS;
-            if (!(ok = wait(&st->ds_ready, t, ST_BQ_DS))) break;
+            if (!(ok = wait(&st->ds_ready[t & 1], t / 2, ST_BQ_DS))) break;
             if (!(ok = wait(&st->k_full[slot], t / KS, ST_BQ_KV_FULL))) break;
             ptx::tc_fence_after();
-            const uint64_t ad = tile_desc(ds_base, 0), bd = tile_desc(k_base + slot * Sh::KV_TILE, SLAB);
+            const uint64_t bd = tile_desc(k_base + slot * Sh::KV_TILE, SLAB);
 #pragma unroll
             for (int k16 = 0; k16 < TILE / 16; k16++)
-              ptx::umma_bf16(tmem_base + COL_DQ + acc * TILE, desc_at(ad, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)),
-                             desc_at(bd, (uint32_t)(k16 * 2048)), idesc, i > 0 || k16 > 0);
-            ptx::umma_commit(bar(&st->dq_done));
+              ptx::umma_bf16_ts(tmem_base + COL_DQ + acc * HD, tmem_base + COL_DS + (t & 1) * 64 + k16 * 8, desc_at(bd, (uint32_t)(k16 * 2048)), idesc,
+                                i > 0 || k16 > 0);
+            ptx::umma_commit(bar(&st->dq_done[t & 1]));
             ptx::umma_commit(bar(&st->k_empty[slot]));
             if (i == steps - 1) ptx::umma_commit(bar(&st->acc_full[acc]));
           }
@@ -898,15 +903,16 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
       const QUnit u = q_unit_of(p, unit);
       const int row = u.x.row + trow;
       __nv_bfloat16 *o = p.dq + ((int64_t)(u.sp.q_off + row) * p.q_heads + u.x.h) * HD;
-      if (!wait(&st->acc_full[units & 1], units / 2, ST_BQ_DQ)) goto teardown;
+      const uint32_t acc = units % ACCS;
+      if (!wait(&st->acc_full[acc], units / ACCS, ST_BQ_DQ)) goto teardown;
       ptx::tc_fence_after();
 #pragma unroll
       for (int q = 0; q < HD / 32; q++) {
         uint32_t r[32];
-        load_columns<32>(lane_addr + COL_DQ + (units & 1) * TILE + q * 32, r);
+        load_columns<32>(lane_addr + COL_DQ + acc * HD + q * 32, r);
         if (q == HD / 32 - 1) {
           ptx::tc_fence_before();
-          arrive(&st->acc_empty[units & 1]);
+          arrive(&st->acc_empty[acc]);
         }
         if (row < u.sp.Tq) {
           store16(o + q * 32, r, p.scale);
@@ -920,8 +926,7 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
     // ================= element-wise work: a thread per (query row, quarter of the columns) =================
     const int quarter = warp & 3, cols = (warp - 8) >> 2;  // columns 32 * cols ...
     const int trow = quarter * 32 + lane;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + cols * 32;
-    const uint32_t ds_addr = ptx::smem_u32(sDS + (cols >> 1) * SLAB + trow * 128);
+    const uint32_t lane_row = tmem_base + ((uint32_t)(quarter * 32) << 16), lane_addr = lane_row + cols * 32;
     const float c = p.scale * LOG2E;
     uint32_t t = 0, units = 0;
     for (int round = 0, unit = unit_at(0); unit < p.units; unit = unit_at(++round), units++) {
@@ -953,12 +958,16 @@ __global__ void __launch_bounds__(BWD_Q_THREADS, 1) window_bwd_q_kernel(const __
 #pragma unroll
           for (int j = 0; j < 32; j++) d[j] = (see >> j) & 1u ? d[j] : 0u;
         }
-        // the product of the step before has read dS
-        if (t > 0 && !wait(&st->dq_done, t - 1, ST_BQ_DQ)) goto teardown;
-        store_chunks<4>(ds_addr, trow, (cols & 1) * 4, d);
-        ptx::fence_proxy_async_smem();
+        uint32_t ds[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) ds[j] = pack_bf16(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
+        // the product of the step before the last has read these columns
+        if (t > 1 && !wait(&st->dq_done[t & 1], t / 2 - 1, ST_BQ_DQ)) goto teardown;
+        ptx::tc_fence_after();
+        ptx::tmem_st16(lane_row + COL_DS + (t & 1) * 64 + cols * 16, ds);
+        ptx::tmem_st_wait();
         ptx::tc_fence_before();
-        arrive(&st->ds_ready);
+        arrive(&st->ds_ready[t & 1]);
       }
     }
   }
