@@ -110,7 +110,8 @@ struct FwdParams {
 
 template <int HD>
 struct FwdShape {
-  static constexpr int Q_TILE = TILE * HD * 2, P_TILE = TILE * TILE * 2, KV_TILE = TILE * HD * 2;
+  static constexpr bool P_IN_TMEM = HD == 64;  // where 128 of its columns are free
+  static constexpr int Q_TILE = TILE * HD * 2, P_TILE = P_IN_TMEM ? 0 : TILE * TILE * 2, KV_TILE = TILE * HD * 2;
   static constexpr int SLOTS = HD == 128 ? 3 : 6;
   struct Tail {
     uint64_t q_full[2], q_empty[2], kv_full[SLOTS], kv_empty[SLOTS], s_full[2], s_read[2], p_ready[2], pv_done[2], o_empty[2], fixed;
@@ -287,7 +288,8 @@ template <int HD, bool DEALT>
 __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid_constant__ FwdParams p) {
   using Sh = FwdShape<HD>;
   constexpr int SLOTS = Sh::SLOTS;
-  constexpr uint32_t TMEM_COLS = 512, COL_O = 256;  // S_0, S_1 (128 columns each), then O_0, O_1 (HD each)
+  // S_0, S_1 (128 columns each), O_0, O_1 (HD each), at head size 64 P_0, P_1 (64 each)
+  constexpr uint32_t TMEM_COLS = 512, COL_O = 256, COL_P = 384;
   extern __shared__ unsigned char window_smem[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(window_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char *sQ = smem, *sP = sQ + 2 * Sh::Q_TILE, *sKV = sP + 2 * Sh::P_TILE;
@@ -456,15 +458,19 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
               ptx::mbar_arrive(bar(&st->kv_empty[slot]));
               continue;
             }
-            // P of this step is in shared memory, the group has rescaled O if its maxima grew - and read the last unit's O
+            // P of this step is in its place, the group has rescaled O if its maxima grew - and read the last unit's O
             if (!(ok = wait(&st->p_ready[g], tp, ST_P))) break;
             if (!begun && units > 0 && !(ok = wait(&st->o_empty[g], units - 1, ST_O_FREE))) break;
             ptx::tc_fence_after();
             const uint64_t pd = tile_desc(p_base, 0), vd = tile_desc(kv_base + slot * Sh::KV_TILE, SLAB);
 #pragma unroll
-            for (int k16 = 0; k16 < TILE / 16; k16++)
-              ptx::umma_bf16(o_col, desc_at(pd, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)), desc_at(vd, (uint32_t)(k16 * 2048)), idesc,
-                             begun || k16 > 0);
+            for (int k16 = 0; k16 < TILE / 16; k16++) {
+              const uint64_t v16 = desc_at(vd, (uint32_t)(k16 * 2048));
+              if constexpr (Sh::P_IN_TMEM)
+                ptx::umma_bf16_ts(o_col, tmem_base + COL_P + (uint32_t)(g * 64 + k16 * 8), v16, idesc, begun || k16 > 0);
+              else
+                ptx::umma_bf16(o_col, desc_at(pd, (uint32_t)((k16 >> 2) * SLAB + (k16 & 3) * 32)), v16, idesc, begun || k16 > 0);
+            }
             begun = true;
             ptx::umma_commit(bar(&st->pv_done[g]));
             ptx::umma_commit(bar(&st->kv_empty[slot]));
@@ -556,9 +562,16 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
           }
           ptx::tmem_st_wait();
         }
-        store_packed<8>(p_addr, trow, 0, pk);
-        store_packed<8>(p_addr + SLAB, trow, 0, pk + 32);
-        ptx::fence_proxy_async_smem();
+        if constexpr (Sh::P_IN_TMEM) {
+          ptx::tc_fence_after();
+          ptx::tmem_st32(lane_addr + COL_P + (uint32_t)(g * 64), pk);
+          ptx::tmem_st32(lane_addr + COL_P + (uint32_t)(g * 64 + 32), pk + 32);
+          ptx::tmem_st_wait();
+        } else {
+          store_packed<8>(p_addr, trow, 0, pk);
+          store_packed<8>(p_addr + SLAB, trow, 0, pk + 32);
+          ptx::fence_proxy_async_smem();
+        }
         ptx::tc_fence_before();
         arrive(&st->p_ready[g]);
         first = false;
