@@ -11,7 +11,7 @@
 //              pair took 5600 cycles
 //   warps 4-11 four per tile, a thread per query row: scores to registers at once - which frees the accumulator for the next
 //              S, so that the tensor cores work while the exponentials are formed -, running maximum and sum,
-//              P = exp2((S - m) scale log2 e) as bf16 through shared memory. The second tile starts when the first has formed its
+//              P = exp2((S - m) scale log2 e) as bf16 through shared (head size 64: tensor) memory. The second tile starts when the first has formed its
 //              first P: one's waits and loads then lie under the other's exponentials
 // The maximum is raised, and O and the sum rescaled, only when a block's maximum exceeds it by more than 2^8.
 // Rounding: scores, statistics and accumulators fp32; P to bf16 (relative to m) before it multiplies V, the tensor cores take
@@ -19,12 +19,14 @@
 // Rows of V that no query of the sequence sees (before its first window, past its end) are zeroed in shared memory, so that
 // whatever they hold never meets the tensor cores; the scores of masked keys are dropped by a select.
 //
-// What bounds it: neither unit alone. A 128 x 128 x 128 product takes 727 cycles (both operands from shared memory), so a step of a pair has
-// 2900 cycles of tensor work and 2 x 128 x 128 exponentials (2050 cycles of the special-function units); a step takes 4000: products and
-// exponentials of the two tiles alternate, but the waits between them (250 cycles each) stay. Measured with 16 query heads on 4 of 128 and 8192
-// tokens: window 1024 97 us (65 GFLOP of visible pairs: 670 TFLOP/s; 86 with the masked parts of the blocks), window 4096 203 us, no window 250 us (1100 TFLOP/s;
-// the causal kernel without windows 330 us). Tried and slower: the second half of the scores' rows on 8 more warps that exchange maxima (127 us),
-// sink blocks in a form of 32 columns (their step is shorter, the others' longer: 107 us).
+// What bounds it, at head size 128: shared memory. A step of a pair moves 384 KB through it - 256 that four products read, 64 of P, 64 of K and V
+// that arrive -, 3070 cycles at 128 bytes each; a product of 128 x 128 x 128 alone takes 727 cycles for its 64 KB. A step takes 4000. At head size
+// 64 there is room for P in tensor memory, where the product takes its rows from: 9 to 11 % less time than through shared memory. At 128 it would
+// have to lie over S, and the next S then waits for P V (no window: 247 -> 299 us).
+// Measured with 16 query heads on 4 of 128 and 8192 tokens: window 1024 97 us (65 GFLOP of visible pairs: 670 TFLOP/s; 86 with the masked parts
+// of the blocks), no window 246 us (1120 TFLOP/s; the causal kernel without windows 330 us); heads of 64: 79 and 207 us. Tried and slower: the second
+// half of the scores' columns on 8 more warps that exchange maxima (127 us where this took 108), sink blocks in a form of 32 columns (their step is
+// shorter, the others' longer: 103 -> 106 us).
 //
 // Every wait is bounded; one that runs out raises the status word that b200_attention_status reads, and the CTA leaves.
 #include <cuda.h>
@@ -630,11 +632,10 @@ teardown:
 // Rounding: P and dS to bf16 once each (dS from the fp32 P), accumulators fp32, one rounding per output.
 // delta is formed from O as the caller holds it, rounded to bf16: a query with few keys loses up to 2^-9 of |dO| |O| against a delta of the
 // fp32 output, which the interface does not carry; the tests bound it.
-// What bounds both: shared memory. A 128 x 128 x 128 product reads 64 KB of operands in the 512 cycles that the multiplication takes, all
-// that shared memory gives, and measures 727; writing P and dS and the tiles that arrive come on top. A step of dQ (three products, 2180
-// cycles) takes 2600 to 2900, one of dK, dV (four, 2910) 3400.
-// Measured with 16 query heads on 4 of 128 and 8192 tokens: window 1024, 4 sinks dQ 130 us, dK and dV 180 us, join 4 us; no window 862 us
-// together (800 TFLOP/s; the causal kernel without windows 1110 us).
+// What bounds both: shared memory. A step of dK, dV moves 384 KB through it (four products of 64, P and dS, Q and dO that arrive; 3070 cycles at
+// 128 bytes each) and takes 3400; one of dQ 224 KB (1800 cycles; its third product reads K only) and takes about 2500.
+// Measured with 16 query heads on 4 of 128 and 8192 tokens: window 1024, 4 sinks dQ 120 us, dK and dV 175 us, join 4 us; no window 825 us
+// together (830 TFLOP/s; the causal kernel without windows 1110 us).
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int DS_TILE = TILE * TILE * 2;
 
