@@ -114,9 +114,9 @@ template <int HD>
 struct FwdShape {
   static constexpr bool P_IN_TMEM = HD == 64;  // where 128 of its columns are free
   static constexpr int Q_TILE = TILE * HD * 2, P_TILE = P_IN_TMEM ? 0 : TILE * TILE * 2, KV_TILE = TILE * HD * 2;
-  static constexpr int SLOTS = HD == 128 ? 3 : 6;
+  static constexpr int SLOTS = HD == 128 ? 3 : 6, RING = 4;
   struct Tail {
-    uint64_t q_full[2], q_empty[2], kv_full[SLOTS], kv_empty[SLOTS], s_full[2], s_read[2], p_ready[2], pv_done[2], o_empty[2], fixed;
+    uint64_t q_full[2], q_empty[2], k_full[RING], v_full[RING], kv_empty[SLOTS], s_full[2], s_read[2], p_ready[2], pv_done[2], o_empty[2], begun, fixed;
     uint32_t tmem_base;
     int abort_flag;
   };
@@ -289,7 +289,7 @@ __device__ __forceinline__ void zero_dead(uint32_t tile, const Span &sp, int kb,
 template <int HD, bool DEALT>
 __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid_constant__ FwdParams p) {
   using Sh = FwdShape<HD>;
-  constexpr int SLOTS = Sh::SLOTS;
+  constexpr int SLOTS = Sh::SLOTS, RING = Sh::RING;
   // S_0, S_1 (128 columns each), O_0, O_1 (HD each), at head size 64 P_0, P_1 (64 each)
   constexpr uint32_t TMEM_COLS = 512, COL_O = 256, COL_P = 384;
   extern __shared__ unsigned char window_smem[];
@@ -313,10 +313,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
       ptx::mbar_init(bar(&st->pv_done[g]), 1);
       ptx::mbar_init(bar(&st->o_empty[g]), TILE);
     }
-    for (int s = 0; s < SLOTS; s++) {
-      ptx::mbar_init(bar(&st->kv_full[s]), 1);
-      ptx::mbar_init(bar(&st->kv_empty[s]), 2);  // V: either tile's issuer; K: twice the one
+    for (int s = 0; s < RING; s++) {
+      ptx::mbar_init(bar(&st->k_full[s]), 1);
+      ptx::mbar_init(bar(&st->v_full[s]), 1);
     }
+    for (int s = 0; s < SLOTS; s++) ptx::mbar_init(bar(&st->kv_empty[s]), 2);  // V: either tile's issuer; K: twice the one
+    ptx::mbar_init(bar(&st->begun), TILE);
     ptx::mbar_init(bar(&st->fixed), 1);
     st->abort_flag = 0;
     ptx::fence_barrier_init();
@@ -339,7 +341,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
   pdl_wait();
 
   // The ring: step t of the CTA (counted through its units) uses K at place max(0, 2 t - 1) and V at place 2 t + 2: a unit's first K
-  // goes before the last unit's last V.
+  // goes before the last unit's last V. A slot holds K and V by turns, but
+  // whoever waits on a barrier must wait for every phase of it (a phase ahead, the parity is that of the last but one): K_t and V_t are announced
+  // on barriers of their own, t % 4. These are free again in time: the last load that needs no slot emptied is K_3 (six slots), and later
+  // ones follow an S or P V product of step t - 3, so whoever waits has seen step t - 4.
   auto k_at = [](uint32_t t) { return t == 0 ? 0u : 2 * t - 1; };
   auto v_at = [](uint32_t t) { return 2 * t + 2; };
 
@@ -350,11 +355,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
       uint32_t t = 0, uq[2] = {0, 0}, fixes = 0;
       bool ok = true;
       auto waitw = [&](uint64_t *b, uint32_t par, int code) { return __all_sync(0xffffffffu, wait(b, par, code)) != 0; };
-      auto load = [&](const CUtensorMap *m, uint32_t n, const Span &sp, int kvh, int kb, bool fix) {
+      auto load = [&](const CUtensorMap *m, uint32_t n, uint64_t *landed, const Span &sp, int kvh, int kb, bool fix) {
         const uint32_t slot = n % SLOTS;
         ok = waitw(&st->kv_empty[slot], n / SLOTS + 1, ST_KV_EMPTY);
         if (!ok) return;
-        const uint32_t tile = ptx::smem_u32(sKV + slot * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(&st->kv_full[slot]);
+        const uint32_t tile = ptx::smem_u32(sKV + slot * Sh::KV_TILE), full = fix ? bar(&st->fixed) : bar(landed);
         if (lane == 0) {
           ptx::mbar_arrive_expect_tx(full, (uint32_t)Sh::KV_TILE);
           ptx::tma_load_3d(tile, m, full, 0, sp.k_off + kb * TILE, kvh * (HD / 64));
@@ -365,13 +370,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         zero_dead<HD>(tile, sp, kb, p.window, p.sinks, lane);
         ptx::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(&st->kv_full[slot]));
+        if (lane == 0) ptx::mbar_arrive(bar(landed));
       };
       // the V of the step before
       Span last_sp;
       int last_kvh = 0, last_kb = 0;
       auto load_last_v = [&]() {
-        load(&p.tmV, v_at(t - 1), last_sp, last_kvh, last_kb, has_dead(last_sp, last_kb, p.window, p.sinks));
+        load(&p.tmV, v_at(t - 1), &st->v_full[(t - 1) % RING], last_sp, last_kvh, last_kb, has_dead(last_sp, last_kb, p.window, p.sinks));
       };
       Walk<DEALT> walk;
       for (int unit = walk.next(p.schedule, p.units); ok && unit < p.units; unit = walk.next(p.schedule, p.units)) {
@@ -391,7 +396,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
               uq[g]++;
             }
           }
-          if (ok) load(&p.tmK, k_at(t), u.sp, kvh, u.block(i), false);
+          if (ok) load(&p.tmK, k_at(t), &st->k_full[t % RING], u.sp, kvh, u.block(i), false);
           if (ok && t > 0) load_last_v();
           last_sp = u.sp;
           last_kvh = kvh;
@@ -415,8 +420,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
           if (ok && u.b.exists) ok = wait(&st->q_full[1], uq[1]++, ST_Q_FULL);
           for (int i = 0; ok && i < u.n; i++, t++) {
             const int kb = u.block(i);
-            const uint32_t n = k_at(t), slot = n % SLOTS;
-            if (!(ok = wait(&st->kv_full[slot], n / SLOTS, ST_KV_FULL))) break;
+            const uint32_t slot = k_at(t) % SLOTS;
+            if (!(ok = wait(&st->k_full[t % RING], t / RING, ST_KV_FULL))) break;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
               const Tile &x = g ? u.b : u.a;
@@ -454,8 +459,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
           const Tile x = g ? u.b : u.a;
           bool begun = false;
           for (int i = 0; ok && i < u.n; i++, t++) {
-            const uint32_t n = v_at(t), slot = n % SLOTS;
-            if (!(ok = wait(&st->kv_full[slot], n / SLOTS, ST_KV_FULL))) break;
+            const uint32_t slot = v_at(t) % SLOTS;
+            if (!(ok = wait(&st->v_full[t % RING], t / RING, ST_KV_FULL))) break;
             if (!x.active(u.block(i), p.sinks)) {
               ptx::mbar_arrive(bar(&st->kv_empty[slot]));
               continue;
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
     const uint32_t p_addr = ptx::smem_u32(sP + g * Sh::P_TILE + trow * 128);
     const float c = p.scale * LOG2E;
     uint32_t t = 0;  // steps of this tile so far
-    if (g == 1 && unit_of(p, Walk<DEALT>().next(p.schedule, p.units)).b.exists && !wait(&st->p_ready[0], 0, ST_P)) goto teardown;
+    if (g == 1 && unit_of(p, Walk<DEALT>().next(p.schedule, p.units)).b.exists && !wait(&st->begun, 0, ST_P)) goto teardown;
     Walk<DEALT> walk;
     for (int unit = walk.next(p.schedule, p.units); unit < p.units; unit = walk.next(p.schedule, p.units)) {
       const Unit u = unit_of(p, unit);
@@ -576,6 +581,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         }
         ptx::tc_fence_before();
         arrive(&st->p_ready[g]);
+        if (g == 0 && t == 0) arrive(&st->begun);
         first = false;
         t++;
       }

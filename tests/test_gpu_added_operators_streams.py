@@ -4,13 +4,13 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
-HQ, HKV, HD, WINDOW, SINKS = 8, 2, 128, 150, 4
+HQ, HKV, WINDOW, SINKS = 8, 2, 150, 4
 
 
 class Work:
     """Norm and rotation, attention, both backwards, and a SwiGLU held in 8 bits: inputs, outputs and what the calls need."""
 
-    def __init__(self, seed, q_lens, workspace=None):
+    def __init__(self, seed, q_lens, HD=128, workspace=None):
         import torch
 
         from ml_dataflow_b200 import ops
@@ -19,7 +19,7 @@ class Work:
         rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)
         self.lens, T = q_lens, sum(q_lens)
         self.offs = [sum(q_lens[:i]) for i in range(len(q_lens))]
-        self.T, self.f = T, 200
+        self.T, self.f, self.HD = T, 200, HD
         self.q, self.k, self.v, self.do = rand(T, HQ * HD), rand(T, HKV * HD), rand(T, HKV * HD), rand(T, HQ * HD)
         self.wq, self.wk = rand(HD), rand(HD)
         self.pos = torch.cat([torch.arange(n, device="cuda", dtype=torch.int32) for n in q_lens])
@@ -36,7 +36,7 @@ class Work:
     def run(self):
         from ml_dataflow_b200 import ops
 
-        o, T = self.out, self.T
+        o, T, HD = self.out, self.T, self.HD
         ops.qk_norm_rope(T, HQ, HKV, HD, 1e-5, 10000, self.pos, self.wq, self.wk, self.q, self.k, o["yq"], o["yk"])
         args = (self.offs, self.lens, self.offs, self.lens, HQ, HKV, HD, o["yq"], o["yk"], self.v, o["o"], o["lse"])
         ops.attention_window_fwd(*args, WINDOW, SINKS)
@@ -61,7 +61,8 @@ def _same(a, b):
         assert torch.equal(a[n], b[n]), n
 
 
-def test_three_streams_at_once():
+@pytest.mark.parametrize("hd", [128, 64])
+def test_three_streams_at_once(hd):
     import torch
 
     from gpu_util import require_b200
@@ -69,14 +70,14 @@ def test_three_streams_at_once():
     require_b200()
     from ml_dataflow_b200 import ops
 
-    works = [Work(1, [700, 33, 400]), Work(2, [1, 1, 3, 1]), Work(3, [1500])]
+    works = [Work(1, [700, 33, 400], hd), Work(2, [1, 1, 3, 1], hd), Work(3, [1500], hd)]
     want = []
     for w in works:
         w.run()
         want.append(w.take())
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in works]  # none of them is the one the tensors were made on
-    for _ in range(4):
+    for _ in range(300):  # loads that arrive late and out of order are rare
         for _ in range(3):
             for w, s in zip(works, streams):
                 with torch.cuda.stream(s):
