@@ -81,19 +81,26 @@ struct Schedule {
 __device__ __forceinline__ int unit_at(int round) {
   return (round & 1) ? (round + 1) * (int)gridDim.x - 1 - (int)blockIdx.x : round * (int)gridDim.x + (int)blockIdx.x;
 }
-template <bool DEALT>
+// The forward of few units on many keys: the CTAs of a cluster share one, each takes a part of its blocks (join_parts below; 512 queries on 16384
+// keys, 16 heads on 4 of 128: 184 -> 77 us).
+enum { WALK_ROUNDS, WALK_DEALT, WALK_SHARED };
+constexpr int MAX_SHARERS = 8;
+template <int WALK>
 struct Walk {
   int at = 0;
   // the CTA's next unit; `units` or more: no more
-  __device__ __forceinline__ int next(const Schedule &s, int units) {
-    if constexpr (!DEALT) {
+  template <typename P>
+  __device__ __forceinline__ int next(const P &p) {
+    if constexpr (WALK == WALK_ROUNDS) {
       return unit_at(at++);
+    } else if constexpr (WALK == WALK_SHARED) {
+      return at++ == 0 ? (int)blockIdx.x / p.cluster : p.units;
     } else {
-      while (at < s.n) {
-        const Schedule::Run r = s.run[at++];
+      while (at < p.schedule.n) {
+        const Schedule::Run r = p.schedule.run[at++];
         if ((unsigned)((int)blockIdx.x - r.cta) < (unsigned)r.n) return r.unit + (int)blockIdx.x - r.cta;
       }
-      return units;
+      return p.units;
     }
   }
 };
@@ -105,7 +112,8 @@ struct FwdParams {
   __nv_bfloat16 *O;
   float *lse;  // [q_heads][total_q]
   int window, sinks, group, q_heads, total_q, pair_heads, units;
-  int whole;  // units from this one on are one tile of a pair each
+  int whole;    // units from this one on are one tile of a pair each
+  int cluster;  // CTAs that share a unit
   float scale;
   int *status;
 };
@@ -144,6 +152,11 @@ struct Unit {
   Tile a, b;
   int n, n_sink, first;
   __device__ __forceinline__ int block(int i) const { return i < n_sink ? i : first + i - n_sink; }
+  // the blocks of this CTA: all, or its share
+  template <int WALK>
+  __device__ __forceinline__ int begin(int cluster) const { return WALK == WALK_SHARED ? n * ((int)blockIdx.x % cluster) / cluster : 0; }
+  template <int WALK>
+  __device__ __forceinline__ int end(int cluster) const { return WALK == WALK_SHARED ? n * ((int)blockIdx.x % cluster + 1) / cluster : n; }
 };
 __host__ __device__ __forceinline__ Tile tile_of(const Span &sp, int window, int h, int row) {
   Tile t;
@@ -286,7 +299,104 @@ __device__ __forceinline__ void zero_dead(uint32_t tile, const Span &sp, int kb,
   }
 }
 
-template <int HD, bool DEALT>
+// A thread's row of a shared unit (its tile, its output in tensor memory unless it saw no key here, its maximum and sum) to shared memory, all
+// CTAs' rows joined in the order of their ranks. The 16-byte pieces of a row are swizzled with the row.
+template <int HD>
+__device__ __forceinline__ uint32_t part_at(uint32_t base, int row, int piece) {
+  return base + (uint32_t)(row * HD * 4 + ((piece ^ row) & (HD / 4 - 1)) * 16);
+}
+template <int HD>
+__device__ __forceinline__ void store_part(uint32_t base, int row, uint32_t o_addr, bool any, float m, float l) {
+#pragma unroll
+  for (int q = 0; q < HD / 32; q++) {
+    uint32_t v[32];
+    load_columns<32>(o_addr + q * 32, v);  // whole warps
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      sts128(part_at<HD>(base, row, q * 8 + j), any ? make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]) : make_uint4(0, 0, 0, 0));
+  }
+  fa::sts32(base + (uint32_t)(2 * TILE * HD * 4 + row * 8), m);
+  fa::sts32(base + (uint32_t)(2 * TILE * HD * 4 + row * 8 + 4), l);
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+template <typename T>
+__device__ __forceinline__ T of_cluster(uint32_t addr, uint32_t rank);
+template <>
+__device__ __forceinline__ float4 of_cluster<float4>(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("{\n.reg .b32 ra;\nmapa.shared::cluster.u32 ra, %4, %5;\nld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n}\n"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr), "r"(rank)
+               : "memory");
+  return v;
+}
+template <>
+__device__ __forceinline__ float2 of_cluster<float2>(uint32_t addr, uint32_t rank) {
+  float2 v;
+  asm volatile("{\n.reg .b32 ra;\nmapa.shared::cluster.u32 ra, %2, %3;\nld.shared::cluster.v2.f32 {%0, %1}, [ra];\n}\n"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(addr), "r"(rank)
+               : "memory");
+  return v;
+}
+// `thread` of 256; this CTA's share of the unit's rows. First every row's weights of the CTAs' parts, then its pieces, all CTAs' loads under way at
+// once (one after the other they took 12 us).
+template <int HD>
+__device__ __forceinline__ void join_parts(const FwdParams &p, uint32_t base, int thread) {
+  constexpr int PIECES = HD / 4, AT_ONCE = 256 / PIECES;
+  const float c = p.scale * LOG2E;
+  const Unit u = unit_of(p, (int)blockIdx.x / p.cluster);
+  const int rows = 2 * TILE / p.cluster, row0 = rows * ((int)blockIdx.x % p.cluster), piece = thread % PIECES;
+  const uint32_t stats = base + (uint32_t)(2 * TILE * HD * 4), weights = stats + 2 * TILE * 8;
+  if (thread < rows) {
+    const int at = row0 + thread, row = at & (TILE - 1);
+    const Tile &x = at < TILE ? u.a : u.b;
+    float2 ml[MAX_SHARERS];
+#pragma unroll
+    for (int k = 0; k < MAX_SHARERS; k++) ml[k] = k < p.cluster ? of_cluster<float2>(stats + at * 8, k) : make_float2(-INFINITY, 0.0f);
+    float M = -INFINITY, L = 0.0f, f[MAX_SHARERS];
+#pragma unroll
+    for (int k = 0; k < MAX_SHARERS; k++) M = fmaxf(M, ml[k].x);
+#pragma unroll
+    for (int k = 0; k < MAX_SHARERS; k++) {
+      f[k] = ml[k].x == -INFINITY ? 0.0f : ex2((ml[k].x - M) * c);
+      L = fmaf(f[k], ml[k].y, L);
+    }
+    const float inv = 1.0f / L;
+#pragma unroll
+    for (int k = 0; k < MAX_SHARERS; k++) fa::sts32(weights + (thread * MAX_SHARERS + k) * 4, f[k] * inv);
+    if (x.exists && x.row + row < u.sp.Tq) p.lse[(int64_t)x.h * p.total_q + u.sp.q_off + x.row + row] = M * p.scale + logf(L);
+  }
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 2
+  for (int q = thread / PIECES; q < rows; q += AT_ONCE) {
+    const int at = row0 + q, row = at & (TILE - 1);
+    const Tile &x = at < TILE ? u.a : u.b;
+    if (!x.exists || x.row + row >= u.sp.Tq) continue;
+    float4 v[MAX_SHARERS];
+#pragma unroll
+    for (int k = 0; k < MAX_SHARERS; k++)
+      if (k < p.cluster) v[k] = of_cluster<float4>(part_at<HD>(base, at, piece), k);
+    const float4 w[2] = {fa::lds128(weights + q * MAX_SHARERS * 4), fa::lds128(weights + q * MAX_SHARERS * 4 + 16)};
+    const float f[MAX_SHARERS] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < MAX_SHARERS; k++)
+      if (k < p.cluster) {
+        sum.x = fmaf(f[k], v[k].x, sum.x);
+        sum.y = fmaf(f[k], v[k].y, sum.y);
+        sum.z = fmaf(f[k], v[k].z, sum.z);
+        sum.w = fmaf(f[k], v[k].w, sum.w);
+      }
+    *reinterpret_cast<uint2 *>(p.O + ((int64_t)(u.sp.q_off + x.row + row) * p.q_heads + x.h) * HD + piece * 4) =
+        make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
+  }
+}
+
+template <int HD, int WALK>
 __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid_constant__ FwdParams p) {
   using Sh = FwdShape<HD>;
   constexpr int SLOTS = Sh::SLOTS, RING = Sh::RING;
@@ -339,6 +449,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
   const uint32_t tmem_base = st->tmem_base;
   pdl_release();
   pdl_wait();
+  float part_m = -INFINITY, part_l = 0.0f;  // of a shared unit
 
   // The ring: step t of the CTA (counted through its units) uses K at place max(0, 2 t - 1) and V at place 2 t + 2: a unit's first K
   // goes before the last unit's last V. A slot holds K and V by turns, but
@@ -378,12 +489,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
       auto load_last_v = [&]() {
         load(&p.tmV, v_at(t - 1), &st->v_full[(t - 1) % RING], last_sp, last_kvh, last_kb, has_dead(last_sp, last_kb, p.window, p.sinks));
       };
-      Walk<DEALT> walk;
-      for (int unit = walk.next(p.schedule, p.units); ok && unit < p.units; unit = walk.next(p.schedule, p.units)) {
+      Walk<WALK> walk;
+      for (int unit = walk.next(p); ok && unit < p.units; unit = walk.next(p)) {
         const Unit u = unit_of(p, unit);
         const int kvh = u.a.h / p.group;
-        for (int i = 0; ok && i < u.n; i++) {
-          if (i == 0) {  // the last unit's S products still read its Q
+        const int begin = u.begin<WALK>(p.cluster), end = u.end<WALK>(p.cluster);
+        for (int i = begin; ok && i < end; i++) {
+          if (i == begin) {  // the last unit's S products still read its Q
 #pragma unroll
             for (int g = 0; g < 2; g++) {
               const Tile &x = g ? u.b : u.a;
@@ -413,12 +525,14 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         const uint32_t q_base = ptx::smem_u32(sQ), kv_base = ptx::smem_u32(sKV);
         uint32_t t = 0, uq[2] = {0, 0}, ts[2] = {0, 0};  // steps; units and S products of either tile
         bool ok = true;
-        Walk<DEALT> walk;
-        for (int unit = walk.next(p.schedule, p.units); ok && unit < p.units; unit = walk.next(p.schedule, p.units)) {
+        Walk<WALK> walk;
+        for (int unit = walk.next(p); ok && unit < p.units; unit = walk.next(p)) {
           const Unit u = unit_of(p, unit);
+          const int begin = u.begin<WALK>(p.cluster), end = u.end<WALK>(p.cluster);
+          if (begin == end) continue;
           if (u.a.exists) ok = wait(&st->q_full[0], uq[0]++, ST_Q_FULL);
           if (ok && u.b.exists) ok = wait(&st->q_full[1], uq[1]++, ST_Q_FULL);
-          for (int i = 0; ok && i < u.n; i++, t++) {
+          for (int i = begin; ok && i < end; i++, t++) {
             const int kb = u.block(i);
             const uint32_t slot = k_at(t) % SLOTS;
             if (!(ok = wait(&st->k_full[t % RING], t / RING, ST_KV_FULL))) break;
@@ -453,12 +567,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         const uint32_t p_base = ptx::smem_u32(sP + g * Sh::P_TILE), kv_base = ptx::smem_u32(sKV), o_col = tmem_base + COL_O + (uint32_t)(g * HD);
         uint32_t t = 0, units = 0, tp = 0;  // steps; units and products of this tile
         bool ok = true;
-        Walk<DEALT> walk;
-        for (int unit = walk.next(p.schedule, p.units); ok && unit < p.units; unit = walk.next(p.schedule, p.units)) {
+        Walk<WALK> walk;
+        for (int unit = walk.next(p); ok && unit < p.units; unit = walk.next(p)) {
           const Unit u = unit_of(p, unit);
           const Tile x = g ? u.b : u.a;
           bool begun = false;
-          for (int i = 0; ok && i < u.n; i++, t++) {
+          const int end = u.end<WALK>(p.cluster);
+          for (int i = u.begin<WALK>(p.cluster); ok && i < end; i++, t++) {
             const uint32_t slot = v_at(t) % SLOTS;
             if (!(ok = wait(&st->v_full[t % RING], t / RING, ST_KV_FULL))) break;
             if (!x.active(u.block(i), p.sinks)) {
@@ -498,9 +613,14 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
     const uint32_t p_addr = ptx::smem_u32(sP + g * Sh::P_TILE + trow * 128);
     const float c = p.scale * LOG2E;
     uint32_t t = 0;  // steps of this tile so far
-    if (g == 1 && unit_of(p, Walk<DEALT>().next(p.schedule, p.units)).b.exists && !wait(&st->begun, 0, ST_P)) goto teardown;
-    Walk<DEALT> walk;
-    for (int unit = walk.next(p.schedule, p.units); unit < p.units; unit = walk.next(p.schedule, p.units)) {
+    if (g == 1) {
+      const Unit u = unit_of(p, Walk<WALK>().next(p));
+      // (of a shared unit's neighbouring tiles the first may see none of this CTA's blocks)
+      const bool both = WALK != WALK_SHARED || (p.pair_heads && u.begin<WALK>(p.cluster) < u.end<WALK>(p.cluster));
+      if (u.b.exists && both && !wait(&st->begun, 0, ST_P)) goto teardown;
+    }
+    Walk<WALK> walk;
+    for (int unit = walk.next(p); unit < p.units; unit = walk.next(p)) {
       const Unit u = unit_of(p, unit);
       const Tile x = g ? u.b : u.a;
       if (!x.exists) continue;
@@ -508,7 +628,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
       const int tile_pos = x.row + u.sp.shift, last_pos = min(tile_pos + TILE, u.sp.Tk) - 1;
       float m = -INFINITY, l = 0.0f;
       bool first = true;
-      for (int i = 0; i < u.n; i++) {
+      const int end = u.end<WALK>(p.cluster);
+      for (int i = u.begin<WALK>(p.cluster); i < end; i++) {
         const int kb = u.block(i);
         if (!x.active(kb, p.sinks)) continue;
         if (!wait(&st->s_full[g], t, ST_S)) goto teardown;
@@ -585,7 +706,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) window_fwd_kernel(const __grid
         first = false;
         t++;
       }
+      if (WALK == WALK_SHARED && t == 0) continue;
       if (!wait(&st->pv_done[g], t - 1, ST_PV)) goto teardown;
+      if (WALK == WALK_SHARED) {
+        part_m = m;
+        part_l = l;
+        continue;
+      }
       ptx::tc_fence_after();
       uint32_t r[HD];
       load_columns<HD>(o_addr, r);
@@ -609,6 +736,20 @@ teardown:
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if constexpr (WALK == WALK_SHARED) {
+    // Every product has been waited for and every tile that was loaded has been used: shared memory is free. (After a wait that ran out: rubbish,
+    // but every thread comes by here.)
+    const int thread = tid - 128;
+    ptx::tc_fence_after();
+    if (warp >= 4) {
+      const uint32_t o_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + COL_O + (uint32_t)((thread >> 7) * HD);
+      store_part<HD>(ptx::smem_u32(smem), thread, o_addr, part_m != -INFINITY, part_m, part_l);
+    }
+    ptx::tc_fence_before();
+    cluster_sync();
+    if (warp >= 4) join_parts<HD>(p, ptx::smem_u32(smem), thread);
+    cluster_sync();  // nobody leaves while another reads its shared memory
+  }
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem_base, TMEM_COLS);
@@ -1486,19 +1627,22 @@ void deal(window::Schedule *s, int sequences, int units, int ctas, F cost, G nex
   s->n = runs;
 }
 
-template <int HD, bool DEALT>
+template <int HD, int WALK>
 int launch_fwd(const window::FwdParams &p, const Device &d, cudaStream_t s) {
   static bool done[MAX_DEVICES];
   constexpr size_t smem = window::FwdShape<HD>::smem;
-  if (allow_smem(window::window_fwd_kernel<HD, DEALT>, smem, &done[d.dev])) return -1;
-  B200_CUDA(b200_launch_overlapped(window::window_fwd_kernel<HD, DEALT>, dim3(p.units < d.sms ? p.units : d.sms), dim3(window::FWD_THREADS), smem, s, 1,
-                                   p));
+  static_assert(smem >= 1024 + 2 * window::TILE * (HD + 2 + window::MAX_SHARERS) * sizeof(float), "the parts of a shared unit");
+  if (allow_smem(window::window_fwd_kernel<HD, WALK>, smem, &done[d.dev])) return -1;
+  const int ctas = p.units * p.cluster;
+  B200_CUDA(b200_launch_overlapped(window::window_fwd_kernel<HD, WALK>, dim3(ctas < d.sms ? ctas : d.sms), dim3(window::FWD_THREADS), smem, s,
+                                   (unsigned)p.cluster, p));
   B200_CHECK_LAUNCH("attention_window_fwd");
   return 0;
 }
 template <int HD>
 int launch_fwd(const window::FwdParams &p, const Device &d, cudaStream_t s) {
-  return p.schedule.n > 0 ? launch_fwd<HD, true>(p, d, s) : launch_fwd<HD, false>(p, d, s);
+  if (p.cluster > 1) return launch_fwd<HD, window::WALK_SHARED>(p, d, s);
+  return p.schedule.n > 0 ? launch_fwd<HD, window::WALK_DEALT>(p, d, s) : launch_fwd<HD, window::WALK_ROUNDS>(p, d, s);
 }
 
 template <int HD>
@@ -1524,9 +1668,18 @@ int launch_bwd_kv(const window::BwdParams &p, const Device &d, cudaStream_t s) {
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 // blocks of 128 keys that a tile of queries sees, at most (of 128 queries that see a block of keys, with the queries' number)
-int blocks_seen(const window::Call &c, int s, int rows) {
-  const int64_t span = (int64_t)c.window + 2 * window::TILE + (c.sinks < c.k_len[s] ? c.sinks : c.k_len[s]);
+int blocks_seen(const window::Call &c, int Tk, int rows) {
+  const int64_t span = (int64_t)c.window + 2 * window::TILE + (c.sinks < Tk ? c.sinks : Tk);
   return (int)(((span < rows ? span : rows) + window::TILE - 1) / window::TILE);
+}
+
+// CTAs that share a pair: joining their parts takes 6 to 8 us, a block that one walks 1.4 (half a pair) or 1.9. Measured at head size 128, in halves
+// and with 2, 4, 8 CTAs a pair: 16 pairs of 6 blocks 14, 19, 16 us, of 8 17, 21, 16, of 24 39, 37, 24; 8 pairs of 16 28, 29, 19, 17; 56 pairs of 16
+// 30, 31, of 24 41, 39. (16 pairs with 8, 28 to 47: not all clusters of eight find a place at once.)
+int sharers(int pairs, int blocks, int sms) {
+  if (pairs * 8 <= sms / 2 && blocks >= 16) return 8;
+  if (pairs * 4 <= sms && blocks >= 10) return 4;
+  return pairs * 2 <= sms && blocks >= 22 ? 2 : 1;
 }
 
 int slot_rows(int sinks) { return sinks < window::TILE ? sinks : window::TILE; }
@@ -1586,13 +1739,13 @@ int sm100_bwd(const Call &c) {
   B200_REQUIRE(p.status != nullptr, "attention_window: the status word of this device is not reachable");
   for (int next = 0; next < c.num_seqs;) {
     p.units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.q_len[s] + TILE - 1) / TILE * c.q_heads; },
-                             [&](int s) { return blocks_seen(c, s, c.k_len[s]); });
+                             [&](int s) { return blocks_seen(c, c.k_len[s], c.k_len[s]); });
     if (p.units == 0) continue;
     if (c.head_dim == 128 ? launch_bwd_q<128>(p, d, c.stream) : launch_bwd_q<64>(p, d, c.stream)) return -1;
   }
   for (int next = 0; next < c.num_seqs;) {
     p.main_units = next_sequences(p.seqs, &next, c, [&](int s) { return (c.k_len[s] + TILE - 1) / TILE * c.kv_heads; },
-                                  [&](int s) { return blocks_seen(c, s, c.q_len[s]); });
+                                  [&](int s) { return blocks_seen(c, c.k_len[s], c.q_len[s]); });
     if (p.main_units == 0) continue;
     // as many units as there are SMs, if the heads of a group give them
     p.parts = p.main_units < MAX_SPLIT_UNITS ? MAX_SPLIT_UNITS / p.main_units : 1;
@@ -1653,12 +1806,15 @@ int sm100_fwd(const Call &c) {
           const int tiles = is_few(c, s) ? 0 : (c.q_len[s] + TILE - 1) / TILE;
           return p.pair_heads ? tiles * (c.q_heads / 2) : (tiles + 1) / 2 * c.q_heads;
         },
-        [&](int s) { return blocks_seen(c, s, c.k_len[s]); });
+        [&](int s) { return blocks_seen(c, c.k_len[s], c.k_len[s]); });
     if (p.units == 0) continue;
     // In the last round, pairs are given to two CTAs as long as there are CTAs without one (8192 tokens, window 1024, 512 pairs: 103 -> 97
     // us; 400 tokens of 8 heads, 16 pairs: 14 -> 11). Not where the units of a long sequence run from one block to all: the last round's are
     // its short ones, and two halves take longer than a pair (no window: 246 -> 250 us).
-    const int last = p.units % d.sms, split = p.units > d.sms && c.window > p.seqs.Tk[0] / 2 ? 0 : (last < d.sms - last ? last : d.sms - last);
+    const int last = p.units % d.sms, halves = last < d.sms - last ? last : d.sms - last;
+    const bool ramp = p.units > d.sms && c.window > p.seqs.Tk[0] / 2;
+    p.cluster = sharers(p.units, blocks_seen(c, p.seqs.Tk[0], p.seqs.Tk[0]), d.sms);
+    const int split = ramp || p.cluster > 1 ? 0 : halves;
     p.whole = p.units - split;
     p.units += split;
     // in quarters of a pair's step: a single tile's step takes three, a unit's begin and end five

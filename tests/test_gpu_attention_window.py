@@ -38,6 +38,12 @@ CASES = [
     ([1, 1, 2], [700, 3, 260], 24, 1, 128, 300, 5),     # few queries: more rows than one 16-row tile of a group; 48 rows go to the tiles
     ([1, 2], [500, 900], 40, 1, 64, 1000, 0),           # a group of 40 heads
     ([1, 3, 1], [2000, 130, 77], 21, 3, 128, 90, 2),    # an odd group
+    # few queries' tiles on many keys: shared by 2, 4 or 8 CTAs, some of which see nothing of a short sequence or of a tile of a pair
+    ([600], [5200], 16, 2, 128, 4000, 4),
+    ([300], [2100], 8, 4, 128, 1500, 17),
+    ([129, 20, 9], [2500, 20, 400], 4, 1, 64, 2300, 0),
+    ([257, 40], [1700, 300], 3, 3, 128, 1400, 130),
+    ([500], [3000], 5, 5, 64, 2600, 3),
     ([2] * 200, [2 + 5 * n for n in range(200)], 2, 1, 64, 64, 3),  # more sequences than one launch of the few-query form takes
 ]
 
