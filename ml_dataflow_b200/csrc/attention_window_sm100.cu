@@ -23,8 +23,8 @@
 // that arrive -, 3070 cycles at 128 bytes each; a product of 128 x 128 x 128 alone takes 727 cycles for its 64 KB. A step takes 4000. At head size
 // 64 there is room for P in tensor memory, where the product takes its rows from: 9 to 11 % less time than through shared memory. At 128 it would
 // have to lie over S, and the next S then waits for P V (no window: 247 -> 299 us).
-// Measured with 16 query heads on 4 of 128 and 8192 tokens: window 1024 97 us (65 GFLOP of visible pairs: 670 TFLOP/s; 86 with the masked parts
-// of the blocks), no window 246 us (1120 TFLOP/s; the causal kernel without windows 330 us); heads of 64: 79 and 207 us. Tried and slower: the second
+// Measured with 16 query heads on 4 of 128 and 8192 tokens: window 1024 96 us (65 GFLOP of visible pairs: 670 TFLOP/s; 86 with the masked parts
+// of the blocks), no window 238 us (1155 TFLOP/s; the causal kernel without windows 330 us); heads of 64: 79 and 207 us. Tried and slower: the second
 // half of the scores' columns on 8 more warps that exchange maxima (127 us where this took 108), sink blocks in a form of 32 columns (their step is
 // shorter, the others' longer: 103 -> 106 us).
 //
