@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(THREADS, BWD ? BWD_BLOCKS : FWD_BLOCKS) qk_nor
       ss += odd;
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float rn = rsqrtf(fmaf(ss, p.inv_dim, p.eps));
+      // the places behind the last head hold zeros: with eps = 0 their 0 * (1 / 0) would be a NaN in the weight gradients, which sum over all places
+      const float rn = BWD && !on ? 0.0f : rsqrtf(fmaf(ss, p.inv_dim, p.eps));
       const uint64_t rr = pack2(rn, rn);
       uint32_t out[4];
       if (!BWD) {
