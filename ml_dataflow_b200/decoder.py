@@ -40,7 +40,7 @@ class DecoderConfig:
     qk_norm: bool = False         # RMSNorm of every query and key head, with weights unless qk_norm_weights is False
     qk_norm_weights: bool = True
     window: int = 0               # keys a query sees, its own included; 0: all before it
-    num_sinks: int = 0            # first keys of a sequence that stay visible
+    num_sinks: int = 0            # first keys of a sequence that stay visible (without a window all do)
     act8: bool = False            # x1 and x3 of the MoE layers in 8 bits between forward and backward
 
 
@@ -145,7 +145,7 @@ class Decoder:
         if not (c.qk_norm or c.window or c.act8):
             return None
         p = lambda t: None if t is None else t.data_ptr()
-        o = _lib.TransformerBlockOptions(window=c.window, num_sinks=c.num_sinks)
+        o = _lib.TransformerBlockOptions(window=c.window, num_sinks=c.num_sinks if c.window else 0)  # no window: every key is seen
         if c.qk_norm:
             o.qk_norm, o.qk_eps, o.q_raw, o.k_raw = 1, c.eps, p(S["q_raw"]), p(S["k_raw"])
         if self.qk_ws is not None:
