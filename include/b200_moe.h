@@ -48,6 +48,10 @@ extern "C" {
 /* Library / device identification. Returns 0 and fills sm_count, cc_major, cc_minor of the current device. */
 int b200_device_info(int *sm_count, int *cc_major, int *cc_minor);
 
+/* Kernels that the q/k norm with rotation, the windowed attention and the 8-bit activations have launched in this process so far, for
+ * accounts of launches: how many a call makes follows from its sizes. No counterpart in the reference. */
+uint64_t b200_launch_count(void);
+
 /* ---- router ------------------------------------------------------------------ */
 
 /*

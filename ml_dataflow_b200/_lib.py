@@ -13,6 +13,7 @@ _vp, _i, _f, _i64, _u64, _sz = C.c_void_p, C.c_int, C.c_float, C.c_int64, C.c_ui
 # name -> (restype, argtypes); mirrors include/b200_moe.h
 SIGNATURES = {
     "b200_device_info": (_i, [_vp, _vp, _vp]),
+    "b200_launch_count": (_u64, []),
     "b200_select_experts": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_build_expert_mapping_workspace_bytes": (_sz, [_i, _i, _i]),
     "b200_build_expert_mapping": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -314,6 +314,7 @@ int rows_fwd(const window::Call &c) {
     if (rows == 0) continue;
     window::rows_fwd_kernel<<<blocks_for(rows * c.q_heads), window::THREADS, 0, c.stream>>>(p);
     B200_CHECK_LAUNCH("attention_window_fwd");
+    count_launch();
   }
   return 0;
 }
@@ -325,12 +326,14 @@ int rows_bwd(const window::Call &c) {
     if (rows == 0) continue;
     window::rows_bwd_q_kernel<<<blocks_for(rows * c.q_heads), window::THREADS, 0, c.stream>>>(p);
     B200_CHECK_LAUNCH("attention_window_bwd (dQ)");
+    count_launch();
   }
   for (int next = 0; next < c.num_seqs;) {
     const int64_t rows = window::next_sequences(p.seqs, &next, c, [&](int s) { return c.k_len[s]; }, [](int) { return 0; });
     if (rows == 0) continue;
     window::rows_bwd_kv_kernel<<<blocks_for(rows * c.kv_heads), window::THREADS, 0, c.stream>>>(p);
     B200_CHECK_LAUNCH("attention_window_bwd (dK, dV)");
+    count_launch();
   }
   return 0;
 }

@@ -35,6 +35,12 @@
 
 static inline bool b200_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+namespace b200 {
+// What b200_launch_count returns: kernels launched by the q/k norm, the windowed attention and the 8-bit activations (router.cu).
+extern uint64_t launch_count;
+static inline void count_launch() { __atomic_fetch_add(&launch_count, 1, __ATOMIC_RELAXED); }
+}  // namespace b200
+
 // Launches a kernel that begins (pdl_release and pdl_wait below) by letting the stream's next kernel come up and by waiting for the kernel before
 // it: its blocks are placed and set up while that one drains. A kernel before it that says nothing of the kind is simply waited for.
 template <typename... Params, typename... Args>
@@ -53,7 +59,9 @@ static inline cudaError_t b200_launch_overlapped(void (*kernel)(Params...), dim3
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  if (e == cudaSuccess) b200::count_launch();
+  return e;
 }
 
 namespace b200 {

@@ -348,6 +348,10 @@ __global__ void gather_router_grad_kernel(int64_t n, int E, int top_k, const int
 
 using namespace b200;
 
+uint64_t b200::launch_count = 0;
+
+extern "C" uint64_t b200_launch_count(void) { return __atomic_load_n(&b200::launch_count, __ATOMIC_RELAXED); }
+
 extern "C" int b200_device_info(int *sm_count, int *cc_major, int *cc_minor) {
   int dev = 0;
   B200_CUDA(cudaGetDevice(&dev));

@@ -45,6 +45,19 @@ def _check(rc, name, launches=None):
     LAUNCHES += _KERNELS_PER_CALL.get(name, 1) if launches is None else launches
 
 
+_reported = 0  # of the launches that the library counts itself, those that LAUNCHES holds already
+
+
+def _check_counted(rc, name, others=0):
+    """The same for ops whose launches follow from their sizes: the library counts them. others: kernels of the call that it does not."""
+    global LAUNCHES, _reported
+    if rc != 0:
+        raise RuntimeError(f"{name} failed (see stderr)")
+    now = _lib.load().b200_launch_count()
+    LAUNCHES += now - _reported + others
+    _reported = now
+
+
 def device_info():
     sm, major, minor = C.c_int(), C.c_int(), C.c_int()
     _check(_lib.load().b200_device_info(C.byref(sm), C.byref(major), C.byref(minor)), "b200_device_info", 0)
@@ -388,8 +401,9 @@ def _int_array(values):
 def transformer_block_fwd(block, x, out, options=None):
     """block: _lib.TransformerBlock; out = block(x). options: _lib.TransformerBlockOptions (q/k norm, window, 8-bit activations)."""
     if options is not None:
-        _check(_lib.load().b200_transformer_block_fwd_options(C.byref(block), C.byref(options), _p(x), _p(out), _stream()),
-               "transformer_block_fwd_options", 20 + (options.codes_w1 is not None))
+        # of the 20 below, the rotation and the attention are counted ops here where the options replace them
+        _check_counted(_lib.load().b200_transformer_block_fwd_options(C.byref(block), C.byref(options), _p(x), _p(out), _stream()),
+                       "transformer_block_fwd_options", 20 - bool(options.qk_norm) - (options.window > 0))
         return
     _check(_lib.load().b200_transformer_block_fwd(C.byref(block), _p(x), _p(out), _stream()), "transformer_block_fwd", 20)
 
@@ -397,8 +411,10 @@ def transformer_block_fwd(block, x, out, options=None):
 def transformer_block_bwd(block, x, dx, grads, scratch, options=None):
     """dx: the gradient at the block's output on entry, at its input on return; grads are accumulated into."""
     if options is not None:
-        _check(_lib.load().b200_transformer_block_bwd_options(C.byref(block), C.byref(options), _p(x), _p(dx), C.byref(grads),
-                                                              C.byref(scratch), _stream()), "transformer_block_bwd_options", 45)
+        # likewise the rotation and the three kernels of the attention; 8-bit activations gather the zone again
+        _check_counted(_lib.load().b200_transformer_block_bwd_options(C.byref(block), C.byref(options), _p(x), _p(dx), C.byref(grads), C.byref(scratch),
+                                                                      _stream()), "transformer_block_bwd_options",
+                       45 - bool(options.qk_norm) - 3 * (options.window > 0) + (options.codes_w1 is not None))
         return
     _check(_lib.load().b200_transformer_block_bwd(C.byref(block), _p(x), _p(dx), C.byref(grads), C.byref(scratch), _stream()),
            "transformer_block_bwd", 45)
@@ -471,7 +487,7 @@ def qk_norm_rope(num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta, se
     op = "qk_norm_rope"
     _sizes(op, num_tokens, num_q_heads, num_kv_heads, head_dim, theta)
     dev, nq, nk = _here(op, X_q), num_tokens * num_q_heads * head_dim, num_tokens * num_kv_heads * head_dim
-    _check(_lib.load().b200_qk_norm_rope(
+    _check_counted(_lib.load().b200_qk_norm_rope(
         DT_BF16, num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta, _ptr(op, "seq_positions", seq_positions, num_tokens, _I32, dev),
         _ptr(op, "q_weight", q_weight, head_dim, _BF, dev, True), _ptr(op, "k_weight", k_weight, head_dim, _BF, dev, True),
         _ptr(op, "X_q", X_q, nq, _BF, dev), _ptr(op, "X_k", X_k, nk, _BF, dev), _ptr(op, "out_q", out_q, nq, _BF, dev),
@@ -489,14 +505,14 @@ def qk_norm_rope_bwd(num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta
     op = "qk_norm_rope_bwd"
     _sizes(op, num_tokens, num_q_heads, num_kv_heads, head_dim, theta)
     dev, nq, nk = _here(op, X_q), num_tokens * num_q_heads * head_dim, num_tokens * num_kv_heads * head_dim
-    _check(_lib.load().b200_qk_norm_rope_bwd(
+    _check_counted(_lib.load().b200_qk_norm_rope_bwd(
         DT_BF16, DT_BF16, num_tokens, num_q_heads, num_kv_heads, head_dim, eps, theta,
         _ptr(op, "seq_positions", seq_positions, num_tokens, _I32, dev), _ptr(op, "q_weight", q_weight, head_dim, _BF, dev, True),
         _ptr(op, "k_weight", k_weight, head_dim, _BF, dev, True), _ptr(op, "X_q", X_q, nq, _BF, dev), _ptr(op, "X_k", X_k, nk, _BF, dev),
         _ptr(op, "d_out_q", d_out_q, nq, _BF, dev), _ptr(op, "d_out_k", d_out_k, nk, _BF, dev), _ptr(op, "dX_q", dX_q, nq, _BF, dev),
         _ptr(op, "dX_k", dX_k, nk, _BF, dev), _ptr(op, "dq_weight", dq_weight, head_dim, _BF, dev, True),
         _ptr(op, "dk_weight", dk_weight, head_dim, _BF, dev, True), 1 if accumulate else 0, 0 if workspace is None else workspace.numel(),
-        _ptr(op, "workspace", workspace, 0, _U8, dev), _raw_stream(dev)), op, 1 if dq_weight is None and dk_weight is None else 2)
+        _ptr(op, "workspace", workspace, 0, _U8, dev), _raw_stream(dev)), op)
 
 
 # ---- attention with a sliding window and sink tokens ---------------------------------------------------------------------
@@ -529,7 +545,7 @@ def attention_window_fwd(q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_
     op = "attention_window_fwd"
     dev, host, args, _, _ = _window_args(op, q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v,
                                          x_attn_out, softmax_lse, window, num_sinks)
-    _check(_lib.load().b200_attention_window_fwd(*args, window, num_sinks, _raw_stream(dev)), op, -(-len(q_lens) // 48))
+    _check_counted(_lib.load().b200_attention_window_fwd(*args, window, num_sinks, _raw_stream(dev)), op)
 
 
 def attention_window_bwd(q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v, x_attn_out,
@@ -538,10 +554,10 @@ def attention_window_bwd(q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_
     op = "attention_window_bwd"
     dev, host, args, nq, nk = _window_args(op, q_offsets, q_lens, k_offsets, k_lens, num_q_heads, num_kv_heads, head_dim, x_q, x_k, x_v,
                                            x_attn_out, softmax_lse, window, num_sinks)
-    _check(_lib.load().b200_attention_window_bwd(
+    _check_counted(_lib.load().b200_attention_window_bwd(
         *args, _ptr(op, "dx_out", dx_out, nq, _BF, dev), _ptr(op, "dx_q", dx_q, nq, _BF, dev), _ptr(op, "dx_k", dx_k, nk, _BF, dev),
         _ptr(op, "dx_v", dx_v, nk, _BF, dev), window, num_sinks, 0 if workspace is None else workspace.numel(),
-        _ptr(op, "workspace", workspace, 0, _U8, dev), _raw_stream(dev)), op, 2 * -(-len(q_lens) // 48))
+        _ptr(op, "workspace", workspace, 0, _U8, dev), _raw_stream(dev)), op)
 
 
 # ---- SwiGLU activations held in 8 bits --------------------------------------------------------------------------------------
@@ -561,23 +577,23 @@ def swiglu_act8(n_rows, n_cols, x_w1, x_w3, out, codes_w1, scales_w1, codes_w3, 
     [n_rows][ceil(n_cols / 32)]."""
     op = "swiglu_act8"
     dev, n, held = _act8_args(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3)
-    _check(_lib.load().b200_swiglu_act8(DT_BF16, n_rows, n_cols, _ptr(op, "x_w1", x_w1, n, _BF, dev), _ptr(op, "x_w3", x_w3, n, _BF, dev),
-                                        _ptr(op, "out", out, n, _BF, dev, True), *held, _raw_stream(dev)), op)
+    _check_counted(_lib.load().b200_swiglu_act8(DT_BF16, n_rows, n_cols, _ptr(op, "x_w1", x_w1, n, _BF, dev), _ptr(op, "x_w3", x_w3, n, _BF, dev),
+                                                _ptr(op, "out", out, n, _BF, dev, True), *held, _raw_stream(dev)), op)
 
 
 def swiglu_recompute_act8(n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, x_w1=None, x_w3=None, out=None):
     """The held x_w1, x_w3 and out = silu(x_w1) * x_w3 of them, each when given."""
     op = "swiglu_recompute_act8"
     dev, n, held = _act8_args(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3)
-    _check(_lib.load().b200_swiglu_recompute_act8(DT_BF16, n_rows, n_cols, *held, _ptr(op, "x_w1", x_w1, n, _BF, dev, True),
-                                                  _ptr(op, "x_w3", x_w3, n, _BF, dev, True), _ptr(op, "out", out, n, _BF, dev, True),
-                                                  _raw_stream(dev)), op)
+    _check_counted(_lib.load().b200_swiglu_recompute_act8(DT_BF16, n_rows, n_cols, *held, _ptr(op, "x_w1", x_w1, n, _BF, dev, True),
+                                                          _ptr(op, "x_w3", x_w3, n, _BF, dev, True), _ptr(op, "out", out, n, _BF, dev, True),
+                                                          _raw_stream(dev)), op)
 
 
 def swiglu_bwd_x_act8(n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3, upstream_dX, dX_w1, dX_w3, out=None):
     """swiglu_bwd_x on the held values; out, when given, receives silu(x_w1) * x_w3 of them."""
     op = "swiglu_bwd_x_act8"
     dev, n, held = _act8_args(op, n_rows, n_cols, codes_w1, scales_w1, codes_w3, scales_w3)
-    _check(_lib.load().b200_swiglu_bwd_x_act8(DT_BF16, n_rows, n_cols, *held, _ptr(op, "upstream_dX", upstream_dX, n, _BF, dev),
-                                              _ptr(op, "dX_w1", dX_w1, n, _BF, dev), _ptr(op, "dX_w3", dX_w3, n, _BF, dev),
-                                              _ptr(op, "out", out, n, _BF, dev, True), _raw_stream(dev)), op)
+    _check_counted(_lib.load().b200_swiglu_bwd_x_act8(DT_BF16, n_rows, n_cols, *held, _ptr(op, "upstream_dX", upstream_dX, n, _BF, dev),
+                                                      _ptr(op, "dX_w1", dX_w1, n, _BF, dev), _ptr(op, "dX_w3", dX_w3, n, _BF, dev),
+                                                      _ptr(op, "out", out, n, _BF, dev, True), _raw_stream(dev)), op)
