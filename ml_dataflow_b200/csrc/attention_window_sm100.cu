@@ -1153,7 +1153,7 @@ struct KeyWalk {
   int t0, t1, tiles, chunk, chunks;
 };
 constexpr int MIN_CHUNK = 8;         // tiles of such a unit: at least this many, and as many as a block's window spans
-constexpr int MAX_SPLIT_UNITS = 148;   // units that the heads of a small batch are split into, at most
+constexpr int MAX_SPLIT_UNITS = 148;   // units that the heads of a small batch are split into: one per SM, at most so many (the workspace holds them)
 constexpr int MAX_SPLIT_SINKS = 1024;  // more sinks than this fill the GPU with blocks of their own: their units walk every tile
 __host__ __device__ inline KeyWalk key_walk(int Tq, int Tk, int kb, int window, int sinks, bool split = true) {
   KeyWalk w;
@@ -1748,7 +1748,8 @@ int sm100_bwd(const Call &c) {
                                   [&](int s) { return blocks_seen(c, c.k_len[s], c.q_len[s]); });
     if (p.main_units == 0) continue;
     // as many units as there are SMs, if the heads of a group give them
-    p.parts = p.main_units < MAX_SPLIT_UNITS ? MAX_SPLIT_UNITS / p.main_units : 1;
+    const int wanted = d.sms < MAX_SPLIT_UNITS ? d.sms : MAX_SPLIT_UNITS;
+    p.parts = p.main_units < wanted ? wanted / p.main_units : 1;
     if (p.parts > p.group) p.parts = p.group;
     p.slot_rows = p.parts > 1 ? TILE : slot_rows(c.sinks);
     int slots = 0, blocks = 0;

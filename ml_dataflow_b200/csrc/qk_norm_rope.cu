@@ -286,13 +286,13 @@ int qkn_lanes(int head_dim) {
 
 // A warp takes whole tokens as long as these alone give every SM 16 warps (backward: 4; its blocks' shares of the weight gradients have to
 // be added up); below that every round of heads gets a warp, so that few tokens spread over the GPU.
-constexpr int QKN_SPREAD_FWD = 148 * 16, QKN_SPREAD_BWD = 148 * 4;
-bool qkn_spread(int tokens, bool bwd) { return tokens < (bwd ? QKN_SPREAD_BWD : QKN_SPREAD_FWD); }
+int qkn_border(bool bwd, int sms) { return sms * (bwd ? 4 : 16); }
+bool qkn_spread(int tokens, bool bwd, int sms) { return tokens < qkn_border(bwd, sms); }
 
-int qkn_blocks(int tokens, int q_heads, int heads, int head_dim, bool bwd) {
+int qkn_blocks(int tokens, int q_heads, int heads, int head_dim, bool bwd, int sms) {
   const int round = 32 / qkn_lanes(head_dim) * qkn::BATCH, rounds = (q_heads + round - 1) / round + (heads - q_heads + round - 1) / round;
-  if (qkn_spread(tokens, bwd)) return (int)(((int64_t)tokens * rounds + qkn::WARPS - 1) / qkn::WARPS);
-  const int want = (tokens - 1) / qkn::WARPS + 1, most = qkn_sms() * (bwd ? qkn::BWD_BLOCKS : qkn::FWD_BLOCKS);
+  if (qkn_spread(tokens, bwd, sms)) return (int)(((int64_t)tokens * rounds + qkn::WARPS - 1) / qkn::WARPS);
+  const int want = (tokens - 1) / qkn::WARPS + 1, most = sms * (bwd ? qkn::BWD_BLOCKS : qkn::FWD_BLOCKS);
   return want < most ? want : most;
 }
 
@@ -367,16 +367,17 @@ extern "C" int b200_qk_norm_rope(int fwd_dt, int num_tokens, int num_q_heads, in
                  X_q, X_k, out_q, out_k))
     return -1;
   if (num_tokens == 0) return 0;
-  p.spread = qkn_spread(num_tokens, false);
-  return qkn_launch<false>("qk_norm_rope", p, qkn_blocks(num_tokens, p.q_heads, p.heads, head_dim, false), (cudaStream_t)stream);
+  const int sms = qkn_sms();
+  p.spread = qkn_spread(num_tokens, false, sms);
+  return qkn_launch<false>("qk_norm_rope", p, qkn_blocks(num_tokens, p.q_heads, p.heads, head_dim, false, sms), (cudaStream_t)stream);
 }
 
 extern "C" uint64_t b200_qk_norm_rope_bwd_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, int head_dim) {
   if (num_tokens <= 0 || num_q_heads < 1 || num_kv_heads < 0 || head_dim < 8 || head_dim % 8 || head_dim > qkn::MAX_HEAD_DIM) return 0;
   // enough for every smaller number of tokens too: the most blocks may run just below the border between the two layouts
-  const int below = num_tokens < QKN_SPREAD_BWD ? num_tokens : QKN_SPREAD_BWD - 1, heads = num_q_heads + num_kv_heads;
-  const int a = qkn_blocks(num_tokens, num_q_heads, heads, head_dim, true),
-            b = qkn_blocks(below, num_q_heads, heads, head_dim, true);
+  const int sms = qkn_sms(), border = qkn_border(true, sms), below = num_tokens < border ? num_tokens : border - 1, heads = num_q_heads + num_kv_heads;
+  const int a = qkn_blocks(num_tokens, num_q_heads, heads, head_dim, true, sms),
+            b = qkn_blocks(below, num_q_heads, heads, head_dim, true, sms);
   return (uint64_t)(a > b ? a : b) * 2 * head_dim * sizeof(float);
 }
 
@@ -400,8 +401,9 @@ extern "C" int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int
   }
   B200_REQUIRE(d_out_q && (num_kv_heads == 0 || d_out_k) && b200_aligned16(d_out_q) && b200_aligned16(d_out_k),
                "qk_norm_rope_bwd: the upstream gradients must be given and 16-byte aligned");
-  p.spread = qkn_spread(num_tokens, true);
-  const int blocks = qkn_blocks(num_tokens, p.q_heads, p.heads, head_dim, true);
+  const int sms = qkn_sms();
+  p.spread = qkn_spread(num_tokens, true, sms);
+  const int blocks = qkn_blocks(num_tokens, p.q_heads, p.heads, head_dim, true, sms);
   if (want_dw) {
     const uint64_t need = (uint64_t)blocks * 2 * head_dim * sizeof(float);
     B200_REQUIRE(workspace && b200_aligned16(workspace) && workspace_bytes >= need,
