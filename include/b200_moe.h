@@ -856,7 +856,8 @@ int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int num_q_head
  *
  * Head sizes 64 and 128 run on the tensor cores (csrc/attention_window_sm100.cu; sequences with few queries, up to 32 rows of a group, in
  * csrc/attention_window_few.cu), the others on the fp32 units. All sums have a fixed order: two runs give the same bits (how keys are split over
- * the GPU follows the batch's lengths: the same sequence beside others may differ in the last bits). Rounding as in
+ * the GPU follows the batch's lengths and how many clusters of CTAs the device seats at once: the same sequence beside others, or on a GPU with
+ * its SMs grouped otherwise, may differ in the last bits). Rounding as in
  * b200_attention_fwd / _bwd, but dS is formed from the fp32 probabilities; delta is formed from x_attn_out as it is stored, in bf16. A
  * value of infinity or NaN reaches the queries of the 128-row tiles that see it. A wait inside the kernels that runs out raises the word
  * that b200_attention_status reads. As with the other entry points, the first call on a device comes before any stream capture.

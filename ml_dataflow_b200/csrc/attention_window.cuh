@@ -62,6 +62,31 @@ int next_sequences(SeqTable &t, int *next, const Call &c, F units_of, G steps_of
   return t.first[t.n];
 }
 
+// Clusters of `size` CTAs that the current device seats at once, asked for on first use and kept in *known; 0 where it cannot tell. A cluster lies
+// within one GPC: here 15 of eight and 33 of four CTAs that fill an SM, where 148 SMs would hold 18 and 37. The kernel's shared memory has been allowed.
+template <typename K>
+int cluster_seats(K kernel, int threads, size_t smem, int size, int *known) {
+  if (*known == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)size);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    *known = n > 0 ? n : -1;
+  }
+  return *known > 0 ? *known : 0;
+}
+
 // attention_window_sm100.cu: tensor-core kernels for head sizes 64 and 128
 bool sm100_supported(int head_dim);
 int sm100_fwd(const Call &c);

@@ -3,8 +3,9 @@
 // Such a call reads every visible key and value once and computes next to nothing: memory bounds it, and, in small batches, latency. The
 // query heads of a group are the rows of one 16-row tile, so K and V are read once for all of them. A unit is such a tile of one
 // sequence and key/value head; its visible keys - the sinks, then the window - are numbered through and cut into blocks of 64, which the
-// CTAs of a cluster take in turn. There are as many CTAs per unit (1, 2, 4 or 8) as every SM can hold two of at once (32 sequences of up
-// to 4100 visible keys, 128 units: 2 CTAs each 37 us, 4 each 44 to 49); they join their partial sums through each other's shared memory, so
+// CTAs of a cluster take in turn. There are as many CTAs per unit (1, 2, 4 or 8) as the device seats clusters of at once (32 sequences of up
+// to 4100 visible keys, 128 units: 2 CTAs each 37 us, 4 each 44 to 49; head size 128, 4100 keys: 33 units are all seated with 8, 15 us, 4 each take
+// 20; 34 units are not, 23 us against 20; 71 units with 4 and with 2 28 and 35, 72 units 39 and 34); they join their partial sums through each other's shared memory, so
 // that a call is one launch and needs no workspace.
 //
 // A CTA: 4 warps, 16 keys of a block each, three blocks of K and V in flight (cp.async, 96 KB at head size 128, two CTAs per SM). Products
@@ -317,8 +318,9 @@ using namespace b200;
 namespace {
 
 template <int HD>
-int launch_few(const window::FewParams &p, int units, cudaStream_t s) {
+int launch_few(window::FewParams &p, int units, int64_t most, cudaStream_t s) {
   static bool done[MAX_DEVICES];
+  static int known[MAX_DEVICES][window::MAX_CLUSTER + 1];
   int dev = -1;
   B200_CUDA(cudaGetDevice(&dev));
   B200_REQUIRE(dev >= 0 && dev < MAX_DEVICES, "attention_window: device ordinal %d is out of range", dev);
@@ -327,6 +329,10 @@ int launch_few(const window::FewParams &p, int units, cudaStream_t s) {
     B200_CUDA(cudaFuncSetAttribute(window::window_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     done[dev] = true;
   }
+  p.cluster = 1;
+  while (p.cluster < window::MAX_CLUSTER && (int64_t)p.cluster * window::KEYS < most &&
+         units <= window::cluster_seats(window::window_few_kernel<HD>, window::FEW_THREADS, smem, 2 * p.cluster, &known[dev][2 * p.cluster]))
+    p.cluster *= 2;
   B200_CUDA(b200_launch_overlapped(window::window_few_kernel<HD>, dim3((unsigned)(units * p.cluster)), dim3(window::FEW_THREADS), smem, s,
                                    (unsigned)p.cluster, p));
   B200_CHECK_LAUNCH("attention_window_fwd (few queries)");
@@ -372,9 +378,7 @@ int few_fwd(const Call &c) {
     }
     if (p.n == 0) return 0;
     const int units = p.first[p.n];
-    p.cluster = 1;
-    while (p.cluster < MAX_CLUSTER && units * p.cluster <= 148 && (int64_t)p.cluster * KEYS < most) p.cluster *= 2;
-    if (c.head_dim == 128 ? launch_few<128>(p, units, c.stream) : launch_few<64>(p, units, c.stream)) return -1;
+    if (c.head_dim == 128 ? launch_few<128>(p, units, most, c.stream) : launch_few<64>(p, units, most, c.stream)) return -1;
   }
   return 0;
 }

@@ -1628,11 +1628,15 @@ void deal(window::Schedule *s, int sequences, int units, int ctas, F cost, G nex
 }
 
 template <int HD, int WALK>
-int launch_fwd(const window::FwdParams &p, const Device &d, cudaStream_t s) {
+int allow_fwd(const Device &d) {
   static bool done[MAX_DEVICES];
+  return allow_smem(window::window_fwd_kernel<HD, WALK>, window::FwdShape<HD>::smem, &done[d.dev]);
+}
+template <int HD, int WALK>
+int launch_fwd(const window::FwdParams &p, const Device &d, cudaStream_t s) {
   constexpr size_t smem = window::FwdShape<HD>::smem;
   static_assert(smem >= 1024 + 2 * window::TILE * (HD + 2 + window::MAX_SHARERS) * sizeof(float), "the parts of a shared unit");
-  if (allow_smem(window::window_fwd_kernel<HD, WALK>, smem, &done[d.dev])) return -1;
+  if (allow_fwd<HD, WALK>(d)) return -1;
   const int ctas = p.units * p.cluster;
   B200_CUDA(b200_launch_overlapped(window::window_fwd_kernel<HD, WALK>, dim3(ctas < d.sms ? ctas : d.sms), dim3(window::FWD_THREADS), smem, s,
                                    (unsigned)p.cluster, p));
@@ -1673,13 +1677,19 @@ int blocks_seen(const window::Call &c, int Tk, int rows) {
   return (int)(((span < rows ? span : rows) + window::TILE - 1) / window::TILE);
 }
 
-// CTAs that share a pair: joining their parts takes 6 to 8 us, a block that one walks 1.4 (half a pair) or 1.9. Measured at head size 128, in halves
-// and with 2, 4, 8 CTAs a pair: 16 pairs of 6 blocks 14, 19, 16 us, of 8 17, 21, 16, of 24 39, 37, 24; 8 pairs of 16 28, 29, 19, 17; 56 pairs of 16
-// 30, 31, of 24 41, 39. (16 pairs with 8, 28 to 47: not all clusters of eight find a place at once.)
-int sharers(int pairs, int blocks, int sms) {
-  if (pairs * 8 <= sms / 2 && blocks >= 16) return 8;
-  if (pairs * 4 <= sms && blocks >= 10) return 4;
-  return pairs * 2 <= sms && blocks >= 22 ? 2 : 1;
+// CTAs that share a pair, as long as all clusters have a seat at once: joining their parts takes 6 to 8 us, a block that one walks 1.4 (half a pair) or
+// 1.9. Measured at head size 128, in halves and with 2, 4, 8 CTAs a pair: 9 pairs of 10 blocks 19, 23, 17, 17 us, of 16 27, 28, 20, 17; 33 pairs of 16
+// 28, 30, 22, of 24 38, 37, 25; 74 pairs of 16 29, 31, of 24 40, 39, of 48 73, 61. Without a seat for every cluster: 16 pairs of 24 with 4 and with 8
+// 23, 35; 34 pairs of 10, in halves and with 4, 19, 33, of 48, with 2 and with 4, 59, 67. Head size 64: the same borders.
+template <int HD>
+int sharers(int pairs, int blocks, int dev) {
+  static int known[MAX_DEVICES][window::MAX_SHARERS + 1];
+  for (int size = window::MAX_SHARERS; size > 1; size /= 2)
+    if (blocks >= (size == 8 ? 16 : size == 4 ? 10 : 22) &&
+        pairs <= window::cluster_seats(window::window_fwd_kernel<HD, window::WALK_SHARED>, window::FWD_THREADS, window::FwdShape<HD>::smem, size,
+                                       &known[dev][size]))
+      return size;
+  return 1;
 }
 
 int slot_rows(int sinks) { return sinks < window::TILE ? sinks : window::TILE; }
@@ -1814,7 +1824,9 @@ int sm100_fwd(const Call &c) {
     // its short ones, and two halves take longer than a pair (no window: 246 -> 250 us).
     const int last = p.units % d.sms, halves = last < d.sms - last ? last : d.sms - last;
     const bool ramp = p.units > d.sms && c.window > p.seqs.Tk[0] / 2;
-    p.cluster = sharers(p.units, blocks_seen(c, p.seqs.Tk[0], p.seqs.Tk[0]), d.sms);
+    const int blocks = blocks_seen(c, p.seqs.Tk[0], p.seqs.Tk[0]);
+    if (c.head_dim == 128 ? allow_fwd<128, WALK_SHARED>(d) : allow_fwd<64, WALK_SHARED>(d)) return -1;
+    p.cluster = c.head_dim == 128 ? sharers<128>(p.units, blocks, d.dev) : sharers<64>(p.units, blocks, d.dev);
     const int split = ramp || p.cluster > 1 ? 0 : halves;
     p.whole = p.units - split;
     p.units += split;
