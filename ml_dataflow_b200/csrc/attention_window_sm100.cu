@@ -777,8 +777,9 @@ teardown:
 // group are split over units the same way (45 - 391 keys, 8 heads on one: 30 -> 13 us).
 //
 // Rounding: P and dS to bf16 once each (dS from the fp32 P), accumulators fp32, one rounding per output.
-// delta is formed from O as the caller holds it, rounded to bf16: a query with few keys loses up to 2^-9 of |dO| |O| against a delta of the
-// fp32 output, which the interface does not carry; the tests bound it.
+// delta is formed from O as the caller holds it: rounded to bf16, off by up to 2^-8 of |O|, after a sum over probabilities that were rounded too. Against
+// a delta of the exact output a dS is off by up to P times 2^-8 of |dO| |O| (and of |dO| sum P |V|), which shows where a query has few keys. The
+// interface does not carry the fp32 output. tests/test_gpu_attention_window_gradients.py holds dQ and dK to the exact gradient within these bounds.
 // What bounds both: shared memory. A step of dK, dV moves 384 KB through it (four products of 64, P and dS, Q and dO that arrive; 3070 cycles at
 // 128 bytes each) and takes 3400; one of dQ 224 KB (1800 cycles; its third product reads K only) and takes about 2500.
 // Measured with 16 query heads on 4 of 128 and 8192 tokens: window 1024, 4 sinks dQ 120 us, dK and dV 175 us, join 4 us; no window 825 us
