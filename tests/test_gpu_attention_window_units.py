@@ -15,7 +15,7 @@ CASES = [
     ([900, 1500, 700], [900, 1500, 1000], 15, 5, 128, 200, 0),  # an odd group, dealt out
     ([1500, 700, 300], [5000, 700, 900], 16, 4, 128, 900, 4),   # chunks of prompts
     ([130 + 7 * i for i in range(60)], [130 + 9 * i for i in range(60)], 8, 2, 128, 100, 2),  # more sequences than one launch takes
-    ([100 + 53 * i % 1400 for i in range(24)], [100 + 53 * i % 1400 for i in range(24)], 8, 2, 64, 256, 1),  # too many kinds of units to deal out
+    ([50 + 37 * i for i in range(40)], [50 + 37 * i for i in range(40)], 8, 2, 64, 1024, 1),  # too many kinds of units to deal out: rounds
     ([1, 900, 2, 1200], [500, 900, 700, 1300], 24, 4, 128, 333, 5),  # two forms in one call
 ]
 
