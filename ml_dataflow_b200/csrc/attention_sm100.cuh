@@ -1,5 +1,5 @@
-// What the fused attention kernels share: shared-memory accesses, the exponential, tensor maps of row-major bf16 tensors, the
-// status word.
+// What the fused attention kernels share: shared-memory accesses, the exponential, the driver's call that makes tensor maps, the status
+// word.
 #pragma once
 
 #include <cuda.h>
@@ -44,7 +44,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-EncodeTiledFn encode_fn() {
+inline EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
   if (!fn) {
     void *sym = nullptr;
@@ -55,23 +55,6 @@ EncodeTiledFn encode_fn() {
     fn = reinterpret_cast<EncodeTiledFn>(sym);
   }
   return fn;
-}
-
-// bf16 [rows][cols] with a row pitch of `cols` elements; boxes of 64 columns x 128 rows, 128-byte swizzle, rows past
-// the end read as zeros
-int rows_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t cols) {
-  EncodeTiledFn fn = encode_fn();
-  B200_REQUIRE(fn != nullptr, "attention: cuTensorMapEncodeTiled is not available from this driver");
-  B200_REQUIRE(b200_aligned16(base) && (cols * 2) % 16 == 0, "attention: tensors must be 16-byte aligned with a 16-byte row pitch");
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {cols * 2};
-  cuuint32_t box[2] = {64, 128};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  B200_REQUIRE(r == CUDA_SUCCESS, "attention: cuTensorMapEncodeTiled failed with code %d", (int)r);
-  return 0;
 }
 
 }  // namespace
