@@ -827,7 +827,8 @@ int b200_attention_status(int *status_out);
  * [num_tokens][num_kv_heads * head_dim] (num_kv_heads may be 0, the key pointers are then ignored). q_weight, k_weight:
  * [head_dim], shared by the query (key) heads; NULL means ones ("QK Norm Weight Type: none"). One rounding. out_q / out_k
  * may be X_q / X_k themselves where no backward follows. head_dim a multiple of 8 up to 256, tensors 16-byte aligned,
- * bf16 only. It stands where the reference submits rms_norm_noscale per head and rope (no fused counterpart there).
+ * bf16 only. The sum of squares is formed in fp32; with eps = 0 a row of zeros is divided by zero. It stands where the
+ * reference submits rms_norm_noscale per head and rope (no fused counterpart there).
  *
  * Backward: dX_q, dX_k are overwritten (and may be d_out_q / d_out_k themselves). dq_weight, dk_weight [head_dim], either
  * may be NULL, not the same array: accumulate != 0 adds to them, 0 writes them. Their sums run in a fixed order (fp32 shares of the blocks in
@@ -858,8 +859,9 @@ int b200_qk_norm_rope_bwd(int fwd_dt, int bwd_dt, int num_tokens, int num_q_head
  * csrc/attention_window_few.cu), the others on the fp32 units. All sums have a fixed order: two runs give the same bits (how keys are split over
  * the GPU follows the batch's lengths and how many clusters of CTAs the device seats at once: the same sequence beside others, or on a GPU with
  * its SMs grouped otherwise, may differ in the last bits). Rounding as in
- * b200_attention_fwd / _bwd, but dS is formed from the fp32 probabilities; delta is formed from x_attn_out as it is stored, in bf16. A
- * value of infinity or NaN reaches the queries of the 128-row tiles that see it. A wait inside the kernels that runs out raises the word
+ * b200_attention_fwd / _bwd, but dS is formed from the fp32 probabilities; delta is formed from x_attn_out as it is stored, in bf16. An
+ * infinity or NaN among the keys and values that some query of the sequence sees may reach every query of a 128-row tile that sees a key of the same
+ * block of 128 keys (and one among queries and upstream gradients the keys of such blocks). A wait inside the kernels that runs out raises the word
  * that b200_attention_status reads. As with the other entry points, the first call on a device comes before any stream capture.
  *
  * The forward needs no workspace. The backward's is sized by b200_attention_window_workspace_bytes(max_num_seqs, ...,
